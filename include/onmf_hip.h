@@ -32,7 +32,7 @@ extern "C" {
 #define ONMF_ERR_NOMEM (-3)     /* scratch allocation failed                             */
 #define ONMF_ERR_TIMEOUT (-4)   /* a bounded device-side wait gave up and no retry was possible */
 
-#define ONMF_ABI_VERSION 3
+#define ONMF_ABI_VERSION 4
 
 /* coder_mode of onmf_sparse_code */
 #define ONMF_CODER_DAMPED 0 /* reference step 1/(sqrt(i+10)(G_kk+1)), src/onmf.py:257       */
@@ -340,6 +340,71 @@ int onmf_ndl_accumulate_edges(onmf_ctx* ctx, int n_nodes, int k, int n_patches, 
 int onmf_numpy_set_jump_table(onmf_ctx* ctx, const uint32_t* table_host, int rows, long long chunk_words);
 int onmf_numpy_rand(onmf_ctx* ctx, const uint32_t* key, int pos, size_t n, float* out, uint32_t* key_out,
                     int* pos_out, void* stream);
+
+/*
+ * A dictionary held in 4 bits (no counterpart in the reference, whose dictionaries are float64 arrays).  The
+ * features of an atom are taken in groups of `group` = 32, 64 or 128 that share a scale s (bfloat16) and a whole
+ * number z; an entry stands for s (q + z) with q in 0..15 and differs from the entry of W by at most s / 2.
+ *   codes   r rows of ceil(d / group) * group / 2 bytes, aligned to 16 bytes: entry j of an eight-feature word is
+ *           nibble (j >> 1) + 4 (j & 1); the padding behind feature d is zero nibbles
+ *   scales  int32[r * ceil(d / group)]: the bits of s in the upper half, z (signed) in the lower
+ * s = max((hi - lo) / 15, max|w| / 255) of the group, rounded up to bfloat16 (14 instead of 15 where rounding both
+ * ends to the grid would need a seventeenth level); a group whose scale would be below 2^-126 reads as zeros, one
+ * with a NaN or an infinity reads as NaNs.
+ * Products with float32 or bfloat16 columns (x_type / h_type: ONMF_TYPE_*), float32 results, all sums in float32:
+ *   correlate  C = W^T X (r x b): what coding starts from (src/onmf.py:243)
+ *   product    R = W H (d x b): np.dot(self.W, code), image_reconstruction.py:352, :385
+ * Each is the other's gradient: dL/dX = W dL/dC, dL/dH = W^T dL/dR.
+ * A column with a NaN or an infinity (or a float32 within 2^-8 of the largest one) has NaNs or infinities in its
+ * result and touches no other column.  ws: at least onmf_dict4_workspace(which, d, r, b, group) bytes of device
+ * memory, in use until the call's work on `stream` is done (so calls on different streams take different ones).
+ * d <= 2^18.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
+ */
+#define ONMF_TYPE_F32 0
+#define ONMF_TYPE_BF16 1
+#define ONMF_DICT4_CORRELATE 0
+#define ONMF_DICT4_PRODUCT 1
+size_t onmf_dict4_workspace(int which, int d, int r, int b, int group);
+int onmf_dict4_pack(onmf_ctx* ctx, int d, int r, int group, const float* W, void* codes, int32_t* scales, void* stream);
+int onmf_dict4_unpack(onmf_ctx* ctx, int d, int r, int group, const void* codes, const int32_t* scales, float* W,
+                      void* stream);
+int onmf_dict4_correlate(onmf_ctx* ctx, int d, int r, int b, int group, const void* codes, const int32_t* scales,
+                         const void* X, int x_type, int ldx, float* C, void* ws, size_t ws_bytes, void* stream);
+int onmf_dict4_product(onmf_ctx* ctx, int d, int r, int b, int group, const void* codes, const int32_t* scales,
+                       const void* H, int h_type, int ldh, float* R, int ldr, void* ws, size_t ws_bytes, void* stream);
+/* onmf_sparse_code_each with a 4-bit dictionary: W^T X and W^T W from its codes. */
+int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, const float* X, int ldx, const void* codes,
+                                const int32_t* scales, const float* H0, uint64_t seed, float alpha, int sub_iter,
+                                float stopping_diff, int coder_mode, float* H, int32_t* sweeps_each, void* stream);
+
+/*
+ * Columns held in 8 bits (no counterpart in the reference): a minibatch X and its code H put away in a quarter of
+ * their room until the dictionary's update or gradient needs them.  128 consecutive columns of a row share a scale
+ * s = max|v| / 127 (float32); an entry stands for s q, q = rint(v / s), ties to even, decided exactly, and differs
+ * from v by at most s / 2.  A group whose scale would be below 2^-126 reads as zeros, one with a NaN or an infinity
+ * as NaNs.
+ *   codes   int8, d rows of ceil(n / 128) * 128, aligned to 16 bytes; the padding behind column n is zeros
+ *   scales  float32, d rows of ceil(n / 128)
+ * onmf_keep8            X (d x n, float32 or bfloat16) -> codes, scales
+ * onmf_keep8_expand     back to float32: all n columns (idx == NULL), or the b columns idx (device int64, a negative one
+ *                       counts from the end as in NumPy, one out of range reads NaN) - X[:, idx], src/onmf.py:214
+ * onmf_keep8_aggregate  onmf_aggregate's A_out and B_out (src/onmf.py:155-156) from a kept X (d x n) and H (r x n);
+ *                       in/out pointers may alias, A_in / B_in NULL means zeros
+ * onmf_keep8_gradient   dW (d x r) = W (H H^T) - X H^T, the gradient of 1/2 |X - W H|^2 to W; d, r <= 2^18
+ * Products inside a group add up exactly in int32, groups in float32, runs of groups and what follows in double.
+ * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, in use until the call's work on
+ * `stream` is done.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
+ */
+size_t onmf_keep8_workspace(int d, int r, int n, int gradient);
+int onmf_keep8(onmf_ctx* ctx, int d, int n, const void* X, int x_type, int ldx, int8_t* codes, float* scales, void* stream);
+int onmf_keep8_expand(onmf_ctx* ctx, int d, int n, const int8_t* codes, const float* scales, const int64_t* idx, int b,
+                      float* X, int ldx, void* stream);
+int onmf_keep8_aggregate(onmf_ctx* ctx, int d, int r, int n, const int8_t* x_codes, const float* x_scales,
+                         const int8_t* h_codes, const float* h_scales, double w, const float* A_in, const float* B_in,
+                         float* A_out, float* B_out, void* ws, size_t ws_bytes, void* stream);
+int onmf_keep8_gradient(onmf_ctx* ctx, int d, int r, int n, const float* W, const int8_t* x_codes, const float* x_scales,
+                        const int8_t* h_codes, const float* h_scales, float* dW, void* ws, size_t ws_bytes,
+                        void* stream);
 
 /* U[0,1) fill, the device stand-in for np.random.rand (src/onmf.py:190, :246). */
 int onmf_fill_uniform(onmf_ctx* ctx, float* out, size_t n, uint64_t seed, void* stream);

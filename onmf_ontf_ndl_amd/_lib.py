@@ -38,6 +38,10 @@ CNT_LARS_SLOTS_USED = 6
 CNT_SWEEPS_TOTAL = 7
 CNT_DEFERRED_REDONE = 8
 CNT_LAG3_REDONE = 9
+TYPE_F32 = 0
+TYPE_BF16 = 1
+DICT4_CORRELATE = 0
+DICT4_PRODUCT = 1
 NDL_GLAUBER = 0
 NDL_PIVOT = 1
 
@@ -99,6 +103,24 @@ SIGNATURES = {
     "onmf_numpy_set_jump_table": (C.c_int, [_ctx, C.c_void_p, C.c_int, C.c_longlong]),
     "onmf_numpy_rand": (C.c_int, [_ctx, C.c_void_p, C.c_int, C.c_size_t, _f, C.c_void_p, C.POINTER(C.c_int),
                                   C.c_void_p]),
+    "onmf_dict4_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "onmf_dict4_pack": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, _f, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "onmf_dict4_unpack": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, _f, C.c_void_p]),
+    "onmf_dict4_correlate": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_int, C.c_int, _f, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "onmf_dict4_product": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_int, C.c_int, _f, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "onmf_sparse_code_each_dict4": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, C.c_int, _f, C.c_int, C.c_void_p,
+                                              C.c_void_p, _f, C.c_uint64, C.c_float, C.c_int, C.c_float, C.c_int, _f,
+                                              C.c_void_p, C.c_void_p]),
+    "onmf_keep8_workspace": (C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "onmf_keep8": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, _f, C.c_void_p]),
+    "onmf_keep8_expand": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_void_p, _f, C.c_void_p, C.c_int, _f, C.c_int,
+                                    C.c_void_p]),
+    "onmf_keep8_aggregate": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, C.c_void_p, _f, C.c_void_p, _f, C.c_double,
+                                       _f, _f, _f, _f, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "onmf_keep8_gradient": (C.c_int, [_ctx, C.c_int, C.c_int, C.c_int, _f, C.c_void_p, _f, C.c_void_p, _f, _f,
+                                      C.c_void_p, C.c_size_t, C.c_void_p]),
     "onmf_fill_uniform": (C.c_int, [_ctx, _f, C.c_size_t, C.c_uint64, C.c_void_p]),
     "onmf_host_lambda_max": (C.c_double, [C.c_void_p, C.c_int]),
     "onmf_set_option": (C.c_int, [_ctx, C.c_int, C.c_int]),

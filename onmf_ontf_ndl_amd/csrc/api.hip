@@ -164,7 +164,8 @@ int onmf_destroy(onmf_ctx* c) {
     (void)hipDeviceSynchronize();
     DevBuf* bufs[] = {&c->slab, &c->cm, &c->gram, &c->hbuf[0], &c->hbuf[1], &c->stats, &c->small,
                       &c->qt, &c->sync, &c->idx, &c->dbuf, &c->slab_side, &c->screen, &c->ddelta, &c->slab_prep,
-                      &c->gstack, &c->rslab, &c->gram64, &c->cm64, &c->lars_ws, &c->lars_meta, &c->lars_overflow, &c->mt};
+                      &c->gstack, &c->rslab, &c->gram64, &c->cm64, &c->lars_ws, &c->lars_meta, &c->lars_overflow, &c->mt,
+                      &c->wdense};
     for (DevBuf* b : bufs)
         if (b->p) (void)hipFree(b->p);
     if (c->pinned) (void)hipHostFree(c->pinned);
@@ -1244,6 +1245,24 @@ int onmf_unfold3(onmf_ctx* c, int n0, int n1, int n2, const float* T, int mode, 
     return ONMF_OK;
 }
 
+// The sweeps of onmf_sparse_code_each from Gm = W^T W and Cm = W^T X.
+static int each_from_products(onmf_ctx* c, int r, int b, const float* Gm, const float* Cm, const float* H0, uint64_t seed,
+                              float alpha, int sub_iter, float stopping_diff, int coder_mode, float* H,
+                              int32_t* sweeps_each, hipStream_t s) {
+    const size_t rb = (size_t)r * b;
+    if (H0) {
+        if (H0 != H) HIP_TRY(c, hipMemcpyAsync(H, H0, rb * sizeof(float), hipMemcpyDeviceToDevice, s));
+    } else if (launch_fill_uniform(H, rb, seed, s) != ONMF_OK) {
+        return onmf_fail(c, ONMF_ERR_HIP, "sparse_code_each: fill launch failed");
+    }
+    if (sub_iter == 0) {
+        if (sweeps_each) HIP_TRY(c, hipMemsetAsync(sweeps_each, 0, (size_t)b * sizeof(int32_t), s));
+        return ONMF_OK;
+    }
+    EachStop es = {stopping_diff, sweeps_each};
+    return launch_sweep_each(c, r, b, Gm, Cm, H, alpha, coder_mode == ONMF_CODER_EXACT_CD, sub_iter, es, s);
+}
+
 int onmf_sparse_code_each(onmf_ctx* c, int d, int r, int b, const float* X, int ldx, const float* W,
                           const float* H0, uint64_t seed, float alpha, int sub_iter, float stopping_diff,
                           int coder_mode, float* H, int32_t* sweeps_each, void* stream) {
@@ -1261,17 +1280,30 @@ int onmf_sparse_code_each(onmf_ctx* c, int d, int r, int b, const float* X, int 
     // of every column in one launch
     ONMF_TRY(launch_gemm(c, true, true, r, r, d, W, r, W, r, 1.f, 0.f, nullptr, Gm, r, s));
     ONMF_TRY(launch_gemm(c, true, true, r, b, d, W, r, X, ldx, 1.f, 0.f, nullptr, Cm, b, s));
-    if (H0) {
-        if (H0 != H) HIP_TRY(c, hipMemcpyAsync(H, H0, rb * sizeof(float), hipMemcpyDeviceToDevice, s));
-    } else if (launch_fill_uniform(H, rb, seed, s) != ONMF_OK) {
-        return onmf_fail(c, ONMF_ERR_HIP, "sparse_code_each: fill launch failed");
-    }
-    if (sub_iter == 0) {
-        if (sweeps_each) HIP_TRY(c, hipMemsetAsync(sweeps_each, 0, (size_t)b * sizeof(int32_t), s));
-        return ONMF_OK;
-    }
-    EachStop es = {stopping_diff, sweeps_each};
-    return launch_sweep_each(c, r, b, Gm, Cm, H, alpha, coder_mode == ONMF_CODER_EXACT_CD, sub_iter, es, s);
+    return each_from_products(c, r, b, Gm, Cm, H0, seed, alpha, sub_iter, stopping_diff, coder_mode, H, sweeps_each, s);
+}
+
+int onmf_sparse_code_each_dict4(onmf_ctx* c, int d, int r, int b, int group, const float* X, int ldx, const void* codes,
+                                const int32_t* scales, const float* H0, uint64_t seed, float alpha, int sub_iter,
+                                float stopping_diff, int coder_mode, float* H, int32_t* sweeps_each, void* stream) {
+    if (!c) return ONMF_ERR_ARG;
+    if (d <= 0 || r <= 0 || b <= 0 || !X || !codes || !scales || !H || ldx < b || sub_iter < 0)
+        return onmf_fail(c, ONMF_ERR_ARG, "sparse_code_each_dict4: bad arguments (d=%d r=%d b=%d ldx=%d)", d, r, b, ldx);
+    hipStream_t s = (hipStream_t)stream;
+    ONMF_ENTER(c);
+    ONMF_TRY(onmf_reserve(c, c->gram, (size_t)r * r * sizeof(float), "Gm"));
+    ONMF_TRY(onmf_reserve(c, c->cm, (size_t)r * b * sizeof(float), "Cm"));
+    ONMF_TRY(onmf_reserve(c, c->wdense, (size_t)d * r * sizeof(float), "unpacked dictionary"));
+    const size_t ws = std::max(onmf_dict4_workspace(ONMF_DICT4_CORRELATE, d, r, b, group),
+                               onmf_dict4_workspace(ONMF_DICT4_CORRELATE, d, r, r, group));
+    ONMF_TRY(onmf_reserve(c, c->slab, ws, "split products"));
+    float* Gm = (float*)c->gram.p;
+    float* Cm = (float*)c->cm.p;
+    float* W = (float*)c->wdense.p;
+    ONMF_TRY(onmf_dict4_unpack(c, d, r, group, codes, scales, W, stream));
+    ONMF_TRY(onmf_dict4_correlate(c, d, r, r, group, codes, scales, W, ONMF_TYPE_F32, r, Gm, c->slab.p, c->slab.bytes, stream));
+    ONMF_TRY(onmf_dict4_correlate(c, d, r, b, group, codes, scales, X, ONMF_TYPE_F32, ldx, Cm, c->slab.p, c->slab.bytes, stream));
+    return each_from_products(c, r, b, Gm, Cm, H0, seed, alpha, sub_iter, stopping_diff, coder_mode, H, sweeps_each, s);
 }
 
 int onmf_sparse_code_lars(onmf_ctx* c, int d, int r, int b, const float* X, int ldx, const float* W, double alpha,

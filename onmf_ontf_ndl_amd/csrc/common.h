@@ -52,6 +52,7 @@ struct onmf_ctx {
     DevBuf qt;          // dictionary pass: Qt = A^T W^T  (r x d)
     DevBuf sync;        // dictionary pass: cross-workgroup slots + counters
     DevBuf idx;         // scatter scratch
+    DevBuf wdense;      // a 4-bit dictionary unpacked (d x r) for its Gram matrix
     std::vector<double> hstats;
     std::vector<float> hgram;
     void* pinned = nullptr;   // small pinned host staging

@@ -13,6 +13,7 @@ import warnings
 import numpy as np
 
 from . import _lib
+from .lowbit import GROUP8, GROUPS4, KeptColumns, PackedDictionary
 
 _engines = {}
 
@@ -330,7 +331,11 @@ class Engine:
     def sparse_code_each(self, X, W, H0=None, alpha=0.0, sub_iter=10, stopping_diff=0.01, seed=None,
                          mode=_lib.CODER_DAMPED, want_sweeps=False):
         """One independent solve per column, each with its own stopping test
-        (image_reconstruction.py:384 calls onmf.py:233-271 once per patch).  No host round trip."""
+        (image_reconstruction.py:384 calls onmf.py:233-271 once per patch).  No host round trip.
+        ``W`` may be a PackedDictionary."""
+        packed = isinstance(W, PackedDictionary)
+        if packed:
+            self._low(W, PackedDictionary, "sparse_code_each")
         d, b = X.shape
         r = W.shape[1]
         if W.shape[0] != d:
@@ -341,6 +346,13 @@ class Engine:
         sweeps = self.torch.empty(b, dtype=self.torch.int32, device=self.device) if want_sweeps else None
         if seed is None:
             seed = self.next_seed()
+        if packed:
+            rc = self.lib.onmf_sparse_code_each_dict4(self.ctx, d, r, b, W.group, _ptr(X), X.stride(0), _ptr(W.codes),
+                                                      _ptr(W.scales), _ptr(H0), C.c_uint64(seed), float(alpha),
+                                                      int(sub_iter), float(stopping_diff), int(mode), _ptr(H),
+                                                      _ptr(sweeps), self.stream())
+            _lib.check(rc, self.ctx, "onmf_sparse_code_each_dict4")
+            return (H, sweeps) if want_sweeps else H
         rc = self.lib.onmf_sparse_code_each(self.ctx, d, r, b, _ptr(X), X.stride(0), _ptr(W), _ptr(H0),
                                             C.c_uint64(seed), float(alpha), int(sub_iter),
                                             float(stopping_diff), int(mode), _ptr(H), _ptr(sweeps),
@@ -380,7 +392,9 @@ class Engine:
         return H, A1, B1, W1
 
     def patch_product(self, W, H):
-        """W @ H (image_reconstruction.py:352, :385)."""
+        """W @ H (image_reconstruction.py:352, :385); ``W`` may be a PackedDictionary."""
+        if isinstance(W, PackedDictionary):
+            return self.dict4_product(W, H)
         d, r = W.shape
         b = H.shape[1]
         R = self.empty(d, b)
@@ -435,6 +449,181 @@ class Engine:
                                           self.stream())
         _lib.check(rc, self.ctx, "onmf_surrogate_loss")
         return loss.value
+
+    # ------------------------------------------------------------------ dictionaries in 4 bits, columns in 8
+    def is_columns(self, a):
+        """A float32 or bfloat16 matrix on this GPU whose rows are contiguous: taken as it is by the products below."""
+        return isinstance(a, self.torch.Tensor) and a.device == self.device and a.dim() == 2 and \
+            a.dtype in (self.torch.float32, self.torch.bfloat16) and a.stride(1) == 1 and a.stride(0) >= a.shape[1]
+
+    def _columns(self, a, rows, what):
+        """(tensor, type, leading dimension) of a column operand."""
+        torch = self.torch
+        if not isinstance(a, torch.Tensor) or a.device != self.device:
+            raise ValueError("%s: the columns must be a tensor on %s" % (what, self.device))
+        if a.dim() != 2 or a.shape[1] == 0 or (rows is not None and a.shape[0] != rows) or a.shape[0] == 0:
+            raise ValueError("%s: the columns must be (%s, b), not %s"
+                             % (what, "d" if rows is None else rows, tuple(a.shape)))
+        if a.dtype is torch.float32:
+            kind = _lib.TYPE_F32
+        elif a.dtype is torch.bfloat16:
+            kind = _lib.TYPE_BF16
+        else:
+            raise ValueError("%s: the columns must be float32 or bfloat16, not %s" % (what, a.dtype))
+        b = a.shape[1]
+        ld = a.stride(0)
+        if (b > 1 and a.stride(1) != 1) or ld < b:         # a transposed, broadcast or reversed view
+            a = a.contiguous()
+            ld = b
+        return a, kind, max(ld, b)
+
+    def _low(self, a, kind, what):
+        if not isinstance(a, kind):
+            raise ValueError("%s needs a %s, not %s" % (what, kind.__name__, type(a).__name__))
+        if a.codes.device != self.device:
+            raise ValueError("%s: the %s is on %s, not on %s" % (what, kind.__name__, a.codes.device, self.device))
+        return a
+
+    def _matrix(self, a, shape, what):
+        if not isinstance(a, self.torch.Tensor) or a.device != self.device or a.dtype is not self.torch.float32 or \
+                tuple(a.shape) != shape or not a.is_contiguous():
+            raise ValueError("%s must be a contiguous float32 tensor of shape %s on %s" % (what, shape, self.device))
+        return a
+
+    def _workspace(self, nbytes):
+        """Device memory for one call, from torch's allocator on the current stream: calls on different streams and
+        captured graphs each get their own."""
+        if nbytes == 0:
+            return None, C.c_void_p(0)
+        t = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
+        return t, C.c_void_p(t.data_ptr())
+
+    def dict4_pack(self, W, group=64):
+        """W (d x r) in 4 bits with a scale and an offset for ``group`` = 32, 64 or 128 features of an atom."""
+        if int(group) not in GROUPS4:
+            raise ValueError("dict4_pack: a group is 32, 64 or 128 features, not %s" % (group,))
+        if not isinstance(W, self.torch.Tensor) or W.dim() != 2 or W.numel() == 0:
+            raise ValueError("dict4_pack: W must be a (d, r) tensor with entries")
+        d, r = W.shape
+        W = self._matrix(W, (d, r), "dict4_pack: W")
+        groups = -(-d // int(group))
+        codes = self.torch.empty(r, groups * int(group) // 2, dtype=self.torch.uint8, device=self.device)
+        scales = self.torch.empty(r, groups, dtype=self.torch.int32, device=self.device)
+        rc = self.lib.onmf_dict4_pack(self.ctx, d, r, int(group), _ptr(W), _ptr(codes), _ptr(scales), self.stream())
+        _lib.check(rc, self.ctx, "onmf_dict4_pack")
+        return PackedDictionary(codes, scales, d, int(group))
+
+    def dict4_unpack(self, P):
+        """The float32 matrix (d x r) that a 4-bit dictionary stands for."""
+        self._low(P, PackedDictionary, "dict4_unpack")
+        d, r = P.shape
+        W = self.empty(d, r)
+        rc = self.lib.onmf_dict4_unpack(self.ctx, d, r, P.group, _ptr(P.codes), _ptr(P.scales), _ptr(W), self.stream())
+        _lib.check(rc, self.ctx, "onmf_dict4_unpack")
+        return W
+
+    def dict4_correlate(self, P, X):
+        """W^T X (r x b, float32) with a 4-bit dictionary and float32 or bfloat16 columns: what coding starts from
+        (src/onmf.py:243), and the gradient of ``dict4_product`` to H."""
+        self._low(P, PackedDictionary, "dict4_correlate")
+        d, r = P.shape
+        X, kind, ld = self._columns(X, d, "dict4_correlate")
+        b = X.shape[1]
+        out = self.empty(r, b)
+        nbytes = self.lib.onmf_dict4_workspace(_lib.DICT4_CORRELATE, d, r, b, P.group)
+        ws, wp = self._workspace(nbytes)
+        rc = self.lib.onmf_dict4_correlate(self.ctx, d, r, b, P.group, P.codes.data_ptr(), P.scales.data_ptr(),
+                                           X.data_ptr(), kind, ld, out.data_ptr(), wp, nbytes, self.stream())
+        if rc:
+            _lib.check(rc, self.ctx, "onmf_dict4_correlate")
+        return out
+
+    def dict4_product(self, P, H):
+        """W H (d x b, float32) with a 4-bit dictionary and float32 or bfloat16 codes
+        (image_reconstruction.py:352, :385), and the gradient of ``dict4_correlate`` to X."""
+        self._low(P, PackedDictionary, "dict4_product")
+        d, r = P.shape
+        H, kind, ld = self._columns(H, r, "dict4_product")
+        b = H.shape[1]
+        out = self.empty(d, b)
+        nbytes = self.lib.onmf_dict4_workspace(_lib.DICT4_PRODUCT, d, r, b, P.group)
+        ws, wp = self._workspace(nbytes)
+        rc = self.lib.onmf_dict4_product(self.ctx, d, r, b, P.group, P.codes.data_ptr(), P.scales.data_ptr(),
+                                         H.data_ptr(), kind, ld, out.data_ptr(), b, wp, nbytes, self.stream())
+        if rc:
+            _lib.check(rc, self.ctx, "onmf_dict4_product")
+        return out
+
+    def keep8(self, X):
+        """X (d x n, float32 or bfloat16) put away in 8 bits with a scale for 128 columns of a row."""
+        X, kind, ld = self._columns(X, None, "keep8")
+        d, n = X.shape
+        groups = -(-n // GROUP8)
+        codes = self.torch.empty(d, groups * GROUP8, dtype=self.torch.int8, device=self.device)
+        scales = self.torch.empty(d, groups, dtype=self.torch.float32, device=self.device)
+        rc = self.lib.onmf_keep8(self.ctx, d, n, X.data_ptr(), kind, ld, codes.data_ptr(), scales.data_ptr(),
+                                 self.stream())
+        if rc:
+            _lib.check(rc, self.ctx, "onmf_keep8")
+        return KeptColumns(codes, scales, n)
+
+    def keep8_expand(self, K, idx=None):
+        """The float32 columns a store stands for: all (d x n), or those at ``idx`` (X[:, idx], src/onmf.py:214)."""
+        self._low(K, KeptColumns, "keep8_expand")
+        d, n = K.shape
+        if idx is None:
+            b, ip = n, C.c_void_p(0)
+        else:
+            idx = self.dev(idx, self.torch.int64)
+            if idx.dim() != 1 or idx.numel() == 0:
+                raise ValueError("keep8_expand: idx must be a vector with entries")
+            self._check_index(idx, n, "keep8_expand")
+            b, ip = idx.numel(), _ptr(idx)
+        out = self.empty(d, b)
+        rc = self.lib.onmf_keep8_expand(self.ctx, d, n, K.codes.data_ptr(), K.scales.data_ptr(), ip, b, out.data_ptr(), b,
+                                        self.stream())
+        if rc:
+            _lib.check(rc, self.ctx, "onmf_keep8_expand")
+        return out
+
+    def _kept_pair(self, X, H, what):
+        self._low(X, KeptColumns, what)
+        self._low(H, KeptColumns, what)
+        if X.n != H.n:
+            raise ValueError("%s: X holds %d columns, H %d" % (what, X.n, H.n))
+        return X.shape[0], H.shape[0], X.n
+
+    def keep8_aggregate(self, X, H, w, A=None, B=None):
+        """``aggregate`` from a kept X (d x n) and a kept H (r x n): (1-w) A + w H H^T and (1-w) B + w H X^T
+        (src/onmf.py:155-156); A and B None: zeros."""
+        d, r, n = self._kept_pair(X, H, "keep8_aggregate")
+        if A is not None:
+            self._matrix(A, (r, r), "keep8_aggregate: A")
+        if B is not None:
+            self._matrix(B, (r, d), "keep8_aggregate: B")
+        A1, B1 = self.empty(r, r), self.empty(r, d)
+        nbytes = self.lib.onmf_keep8_workspace(d, r, n, 0)
+        ws, wp = self._workspace(nbytes)
+        rc = self.lib.onmf_keep8_aggregate(self.ctx, d, r, n, X.codes.data_ptr(), X.scales.data_ptr(), H.codes.data_ptr(),
+                                           H.scales.data_ptr(), float(w), _ptr(A), _ptr(B), A1.data_ptr(), B1.data_ptr(),
+                                           wp, nbytes, self.stream())
+        if rc:
+            _lib.check(rc, self.ctx, "onmf_keep8_aggregate")
+        return A1, B1
+
+    def keep8_gradient(self, W, X, H):
+        """The gradient of 1/2 |X - W H|^2 to W (d x r) from a kept X and a kept H: W (H H^T) - X H^T."""
+        d, r, n = self._kept_pair(X, H, "keep8_gradient")
+        self._matrix(W, (d, r), "keep8_gradient: W")
+        dW = self.empty(d, r)
+        nbytes = self.lib.onmf_keep8_workspace(d, r, n, 1)
+        ws, wp = self._workspace(nbytes)
+        rc = self.lib.onmf_keep8_gradient(self.ctx, d, r, n, W.data_ptr(), X.codes.data_ptr(), X.scales.data_ptr(),
+                                          H.codes.data_ptr(), H.scales.data_ptr(), dW.data_ptr(), wp, nbytes,
+                                          self.stream())
+        if rc:
+            _lib.check(rc, self.ctx, "onmf_keep8_gradient")
+        return dW
 
     # ------------------------------------------------------------------ network patches
     def ndl_graph(self, row_ptr, nbr):

@@ -15,6 +15,7 @@ already scaled to [0, 1]).  Everything numeric runs on the GPU through libonmf_h
 
 Extra keyword-only arguments: ``rng`` ("numpy": corners, dictionaries and starting codes are drawn
 from NumPy's global generator in the reference's order; "device": drawn on the GPU), ``device``.
+For reconstruction ``W`` may be set to a ``PackedDictionary`` (lowbit.py).
 """
 from __future__ import annotations
 
@@ -22,6 +23,7 @@ import numpy as np
 
 from .engine import get_engine
 from .legacy.onmf import Online_NMF
+from .lowbit import PackedDictionary
 from .onmf import _is_torch, _out
 
 __all__ = ["Image_Reconstructor", "downscale_local_mean"]
@@ -95,6 +97,10 @@ class Image_Reconstructor():
                 self._data_dev = eng.dev(self.data)
             return self._data_dev
         return eng.dev(data)
+
+    def _dict_dev(self):
+        """``self.W`` as the products take it: a PackedDictionary as it is, anything else on the GPU."""
+        return self.W if isinstance(self.W, PackedDictionary) else self._engine().dev(self.W)
 
     # -- reading --------------------------------------------------------------------------
     def read_img_as_array(self, path, is_matrix=False, is_color=True):
@@ -211,8 +217,9 @@ class Image_Reconstructor():
         X = eng.extract_patches(img, k, grid=grid, stride=1)
         self.nmf = Online_NMF(X, self.n_components, self.iterations, self.batch_size, rng=self.rng,
                               device=self._device)
-        code = self.nmf.sparse_code(X, eng.dev(self.W))
-        R = eng.patch_product(eng.dev(self.W), code)
+        Wd = self._dict_dev()
+        code = self.nmf.sparse_code(X, Wd)
+        R = eng.patch_product(Wd, code)
         out, _ = eng.fold_patches(R, (h, w), k, grid, stride=1)
         self.img_recons = _out(out, False)
         return _out(code, False)
@@ -236,7 +243,7 @@ class Image_Reconstructor():
             self.A_recons = _out(out, like_torch)
             return self.A_recons
         X = eng.extract_patches(Ad, k, grid=grid, stride=s)
-        Wd = eng.dev(self.W)
+        Wd = self._dict_dev()
         r, b = Wd.shape[1], X.shape[1]
         H0 = None
         if self.rng == "numpy":

@@ -3,7 +3,8 @@
 Same constructor, method names, argument order and return conventions as the reference
 (src/onmf.py:20-271); the arithmetic runs in libonmf_hip.so on an MI355X.  Inputs may be NumPy
 arrays (results come back as float64 NumPy arrays, like the reference's) or ROCm ``torch`` tensors
-(results stay on the GPU as float32 tensors).
+(results stay on the GPU as float32 tensors).  ``X`` may also be ``KeptColumns`` (columns held in 8 bits; the
+results are tensors) and a dictionary that is only read a ``PackedDictionary`` (lowbit.py).
 
 Extra keyword-only arguments (not in the reference):
   rng     "numpy" (default): draw the initial dictionary, the subsample indices and every H0 from
@@ -23,6 +24,7 @@ import numpy as np
 
 from . import _lib
 from .engine import get_engine
+from .lowbit import KeptColumns, PackedDictionary
 
 __all__ = ["Online_NMF", "update_code_within_radius", "sparse_code_update", "dict_update", "surrogate_loss"]
 
@@ -40,6 +42,16 @@ def _out(t, like_torch):
     if like_torch:
         return t
     return t.detach().cpu().numpy().astype(np.float64)
+
+
+def _columns_dev(eng, X):
+    """The float32 columns of X on the engine's GPU; columns held in 8 bits are brought back."""
+    return eng.keep8_expand(X) if isinstance(X, KeptColumns) else eng.dev(X)
+
+
+def _dict_dev(eng, W):
+    """The float32 dictionary on the engine's GPU; one held in 4 bits is brought back."""
+    return eng.dict4_unpack(W) if isinstance(W, PackedDictionary) else eng.dev(W)
 
 
 def _weight(t, beta):
@@ -82,7 +94,7 @@ class Online_NMF():
         self.rng = rng
         self.seed = seed
         self._device = device
-        self._torch_io = _is_torch(X)
+        self._torch_io = _is_torch(X) or isinstance(X, KeptColumns)
         self._code_dev = None            # device copy of the accumulated code (lazy)
         self._code_host = None
         self._X_dev = None
@@ -122,12 +134,12 @@ class Online_NMF():
     # -- reference API ----------------------------------------------------------------------
     def sparse_code(self, X, W):
         """H (r x n) >= 0 with W H ~ X: ten damped Gauss-Seidel sweeps at most, stopping_diff 0.01
-        (src/onmf.py:51-90)."""
+        (src/onmf.py:51-90).  X may be KeptColumns, W a PackedDictionary."""
         if DEBUG:
             print('sparse_code', 'X.shape:', X.shape, 'W.shape:', W.shape)
         eng = self._engine()
-        like_torch = _is_torch(X)
-        Xd, Wd = eng.dev(X), eng.dev(W)
+        like_torch = _is_torch(X) or isinstance(X, KeptColumns)
+        Xd, Wd = _columns_dev(eng, X), _dict_dev(eng, W)
         H0, seed = self._draw_h0(eng, Wd.shape[1], Xd.shape[1])
         H, sweeps, dist = eng.sparse_code(Xd, Wd, H0=H0, alpha=self._alpha(), sub_iter=10,
                                           stopping_diff=0.01, seed=seed)
@@ -143,8 +155,8 @@ class Online_NMF():
     def step(self, X, aggregates, W, t):
         """One online-NMF iteration (src/onmf.py:119-167): returns H1, [A1, B1(, C1)], W1."""
         eng = self._engine()
-        like_torch = _is_torch(X)
-        Xd, Wd = eng.dev(X), eng.dev(W)
+        like_torch = _is_torch(X) or isinstance(X, KeptColumns)
+        Xd, Wd = _columns_dev(eng, X), eng.dev(W)
         Ad, Bd = eng.dev(aggregates[0]), eng.dev(aggregates[1])
         Cd = eng.dev(aggregates[2]) if len(aggregates) == 3 else None
         H1, agg1, W1 = self._step_dev(eng, Xd, Ad, Bd, Cd, Wd, t, want_code=True)
@@ -165,8 +177,9 @@ class Online_NMF():
         """Learn W from the columns of self.X (src/onmf.py:169-226): returns W, aggregates, code."""
         eng = self._engine()
         like_torch = self._torch_io
-        if self._X_dev is None:
-            self._X_dev = eng.dev(self.X)
+        kept = isinstance(self.X, KeptColumns) and self.subsample     # minibatches are brought back one by one
+        if self._X_dev is None or (isinstance(self._X_dev, KeptColumns) and not kept):
+            self._X_dev = self.X if kept else _columns_dev(eng, self.X)
         Xd = self._X_dev
         d, n = Xd.shape
         r = self.n_components
@@ -203,7 +216,7 @@ class Online_NMF():
                     idx = np.random.randint(n, size=self.batch_size)   # src/onmf.py:212
                 else:
                     idx = eng.torch.randint(n, (self.batch_size,), device=eng.device)
-                Xb = eng.gather_columns(Xd, idx)
+                Xb = eng.keep8_expand(Xd, idx) if kept else eng.gather_columns(Xd, idx)
             # every step starts from the aggregates this call was given (src/onmf.py:217-219)
             H, last, Wd = self._step_dev(eng, Xb, Ad, Bd, Cd, Wd, t0 + i, want_code=True)
             eng.code_accumulate(code_dev, idx, H)                       # src/onmf.py:221
@@ -233,8 +246,8 @@ def update_code_within_radius(X, W, H0=None, r=None, alpha=0, sub_iter=10, stopp
     if r is not None and not r > 0:
         raise ValueError("update_code_within_radius: the radius must be positive (or None)")
     eng = get_engine(device)
-    like_torch = _is_torch(X)
-    Xd, Wd = eng.dev(X), eng.dev(W)
+    like_torch = _is_torch(X) or isinstance(X, KeptColumns)
+    Xd, Wd = _columns_dev(eng, X), _dict_dev(eng, W)
     H0 = eng.numpy_rand(Wd.shape[1], Xd.shape[1]) if H0 is None else eng.dev(H0)       # src/onmf.py:245-246
     H, sweeps, dist = eng.sparse_code(Xd, Wd, H0=H0, alpha=alpha, sub_iter=sub_iter,
                                       stopping_diff=stopping_diff, radius=r)
