@@ -393,7 +393,7 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  * onmf_keep8_gradient   dW (d x r) = W (H H^T) - X H^T, the gradient of 1/2 |X - W H|^2 to W; d, r <= 2^18
  * Products inside a group add up exactly in int32, groups in float32, runs of groups and what follows in double.
  * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, in use until the call's work on
- * `stream` is done.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
+ * `stream` is done.  n <= 2^28.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
  */
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient);
 int onmf_keep8(onmf_ctx* ctx, int d, int n, const void* X, int x_type, int ldx, int8_t* codes, float* scales, void* stream);

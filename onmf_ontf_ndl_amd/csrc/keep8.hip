@@ -10,11 +10,11 @@
 #include <algorithm>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 namespace {
 
 constexpr int GROUP = 128;
+constexpr int MOST_COLS = 1 << 28;       // eight rows' codes lie within 32 bits
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ float load_val(const float* p) { return *p; }
@@ -122,198 +122,293 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 }
 
 // ------------------------------------------------------------------------------------------- sums
-// 128 x 128 tiles of [H H^T | H X^T] (the columns of the second part start on a tile), one 128-column group
-// of the contraction a step; a workgroup takes a run of groups and writes its sums to a slab.  int32 inside a
-// group, float32 over a workgroup's run, double over the runs.
-constexpr int BM = 128, BN = 128, LROW = GROUP + 16;       // LDS row stride in bytes: 16-byte reads of 16 rows meet every bank once
+// Tiles of [H H^T | H X^T], one 128-column group of the contraction a step; a workgroup takes a run of groups and
+// writes its sums to a slab.  int32 inside a group (at most 128 * 127^2), float32 over a workgroup's run, double
+// over the runs.
+// Eight waves; a wave owns 16 MI x 16 NJ outputs in 16x16x64 tiles (four of X's scales and one of H's a lane
+// and tile: half the scale reads of the 32x32 shape).  The codes go from memory straight to LDS, two groups ahead,
+// in rows of 128 bytes whose 16-byte chunks are permuted by (row >> 1) & 7, so that the 16 rows of an operand read
+// meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.
+// Per group and output three vector instructions (conversion, product of the scales, fused multiply-add) stand
+// against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not.
+template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
+    static constexpr int mi = MI, nj = NJ, wm = WM_, wn = WN_, stages = STAGES;
+    static constexpr int bm = 16 * MI * WM_, bn = 16 * NJ * WN_, waves = WM_ * WN_;
+    static constexpr int rows = (bm + bn + 8 * waves - 1) / (8 * waves) * (8 * waves);     // of a stage: every wave loads as many
+    static constexpr int srows = (bm + bn + 16 * waves - 1) / (16 * waves) * (16 * waves);  // the same for the scales
+};
 
 struct SumParams {
     const int8_t *hc, *xc;
     const float *hs, *xs;
     float* slab;              // [split][r][cols]
-    int d, r, groups, per_split;
-    int tiles_m, tiles_h;     // tiles along r (rows), tiles of the H H^T part along the columns
-    int cols;                 // columns of a slab row: tiles_h * BN + d
+    int d, r, groups, per_split, splits;
+    int tiles_m, tiles_h, tiles;     // tiles along r (rows); column tiles of the H H^T part; all tiles
+    int cols_h, cols;         // columns of a slab row: the H H^T part's, all (both multiples of 4)
 };
 
-__global__ __launch_bounds__(256) void keep8_sums_kernel(SumParams p) {
-    __shared__ __align__(16) int8_t la[2][BM * LROW], lb[2][BN * LROW];
-    __shared__ float sa[2][BM], sb[2][BN];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int tm = blockIdx.x % p.tiles_m, tn = blockIdx.x / p.tiles_m;
-    const int m0 = tm * BM;
+template <typename S>
+__global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) {
+    constexpr int STAGES = S::stages, AHEAD = STAGES - 1, STAGE = S::rows * GROUP;
+    extern __shared__ __align__(16) int8_t lds[];            // [STAGES][STAGE], then float [2][S::srows][4]
+    float* lsc = (float*)(lds + STAGES * STAGE);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // workgroups of one run share H's codes: they follow each other on one XCD (workgroups go to the XCDs in turn,
+    // an eighth of them to each)
+    const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    const int split = at / p.tiles, tile = at % p.tiles;
+    if (split >= p.splits) return;
+    const int tm = tile % p.tiles_m, tn = tile / p.tiles_m;
+    const int m0 = tm * S::bm;
     const bool is_h = tn < p.tiles_h;
-    const int n0 = is_h ? tn * BN : (tn - p.tiles_h) * BN;
+    const int n0 = (is_h ? tn : tn - p.tiles_h) * S::bn;
     const int N = is_h ? p.r : p.d;
     const int8_t* bc = is_h ? p.hc : p.xc;
     const float* bs = is_h ? p.hs : p.xs;
     const size_t ld = (size_t)p.groups * GROUP;
-    const int g0 = blockIdx.y * p.per_split, g1 = min(p.groups, g0 + p.per_split);
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
+    const int g0 = split * p.per_split, g1 = min(p.groups, g0 + p.per_split);
+    const int wm = (wave % S::wm) * 16 * S::mi, wn = (wave / S::wm) * 16 * S::nj;
 
-    uint4 ra[4], rb[4];
-    float fs = 0.f;
-    auto fetch = [&](int g) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = (t >> 3) + 32 * j, col = (t & 7) * 16;
-            ra[j] = rb[j] = make_uint4(0, 0, 0, 0);
-            if (m0 + row < p.r) ra[j] = *reinterpret_cast<const uint4*>(p.hc + (size_t)(m0 + row) * ld + (size_t)g * GROUP + col);
-            if (n0 + row < N) rb[j] = *reinterpret_cast<const uint4*>(bc + (size_t)(n0 + row) * ld + (size_t)g * GROUP + col);
-        }
-        const int row = t & 127;
-        fs = 0.f;
-        if (t < 128) { if (m0 + row < p.r) fs = p.hs[(size_t)(m0 + row) * p.groups + g]; }
-        else if (n0 + row < N) fs = bs[(size_t)(n0 + row) * p.groups + g];
+    // A wave's loads are eight rows each, dealt out to the waves in turn; scales come four groups at a time, four
+    // lanes to a row (a row's are 4 bytes a group: taken one group at a time they were as many requests as the
+    // codes): [row][4].  Addresses: a base for the wave and 32 bits a lane.
+    constexpr int NW = S::waves, LOADS = S::rows / 8 / NW, SLOADS = S::srows / 16 / NW;
+    auto rows_of = [&](int row, int& first, int& last) {         // the matrix row at row `row` of a stage, and the last there is
+        const bool of_h = row < S::bm;
+        last = of_h ? p.r - 1 : N - 1;
+        first = min(of_h ? m0 + row : n0 + row - S::bm, last);
+        return of_h;
     };
-    auto stage = [&](int buf) {
+    const int8_t* base[LOADS];
+    uint32_t off[LOADS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int row = (t >> 3) + 32 * j, col = (t & 7) * 16;
-            *reinterpret_cast<uint4*>(&la[buf][row * LROW + col]) = ra[j];
-            *reinterpret_cast<uint4*>(&lb[buf][row * LROW + col]) = rb[j];
-        }
-        if (t < 128) sa[buf][t] = fs; else sb[buf][t - 128] = fs;
-    };
-
-    f32x16 acc[2][2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    fetch(g0);
-    stage(0);
-    for (int g = g0; g < g1; ++g) {
-        const int buf = (g - g0) & 1;
-        __syncthreads();
-        if (g + 1 < g1) fetch(g + 1);
-        i32x16 part[2][2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) part[i][j][e] = 0;
-        const int at = (lane & 31) * LROW + (lane >> 5) * 16;
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            i32x4 fa[2], fb[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                fa[i] = *reinterpret_cast<const i32x4*>(&la[buf][(wm + i * 32) * LROW + at + h * 32]);
-                fb[i] = *reinterpret_cast<const i32x4*>(&lb[buf][(wn + i * 32) * LROW + at + h * 32]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    part[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[i], fb[j], part[i][j], 0, 0, 0);
-        }
-        float cs[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) cs[j] = sb[buf][wn + j * 32 + (lane & 31)];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float rs = sa[buf][wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j][e] = fmaf(rs, cs[j] * (float)part[i][j][e], acc[i][j][e]);
-            }
-        if (g + 1 < g1) stage(buf ^ 1);
+    for (int j = 0; j < LOADS; ++j) {
+        const int row = (j * NW + wave) * 8;
+        int first, last;
+        base[j] = rows_of(row, first, last) ? p.hc : bc;
+        base[j] += (size_t)first * ld;
+        off[j] = (uint32_t)(min(first + (lane >> 3), last) - first) * (uint32_t)ld +
+                 (((lane & 7) ^ (((row + (lane >> 3)) >> 1) & 7)) * 16);
     }
+    const float* sbase[SLOADS];
+    uint32_t soff[SLOADS];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int n = n0 + wn + j * 32 + (lane & 31);
-        if (n >= N) continue;
-        const int col = is_h ? n : p.tiles_h * BN + n;
+    for (int j = 0; j < SLOADS; ++j) {
+        int first, last;
+        sbase[j] = rows_of((j * NW + wave) * 16, first, last) ? p.hs : bs;
+        sbase[j] += (size_t)first * p.groups;
+        soff[j] = (uint32_t)(min(first + (lane >> 2), last) - first) * (uint32_t)p.groups * 4;
+    }
+    auto fetch = [&](int g, int buf) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int j = 0; j < LOADS; ++j)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base[j] + (size_t)g * GROUP + off[j]),
+                                             (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (j * NW + wave) * 1024),
+                                             16, 0, 0);
+    };
+    auto fetch_scales = [&](int g, int half) {
+        const uint32_t q = (uint32_t)min(lane & 3, p.groups - 1 - g) * 4;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                if (m < p.r) p.slab[((size_t)blockIdx.y * p.r + m) * p.cols + col] = acc[i][j][e];
-            }
+        for (int j = 0; j < SLOADS; ++j)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)(sbase[j] + g) + (soff[j] + q)),
+                                             (__attribute__((address_space(3))) void*)(lsc + half * 4 * S::srows + (j * NW + wave) * 64),
+                                             4, 0, 0);
+    };
+
+    f32x4 acc[S::mi][S::nj];
+#pragma unroll
+    for (int i = 0; i < S::mi; ++i)
+#pragma unroll
+        for (int j = 0; j < S::nj; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // where a lane's operands and scales lie in a stage (whole tiles of 16 rows further on the chunks lie alike)
+    const int op0 = (wm + (lane & 15)) * GROUP + (((lane >> 4) ^ ((lane >> 1) & 7)) * 16), op1 = op0 ^ 64;
+    const int ba = (S::bm + wn - wm) * GROUP;
+    const int sc_h = 4 * (wm + (lane & 15)), sc_x = 4 * (S::bm + wn + 4 * (lane >> 4));
+    // AHEAD groups are on their way while one is computed, and the scales of the next four.  Loads come back in order:
+    // with only what was sent behind this group's codes still out - the codes of the AHEAD - 1 groups behind it, and
+    // the scales where a fetch of them lies in between - this one's have arrived; behind the barrier those of all
+    // waves have, and all waves are done with the group before, whose place the next one sent for takes.
+    const int n = g1 - g0;
+    fetch_scales(g0, 0);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+        if (k < n) fetch(g0 + k, k);
+    int buf = 0;
+    for (int k = 0; k < n; ++k) {
+        // (step i sent for scales where i is a multiple of four and group i + 4 is there)
+        const int i = (k - 1) & ~3;
+        const bool scales_out = i >= k - AHEAD && i >= 0 && i + 4 < n;
+        if (k + AHEAD > n) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else if (scales_out) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS + SLOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS) : "memory");
+        if (k + AHEAD < n) fetch(g0 + k + AHEAD, buf == 0 ? AHEAD : buf - 1);
+        if ((k & 3) == 0 && k + 4 < n) fetch_scales(g0 + k + 4, ((k >> 2) + 1) & 1);
+        const int8_t* la0 = lds + buf * STAGE + op0;
+        const int8_t* la1 = lds + buf * STAGE + op1;
+        const float* sa = lsc + ((k >> 2) & 1) * 4 * S::srows + (k & 3) + sc_h;
+        const float* sb = lsc + ((k >> 2) & 1) * 4 * S::srows + (k & 3) + sc_x;
+        // (X's rows are the matrix instruction's rows and H's its columns: a lane's four values lie side by side in
+        // the slab)
+        i32x4 fa[S::mi][2];
+        float hs[S::mi];
+#pragma unroll
+        for (int i = 0; i < S::mi; ++i) {
+            fa[i][0] = *reinterpret_cast<const i32x4*>(la0 + 16 * i * GROUP);
+            fa[i][1] = *reinterpret_cast<const i32x4*>(la1 + 16 * i * GROUP);
+            hs[i] = sa[4 * 16 * i];
+        }
+#pragma unroll
+        for (int j = 0; j < S::nj; ++j) {
+            const i32x4 fb0 = *reinterpret_cast<const i32x4*>(la0 + ba + 16 * j * GROUP);
+            const i32x4 fb1 = *reinterpret_cast<const i32x4*>(la1 + ba + 16 * j * GROUP);
+            float xs[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) xs[e] = sb[4 * (16 * j + e)];
+            i32x4 part[S::mi];
+#pragma unroll
+            for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb0, fa[i][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb1, fa[i][1], part[i], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < S::mi; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(xs[e] * hs[i], (float)part[i][e], acc[i][j][e]);
+        }
+        buf = buf == AHEAD ? 0 : buf + 1;
+    }
+    float* out = p.slab + (size_t)split * p.r * p.cols + (is_h ? 0 : p.cols_h);
+#pragma unroll
+    for (int i = 0; i < S::mi; ++i) {
+        const int m = m0 + wm + 16 * i + (lane & 15);
+        if (m >= p.r) continue;
+#pragma unroll
+        for (int j = 0; j < S::nj; ++j) {
+            const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
+            if (n < N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.cols + n) = acc[i][j];      // (rows of the slab are padded to whole quads)
+        }
     }
 }
 
-// A = keep A_in + w sum, B = keep B_in + w sum over the slabs, in order and in double.  With Ad, Bd (the gradient)
-// the sums themselves are written there as doubles.
-__global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int colh, int cols, int splits,
+// sum over the slabs of four neighbouring entries, in double and in a fixed order: the ZL threads of an entry take
+// every ZL-th slab and are added in turn
+template <int ZL>
+__device__ __forceinline__ void sum_slabs(const float* src, size_t stride, int splits, int z0, double (&s)[4]) {
+    s[0] = s[1] = s[2] = s[3] = 0.0;
+#pragma unroll 8
+    for (int z = z0; z < splits; z += ZL) {
+        const float4 v = *reinterpret_cast<const float4*>(src + (size_t)z * stride);
+        s[0] += (double)v.x; s[1] += (double)v.y; s[2] += (double)v.z; s[3] += (double)v.w;
+    }
+}
+
+// A = keep A_in + w sum, B = keep B_in + w sum; with Ad and Bd (the gradient) the sums themselves, as doubles.
+template <int ZL>
+__global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int cols_h, int cols, int splits,
                                                             const float* __restrict__ slab, double w, double keep,
                                                             const float* A_in, const float* B_in, float* A, float* B,
                                                             double* __restrict__ Ad, double* __restrict__ Bd) {
-    const size_t one = (size_t)r * cols, all = (size_t)r * (r + d);
-    for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < all; e += (size_t)gridDim.x * 256) {
-        const int k = (int)(e / (r + d)), j = (int)(e % (r + d));
-        const float* src = slab + (size_t)k * cols + (j < r ? j : colh + (j - r));
-        double s = 0.0;
-        for (int z = 0; z < splits; ++z) s += (double)src[(size_t)z * one];
-        if (Ad) {
-            if (j < r) Ad[(size_t)k * r + j] = s;
-            else Bd[(size_t)k * d + (j - r)] = s;
-        } else if (j < r) {
-            const size_t at = (size_t)k * r + j;
-            A[at] = (float)(w * s + (A_in ? keep * (double)A_in[at] : 0.0));
-        } else {
-            const size_t at = (size_t)k * d + (j - r);
-            B[at] = (float)(w * s + (B_in ? keep * (double)B_in[at] : 0.0));
-        }
+    constexpr int Q = 256 / ZL;
+    __shared__ double part[ZL][Q][4];
+    const int q = threadIdx.x % Q, z0 = threadIdx.x / Q;
+    const int quads = cols / 4;
+    const size_t all = (size_t)r * quads, one = (size_t)r * cols;
+    const size_t e = (size_t)blockIdx.x * Q + q;
+    const int k = e < all ? (int)(e / quads) : 0, c = e < all ? (int)(e % quads) * 4 : 0;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    if (e < all) sum_slabs<ZL>(slab + (size_t)k * cols + c, one, splits, z0, s);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[z0][q][j] = s[j];
+    __syncthreads();
+    if (z0 != 0 || e >= all) return;
+    const bool is_h = c < cols_h;
+    const int n0 = is_h ? c : c - cols_h, N = is_h ? r : d;
+    const float* in = is_h ? A_in : B_in;
+    float* out = is_h ? A : B;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (n0 + j >= N) break;
+        double v = part[0][q][j];
+#pragma unroll
+        for (int z = 1; z < ZL; ++z) v += part[z][q][j];
+        const size_t at = (size_t)k * N + n0 + j;
+        if (Ad) (is_h ? Ad : Bd)[at] = v;
+        else out[at] = (float)(w * v + (in ? keep * (double)in[at] : 0.0));
     }
 }
 
-// dW[i][k] = sum_j W[i][j] A[j][k] - B[k][i] in double, rounded once: near a stationary dictionary the two
-// terms nearly cancel.
+// dW[i][k] = sum_j W[i][j] A[j][k] - B[k][i] in double, rounded once: near a stationary dictionary the two terms
+// nearly cancel.  32 x 32 tiles, a 16 x 16 one a wave on the double matrix pipe (16x16x4: row l % 16 and column
+// l % 16 of the operands at j + l / 16, output row 4 e + l / 16); the next 32 steps of j are loaded into registers
+// while these are computed.
+typedef double f64x4 __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(256) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
                                                               const double* __restrict__ A,
                                                               const double* __restrict__ B, float* __restrict__ dW) {
-    __shared__ double tw[32][17], ta[16][33], tb[32][33];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    __shared__ double tw[32][33], ta[32][34], tb[32][33];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
-    double acc[2][2] = {{0.0, 0.0}, {0.0, 0.0}};
-    for (int j0 = 0; j0 < r; j0 += 16) {
-        for (int e = threadIdx.x; e < 512; e += 256) {
-            const int i = e >> 4, j = e & 15;
-            tw[i][j] = (i0 + i < d && j0 + j < r) ? (double)W[(size_t)(i0 + i) * r + j0 + j] : 0.0;
-            const int jj = e >> 5, k = e & 31;
-            ta[jj][k] = (j0 + jj < r && k0 + k < r) ? A[(size_t)(j0 + jj) * r + k0 + k] : 0.0;
+    const int wi = (wave & 1) * 16, wk = (wave >> 1) * 16;
+    const int row = t >> 5, col = t & 31;                   // and the rows 8, 16, 24 behind it
+    float vw[4];
+    double va[4];
+    auto fetch = [&](int j0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int y = row + 8 * q;
+            vw[q] = (i0 + y < d && j0 + col < r) ? W[(size_t)(i0 + y) * r + j0 + col] : 0.f;
+            va[q] = (j0 + y < r && k0 + col < r) ? A[(size_t)(j0 + y) * r + k0 + col] : 0.0;
         }
+    };
+    fetch(0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int k = k0 + row + 8 * q, i = i0 + col;
+        tb[col][row + 8 * q] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
+    }
+    f64x4 acc = f64x4{0.0, 0.0, 0.0, 0.0};
+    for (int j0 = 0; j0 < r; j0 += 32) {
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) acc[a][c] = fma(tw[ty + 16 * a][j], ta[j][tx + 16 * c], acc[a][c]);
-        __syncthreads();
-    }
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-        const int k = e >> 5, i = e & 31;
-        tb[i][k] = (k0 + k < r && i0 + i < d) ? B[(size_t)(k0 + k) * d + i0 + i] : 0.0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int i = i0 + ty + 16 * a, k = k0 + tx + 16 * c;
-            if (i < d && k < r) dW[(size_t)i * r + k] = (float)(acc[a][c] - tb[ty + 16 * a][tx + 16 * c]);
+        for (int q = 0; q < 4; ++q) {
+            tw[row + 8 * q][col] = (double)vw[q];
+            ta[row + 8 * q][col] = va[q];
         }
+        __syncthreads();
+        if (j0 + 32 < r) fetch(j0 + 32);
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(tw[wi + (lane & 15)][j + (lane >> 4)],
+                                                       ta[j + (lane >> 4)][wk + (lane & 15)], acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int i = wi + 4 * e + (lane >> 4), k = wk + (lane & 15);
+        if (i0 + i < d && k0 + k < r) dW[(size_t)(i0 + i) * r + k0 + k] = (float)(acc[e] - tb[i][k]);
+    }
 }
 
 // ------------------------------------------------------------------------------------------- launches
-struct SumPlan { int tiles_m, tiles_h, tiles_x, cols, splits, per; };
+// The tile follows r, so that X is read once: its columns are the wider the fewer rows there are.
+using Wide = Tile<4, 2, 4, 4, 3>;       // 256 x 128
+using Middle = Tile<4, 2, 2, 8, 3>;     // 128 x 256
+using Narrow = Tile<4, 2, 1, 8, 3>;     // 64 x 256
+using Slim = Tile<2, 2, 1, 8, 3>;       // 32 x 256
+
+struct SumPlan { int tile, bm, bn, tiles_m, tiles_h, tiles_x, cols_h, cols, splits, per; };
 SumPlan sum_plan(int d, int r, int n) {
     SumPlan q;
     const int groups = (n + GROUP - 1) / GROUP;
-    q.tiles_m = (r + BM - 1) / BM;
-    q.tiles_h = (r + BN - 1) / BN;
-    q.tiles_x = (d + BN - 1) / BN;
-    q.cols = q.tiles_h * BN + d;
+    const int tile[4][2] = {{Slim::bm, Slim::bn}, {Narrow::bm, Narrow::bn}, {Middle::bm, Middle::bn}, {Wide::bm, Wide::bn}};
+    q.tile = r <= Slim::bm ? 0 : r <= Narrow::bm ? 1 : r <= Middle::bm ? 2 : 3;
+    q.bm = tile[q.tile][0];
+    q.bn = tile[q.tile][1];
+    q.tiles_m = (r + q.bm - 1) / q.bm;
+    q.tiles_h = (r + q.bn - 1) / q.bn;
+    q.tiles_x = (d + q.bn - 1) / q.bn;
+    q.cols_h = (r + 3) & ~3;
+    q.cols = q.cols_h + ((d + 3) & ~3);
     const long long tiles = (long long)q.tiles_m * (q.tiles_h + q.tiles_x);
-    long long splits = std::max<long long>(1, 512 / tiles);
+    long long splits = std::max<long long>(1, 256 / tiles);
     splits = std::min<long long>(splits, groups);
     q.per = (int)((groups + splits - 1) / splits);
     q.splits = (groups + q.per - 1) / q.per;
@@ -324,7 +419,18 @@ size_t sums_bytes(const SumPlan& q, int r) { return ((size_t)q.splits * r * q.co
 int check8(onmf_ctx* c, const char* what, int d, int n, const void* codes, const void* scales) {
     if (d <= 0 || n <= 0 || !codes || !scales || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
         return onmf_fail(c, ONMF_ERR_ARG, "%s: bad arguments (d=%d n=%d; codes must be aligned to 16 bytes)", what, d, n);
-    if (n > 2147483647 - 2 * GROUP) return onmf_fail(c, ONMF_ERR_ARG, "%s: n=%d is too large", what, n);
+    if (n > MOST_COLS) return onmf_fail(c, ONMF_ERR_ARG, "%s: n=%d is more than 2^28 columns", what, n);
+    return ONMF_OK;
+}
+
+template <typename S>
+int launch_sums(onmf_ctx* c, const SumParams& p, hipStream_t s) {
+    constexpr size_t bytes = S::stages * (size_t)S::rows * GROUP + 2 * (size_t)S::srows * 4 * sizeof(float);
+    static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
+    static LdsLimit lim;
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_sums_kernel<S>, bytes));
+    hipLaunchKernelGGL(keep8_sums_kernel<S>, dim3((p.tiles * p.splits + 7) / 8 * 8), dim3(64 * S::waves), bytes, s, p);
+    HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
 
@@ -332,14 +438,31 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
              const float* hs, float* slab, hipStream_t s) {
     SumParams p;
     p.hc = hc; p.xc = xc; p.hs = hs; p.xs = xs; p.slab = slab;
-    p.d = d; p.r = r; p.groups = (n + GROUP - 1) / GROUP; p.per_split = q.per;
-    p.tiles_m = q.tiles_m; p.tiles_h = q.tiles_h; p.cols = q.cols;
-    hipLaunchKernelGGL(keep8_sums_kernel, dim3(q.tiles_m * (q.tiles_h + q.tiles_x), q.splits), dim3(256), 0, s, p);
+    p.d = d; p.r = r; p.groups = (n + GROUP - 1) / GROUP; p.per_split = q.per; p.splits = q.splits;
+    p.tiles_m = q.tiles_m; p.tiles_h = q.tiles_h; p.tiles = q.tiles_m * (q.tiles_h + q.tiles_x);
+    p.cols_h = q.cols_h; p.cols = q.cols;
+    switch (q.tile) {
+        case 0: return launch_sums<Slim>(c, p, s);
+        case 1: return launch_sums<Narrow>(c, p, s);
+        case 2: return launch_sums<Middle>(c, p, s);
+        default: return launch_sums<Wide>(c, p, s);
+    }
+}
+
+// (few entries with many slabs: more threads to an entry)
+int run_reduce(onmf_ctx* c, const SumPlan& q, int d, int r, const float* slab, double w, double keep, const float* A_in,
+               const float* B_in, float* A, float* B, double* Ad, double* Bd, hipStream_t s) {
+    const size_t quads = (size_t)r * q.cols / 4;
+    if (quads < 16384)
+        hipLaunchKernelGGL(keep8_reduce_kernel<16>, dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, s, d, r, q.cols_h, q.cols,
+                           q.splits, slab, w, keep, A_in, B_in, A, B, Ad, Bd);
+    else
+        hipLaunchKernelGGL(keep8_reduce_kernel<4>, dim3((unsigned)((quads + 63) / 64)), dim3(256), 0, s, d, r, q.cols_h, q.cols,
+                           q.splits, slab, w, keep, A_in, B_in, A, B, Ad, Bd);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
 
-unsigned reduce_blocks(int d, int r) { return (unsigned)std::min<size_t>(((size_t)r * (r + d) + 255) / 256, 8192); }
 unsigned group_blocks(int d, int n) {
     return (unsigned)std::min<size_t>(((size_t)d * ((n + GROUP - 1) / GROUP) + 7) / 8, 8192);
 }
@@ -388,7 +511,7 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
 }
 
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
-    if (d <= 0 || r <= 0 || n <= 0 || n > 2147483647 - 2 * GROUP) return 0;
+    if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;
     return sums_bytes(sum_plan(d, r, n), r) + (gradient ? sizeof(double) * (size_t)r * ((size_t)r + d) : 0);
 }
 
@@ -406,10 +529,7 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
     hipStream_t s = (hipStream_t)stream;
     const SumPlan q = sum_plan(d, r, n);
     ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, s));
-    hipLaunchKernelGGL(keep8_reduce_kernel, dim3(reduce_blocks(d, r)), dim3(256), 0, s, d, r, q.tiles_h * BN, q.cols, q.splits,
-                       (const float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, (double*)nullptr, (double*)nullptr);
-    HIP_TRY(c, hipGetLastError());
-    return ONMF_OK;
+    return run_reduce(c, q, d, r, (const float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr, nullptr, s);
 }
 
 int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const int8_t* x_codes, const float* x_scales,
@@ -428,13 +548,10 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
     hipStream_t s = (hipStream_t)stream;
     const SumPlan q = sum_plan(d, r, n);
     double* Ad = (double*)((char*)ws + sums_bytes(q, r));
-    double* Bd = Ad + (size_t)r * r;
     ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, s));
-    hipLaunchKernelGGL(keep8_reduce_kernel, dim3(reduce_blocks(d, r)), dim3(256), 0, s, d, r, q.tiles_h * BN, q.cols, q.splits,
-                       (const float*)ws, 1.0, 0.0, (const float*)nullptr, (const float*)nullptr, (float*)nullptr, (float*)nullptr,
-                       Ad, Bd);
-    HIP_TRY(c, hipGetLastError());
-    hipLaunchKernelGGL(keep8_gradient_kernel, dim3((r + 31) / 32, (d + 31) / 32), dim3(256), 0, s, d, r, W, Ad, Bd, dW);
+    ONMF_TRY(run_reduce(c, q, d, r, (const float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr, Ad, Ad + (size_t)r * r, s));
+    hipLaunchKernelGGL(keep8_gradient_kernel, dim3((r + 31) / 32, (d + 31) / 32), dim3(256), 0, s, d, r, W, Ad,
+                       Ad + (size_t)r * r, dW);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }

@@ -21,7 +21,7 @@ _engines = {}
 def get_engine(device=None):
     """Engine for a GPU (default: torch's current device)."""
     import torch
-    if not torch.cuda.is_available():
+    if not _engines and not torch.cuda.is_available():      # (asked once: the question takes a microsecond)
         raise _lib.OnmfLibraryError("onmf_ontf_ndl_amd needs a ROCm GPU: torch.cuda.is_available() "
                                     "is False and there is no CPU path")
     if device is None:
@@ -53,6 +53,7 @@ class Engine:
         self._seed_counter = 0
         self._timeouts_seen = 0
         self._mt_table_set = False
+        self._get_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
     def __del__(self):
         try:
@@ -65,6 +66,13 @@ class Engine:
     # ------------------------------------------------------------------ plumbing
     def stream(self):
         return C.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
+
+    def _raw_stream(self):
+        """The current stream's handle as a number: a short product's time is the host's (0.1 us against 1.9 us for
+        the stream object that torch would build around it)."""
+        if self._get_stream is not None:
+            return self._get_stream(self.index)
+        return self.torch.cuda.current_stream(self.device).cuda_stream
 
     def dev(self, a, dtype=None):
         """numpy array / torch tensor -> contiguous float32 tensor on this GPU (no copy if already so)."""
@@ -461,16 +469,17 @@ class Engine:
         torch = self.torch
         if not isinstance(a, torch.Tensor) or a.device != self.device:
             raise ValueError("%s: the columns must be a tensor on %s" % (what, self.device))
-        if a.dim() != 2 or a.shape[1] == 0 or (rows is not None and a.shape[0] != rows) or a.shape[0] == 0:
+        shape = a.shape
+        if len(shape) != 2 or shape[1] == 0 or shape[0] == 0 or (rows is not None and shape[0] != rows):
             raise ValueError("%s: the columns must be (%s, b), not %s"
-                             % (what, "d" if rows is None else rows, tuple(a.shape)))
+                             % (what, "d" if rows is None else rows, tuple(shape)))
         if a.dtype is torch.float32:
             kind = _lib.TYPE_F32
         elif a.dtype is torch.bfloat16:
             kind = _lib.TYPE_BF16
         else:
             raise ValueError("%s: the columns must be float32 or bfloat16, not %s" % (what, a.dtype))
-        b = a.shape[1]
+        b = shape[1]
         ld = a.stride(0)
         if (b > 1 and a.stride(1) != 1) or ld < b:         # a transposed, broadcast or reversed view
             a = a.contiguous()
@@ -494,9 +503,9 @@ class Engine:
         """Device memory for one call, from torch's allocator on the current stream: calls on different streams and
         captured graphs each get their own."""
         if nbytes == 0:
-            return None, C.c_void_p(0)
+            return None, None
         t = self.torch.empty(nbytes, dtype=self.torch.uint8, device=self.device)
-        return t, C.c_void_p(t.data_ptr())
+        return t, t.data_ptr()
 
     def dict4_pack(self, W, group=64):
         """W (d x r) in 4 bits with a scale and an offset for ``group`` = 32, 64 or 128 features of an atom."""
@@ -509,7 +518,7 @@ class Engine:
         groups = -(-d // int(group))
         codes = self.torch.empty(r, groups * int(group) // 2, dtype=self.torch.uint8, device=self.device)
         scales = self.torch.empty(r, groups, dtype=self.torch.int32, device=self.device)
-        rc = self.lib.onmf_dict4_pack(self.ctx, d, r, int(group), _ptr(W), _ptr(codes), _ptr(scales), self.stream())
+        rc = self.lib.onmf_dict4_pack(self.ctx, d, r, int(group), _ptr(W), _ptr(codes), _ptr(scales), self._raw_stream())
         _lib.check(rc, self.ctx, "onmf_dict4_pack")
         return PackedDictionary(codes, scales, d, int(group))
 
@@ -518,7 +527,7 @@ class Engine:
         self._low(P, PackedDictionary, "dict4_unpack")
         d, r = P.shape
         W = self.empty(d, r)
-        rc = self.lib.onmf_dict4_unpack(self.ctx, d, r, P.group, _ptr(P.codes), _ptr(P.scales), _ptr(W), self.stream())
+        rc = self.lib.onmf_dict4_unpack(self.ctx, d, r, P.group, _ptr(P.codes), _ptr(P.scales), _ptr(W), self._raw_stream())
         _lib.check(rc, self.ctx, "onmf_dict4_unpack")
         return W
 
@@ -533,7 +542,7 @@ class Engine:
         nbytes = self.lib.onmf_dict4_workspace(_lib.DICT4_CORRELATE, d, r, b, P.group)
         ws, wp = self._workspace(nbytes)
         rc = self.lib.onmf_dict4_correlate(self.ctx, d, r, b, P.group, P.codes.data_ptr(), P.scales.data_ptr(),
-                                           X.data_ptr(), kind, ld, out.data_ptr(), wp, nbytes, self.stream())
+                                           X.data_ptr(), kind, ld, out.data_ptr(), wp, nbytes, self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_dict4_correlate")
         return out
@@ -549,7 +558,7 @@ class Engine:
         nbytes = self.lib.onmf_dict4_workspace(_lib.DICT4_PRODUCT, d, r, b, P.group)
         ws, wp = self._workspace(nbytes)
         rc = self.lib.onmf_dict4_product(self.ctx, d, r, b, P.group, P.codes.data_ptr(), P.scales.data_ptr(),
-                                         H.data_ptr(), kind, ld, out.data_ptr(), b, wp, nbytes, self.stream())
+                                         H.data_ptr(), kind, ld, out.data_ptr(), b, wp, nbytes, self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_dict4_product")
         return out
@@ -562,7 +571,7 @@ class Engine:
         codes = self.torch.empty(d, groups * GROUP8, dtype=self.torch.int8, device=self.device)
         scales = self.torch.empty(d, groups, dtype=self.torch.float32, device=self.device)
         rc = self.lib.onmf_keep8(self.ctx, d, n, X.data_ptr(), kind, ld, codes.data_ptr(), scales.data_ptr(),
-                                 self.stream())
+                                 self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_keep8")
         return KeptColumns(codes, scales, n)
@@ -572,7 +581,7 @@ class Engine:
         self._low(K, KeptColumns, "keep8_expand")
         d, n = K.shape
         if idx is None:
-            b, ip = n, C.c_void_p(0)
+            b, ip = n, None
         else:
             idx = self.dev(idx, self.torch.int64)
             if idx.dim() != 1 or idx.numel() == 0:
@@ -581,7 +590,7 @@ class Engine:
             b, ip = idx.numel(), _ptr(idx)
         out = self.empty(d, b)
         rc = self.lib.onmf_keep8_expand(self.ctx, d, n, K.codes.data_ptr(), K.scales.data_ptr(), ip, b, out.data_ptr(), b,
-                                        self.stream())
+                                        self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_keep8_expand")
         return out
@@ -606,7 +615,7 @@ class Engine:
         ws, wp = self._workspace(nbytes)
         rc = self.lib.onmf_keep8_aggregate(self.ctx, d, r, n, X.codes.data_ptr(), X.scales.data_ptr(), H.codes.data_ptr(),
                                            H.scales.data_ptr(), float(w), _ptr(A), _ptr(B), A1.data_ptr(), B1.data_ptr(),
-                                           wp, nbytes, self.stream())
+                                           wp, nbytes, self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_keep8_aggregate")
         return A1, B1
@@ -620,7 +629,7 @@ class Engine:
         ws, wp = self._workspace(nbytes)
         rc = self.lib.onmf_keep8_gradient(self.ctx, d, r, n, W.data_ptr(), X.codes.data_ptr(), X.scales.data_ptr(),
                                           H.codes.data_ptr(), H.scales.data_ptr(), dW.data_ptr(), wp, nbytes,
-                                          self.stream())
+                                          self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_keep8_gradient")
         return dW

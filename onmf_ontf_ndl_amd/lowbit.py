@@ -30,8 +30,9 @@ class PackedDictionary:
         if group not in GROUPS4:
             raise ValueError("a group is 32, 64 or 128 features, not %d" % group)
         groups = -(-d // group)
-        if d <= 0 or codes.dim() != 2 or codes.shape[0] == 0 or codes.shape[1] * 2 != groups * group or \
-                scales.shape != (codes.shape[0], groups):
+        shape = codes.shape
+        if d <= 0 or len(shape) != 2 or shape[0] == 0 or shape[1] * 2 != groups * group or \
+                scales.shape != (shape[0], groups):
             raise ValueError("codes must be (r, %d) and scales (r, %d) for d=%d, group=%d"
                              % (groups * group // 2, groups, d, group))
         if str(codes.dtype) != "torch.uint8" or str(scales.dtype) != "torch.int32" or codes.device != scales.device:
@@ -65,8 +66,9 @@ class KeptColumns:
     def __init__(self, codes, scales, n):
         n = int(n)
         groups = -(-n // GROUP8)
-        if n <= 0 or codes.dim() != 2 or codes.shape[0] == 0 or codes.shape[1] != groups * GROUP8 or \
-                scales.shape != (codes.shape[0], groups):
+        shape = codes.shape
+        if n <= 0 or len(shape) != 2 or shape[0] == 0 or shape[1] != groups * GROUP8 or \
+                scales.shape != (shape[0], groups):
             raise ValueError("codes must be (d, %d) and scales (d, %d) for n=%d" % (groups * GROUP8, groups, n))
         if str(codes.dtype) != "torch.int8" or str(scales.dtype) != "torch.float32" or codes.device != scales.device:
             raise ValueError("codes must be int8 and scales float32, on one device")
