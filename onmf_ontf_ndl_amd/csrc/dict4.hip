@@ -317,162 +317,203 @@ __global__ __launch_bounds__(256) void dict4_product_few_reduce_kernel(int d, in
 }
 
 // ------------------------------------------------------------------------------------------- many columns
-// 128 x 128 output tiles on the bfloat16 matrix pipe (32x32x16), exact to float32's rounding: a float32 value
-// is the sum of three bfloat16 pieces (8 + 8 + 8 bits), a bfloat16 one is its own piece.
-//  correlate: the whole numbers q + z (|q + z| <= 255) are bfloat16 values; a group's products are summed on
-//             their own (exactly, but for the float32 accumulation) and multiplied by the group's scale.
+// The bfloat16 matrix pipe (16x16x32), exact to float32's rounding: a float32 value is the sum of three bfloat16
+// pieces (8 + 8 + 8 bits), a bfloat16 one is its own piece.
+//  correlate: the whole numbers q + z (|q + z| <= 255) are bfloat16 values; 32 features' products are summed on
+//             their own and multiplied by their group's scale.
 //  product:   s (q + z) has at most 16 significant bits: two bfloat16 pieces hold it exactly; of the six
 //             products of pieces the last (2^-24) is left out.
-// LDS tiles are [row][32 k] with a row stride of 80 bytes (16-byte reads of 16 rows touch every bank once).
-constexpr int BM = 128, BN = 128, BK = 32, LROW = 40;      // LROW in bfloat16 values
-constexpr int LTILE = 128 * LROW;
+// The weights are laid out as bfloat16 rows [piece][m][k] in the workspace first (unpacked in the product's kernel
+// itself they cost every 128 columns as many vector instructions as the columns' own split).
+// A workgroup owns 16 MT rows and 128 columns, a wave all its rows and 32 columns, so that every column is split
+// into its pieces once and in registers: lane l holds columns 2 (l % 16) and the next, at k = 8 (l / 16) .. + 7,
+// the operand of two tiles.  The weights go from memory to LDS, one step of 32 ahead, in rows of 64 bytes whose
+// 16-byte chunks are permuted by (row >> 2) & 3: the 16 rows of an operand read meet every bank once.
+constexpr int BK = 32, BN = 128;
 
-struct ManyParams {
-    const uint32_t* codes;
-    const uint32_t* scales;
-    const void* X;           // the float operand: [k][n]
-    float* out;              // [m][n]
-    float* slab;             // [split][m][n], or null
-    int M, N, K;             // rows of the output, its columns, contraction length
-    int ldx, ldo;
-    int group, groups, words;
-    int tiles_m, k_per_split;
-    int vec;                 // 16-byte loads of X allowed
-};
-
-template <typename T>
-__device__ __forceinline__ void load_quad(const ManyParams& p, int k, int n, float (&v)[4]) {
-    const T* src = (const T*)p.X + (size_t)k * p.ldx + n;
-    v[0] = v[1] = v[2] = v[3] = 0.f;
-    if (k >= p.K) return;
-    if (p.vec && n + 3 < p.N) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(src);
-            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-        } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(src);
-            v[0] = bf16_lo(u.x); v[1] = bf16_hi(u.x); v[2] = bf16_lo(u.y); v[3] = bf16_hi(u.y);
-        }
-    } else {
+// correlate's weights: [k][features, padded to whole groups with zeros] whole numbers, and the scales as floats [group][k]
+__global__ __launch_bounds__(256) void dict4_lay_correlate_kernel(int d, int r, int words, int group, int groups,
+                                                                   const uint32_t* __restrict__ codes,
+                                                                   const uint32_t* __restrict__ scales,
+                                                                   uint4* __restrict__ A, float* __restrict__ S) {
+    const size_t all = (size_t)r * words;
+    for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < all; e += (size_t)gridDim.x * 256) {
+        const int k = (int)(e / words), w = (int)(e % words), g = w * 8 / group;
+        const uint32_t sc = scales[(size_t)k * groups + g];
+        const float z = word_offset(sc);
+        float q[8];
+        word_entries(codes[e], q);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (n + j < p.N) v[j] = load_val(src + j);
+        for (int j = 0; j < 8; ++j) q[j] = w * 8 + j < d ? q[j] + z : 0.f;
+        A[e] = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
+        if (w * 8 % group == 0) S[(size_t)g * r + k] = word_scale(sc);
     }
 }
 
-template <bool PROD, typename T, int G>
-__global__ __launch_bounds__(256) void dict4_many_kernel(ManyParams p) {
+// the product's weights: [piece][feature][atoms, padded to kp with zeros]; 128 features x 64 atoms a workgroup,
+// turned round in LDS
+__global__ __launch_bounds__(256) void dict4_lay_product_kernel(int d, int r, int words, int group, int groups, int kp,
+                                                                 const uint32_t* __restrict__ codes,
+                                                                 const uint32_t* __restrict__ scales,
+                                                                 uint16_t* __restrict__ A) {
+    __shared__ __align__(16) uint16_t tile[2][128][64 + 8];
+    const int t = threadIdx.x, w0 = blockIdx.y * 16, k0 = blockIdx.x * 64;
+    const int w = w0 + (t & 15), k = k0 + (t >> 4) * 4;
+    float v[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool there = k + j < r && w < words;
+        const uint32_t sc = there ? scales[(size_t)(k + j) * groups + w * 8 / group] : 0;
+        word_entries(there ? codes[(size_t)(k + j) * words + w] : 0, v[j]);
+#pragma unroll
+        for (int f = 0; f < 8; ++f) v[j][f] = word_scale(sc) * (v[j][f] + word_offset(sc));
+    }
+#pragma unroll
+    for (int f = 0; f < 8; ++f) {
+        const uint32_t a = pack_bf16(v[0][f], v[1][f]), b = pack_bf16(v[2][f], v[3][f]);
+        const uint32_t c = pack_bf16(v[0][f] - bf16_lo(a), v[1][f] - bf16_hi(a)), e = pack_bf16(v[2][f] - bf16_lo(b), v[3][f] - bf16_hi(b));
+        *reinterpret_cast<uint2*>(&tile[0][(t & 15) * 8 + f][(t >> 4) * 4]) = make_uint2(a, b);
+        *reinterpret_cast<uint2*>(&tile[1][(t & 15) * 8 + f][(t >> 4) * 4]) = make_uint2(c, e);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = t; e < 2 * 128 * 8; e += 256) {
+        const int piece = e >> 10, f = (e >> 3) & 127, c = (e & 7) * 8;
+        const int i = w0 * 8 + f;
+        if (i < d && k0 + c < kp)
+            *reinterpret_cast<uint4*>(A + ((size_t)piece * d + i) * kp + k0 + c) = *reinterpret_cast<const uint4*>(&tile[piece][f][c]);
+    }
+}
+
+struct ManyParams {
+    const uint16_t* A;       // [piece][M][kp] bfloat16
+    const float* S;          // correlate: [group][M]
+    const void* X;           // the float operand: [k][n]
+    float* out;              // [m][n]
+    float* slab;             // [split][m][n], or null
+    int M, N, K, kp;         // rows of the output, its columns, contraction length and that of A's rows
+    int ldx, ldo, group;
+    int tiles_m, tiles, k_per_split;
+    int vec;                 // two columns may be loaded at once
+    int vec_out;             // ... and stored
+};
+
+// columns n and n + 1 of row k
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_two(const T* row, int n, int n1, float& a, float& b) {
+    if constexpr (VEC && sizeof(T) == 4) {
+        const float2 v = *reinterpret_cast<const float2*>(row + n);
+        a = v.x; b = v.y;
+    } else if constexpr (VEC) {
+        const uint32_t v = *reinterpret_cast<const uint32_t*>(row + n);
+        a = bf16_lo(v); b = bf16_hi(v);
+    } else {
+        a = load_val(row + n);
+        b = load_val(row + n1);
+    }
+}
+
+template <bool PROD, typename T, int MT, bool VEC>
+__global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     constexpr int PX = sizeof(T) == 4 ? 3 : 1;        // pieces of the float operand
     constexpr int PW = PROD ? 2 : 1;                   // pieces of the weights
-    extern __shared__ __align__(16) uint16_t lds[];
-    uint16_t* la = lds;                                // [2][PW][128][LROW]
-    uint16_t* lb = lds + 2 * PW * LTILE;               // [2][PX][128][LROW]
-    float* lscale = (float*)(lb + 2 * PX * LTILE);     // [2][128] (correlate)
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const int m0 = (blockIdx.x % p.tiles_m) * BM, n0 = (blockIdx.x / p.tiles_m) * BN;
-    const int kbeg = blockIdx.y * p.k_per_split, kend = min(PROD ? p.K : p.words * 8, kbeg + p.k_per_split);
-    const int steps = (kend - kbeg + BK - 1) / BK;
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    // the 4 x 4 block of X that this thread stages, and its part of the weights
-    const int xk = (lane & 7) * 4, xn = (wave * 8 + (lane >> 3)) * 4;
+    constexpr int ROWS = PW * 16 * MT, STAGE = ROWS * 64;
+    constexpr int SROWS = PROD ? 0 : (16 * MT + 63) / 64 * 64;
+    extern __shared__ __align__(16) char lds[];       // [2][STAGE], then float [2][SROWS]
+    float* lscale = (float*)(lds + 2 * STAGE);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // row tiles of the same columns follow each other on one XCD
+    const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= p.tiles) return;
+    const int m0 = (at % p.tiles_m) * 16 * MT, n0 = (at / p.tiles_m) * BN + wave * 32;
+    const int kbeg = blockIdx.y * p.k_per_split, kend = min(p.kp, kbeg + p.k_per_split);
+    const int steps = (kend - kbeg) / BK;
+    // a column behind the last one reads the last one's (its results are not stored), a row behind the last one the
+    // last one (the weights are zero there)
+    const int na = min(n0 + 2 * (lane & 15), VEC ? max(p.N - 2, 0) : p.N - 1), nb = min(n0 + 2 * (lane & 15) + 1, p.N - 1);
+    const int kl = 8 * (lane >> 4);
 
-    float xv[4][4];
-    uint32_t cw[2], cs[2];
-    auto fetch = [&](int step) {
-        const int k = kbeg + step * BK;
+    // 16 rows of weights a load: a base for the wave and 32 bits a lane
+    constexpr int LOADS = (ROWS / 16 + 3) / 4;
+    const char* base[LOADS];
+    uint32_t off[LOADS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load_quad<T>(p, k + xk + j, n0 + xn, xv[j]);
-        if constexpr (!PROD) {
-            const int m = m0 + (t >> 1), w = k / 8 + (t & 1) * 2;
-            cw[0] = cw[1] = cs[0] = 0;
-            if (m < p.M) {
-                const uint2 v = *reinterpret_cast<const uint2*>(p.codes + (size_t)m * p.words + w);
-                cw[0] = v.x; cw[1] = v.y;
-                cs[0] = p.scales[(size_t)m * p.groups + k / G];
-            }
-        } else {
-            const int w = m0 / 8 + (t & 15);
+    for (int j = 0; j < LOADS; ++j) {
+        const int row = (j * 4 + wave) * 16, piece = row / (16 * MT);
+        const int first = min(m0 + row - piece * 16 * MT, p.M - 1);
+        base[j] = (const char*)(p.A + ((size_t)piece * p.M + first) * p.kp);
+        off[j] = (uint32_t)(min(first + (lane >> 2), p.M - 1) - first) * (uint32_t)p.kp * 2 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16);
+    }
+    const uint32_t soff = PROD ? 0 : (uint32_t)min(m0 + t, p.M - 1) * 4;
+    auto fetch_a = [&](int k, int buf) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int kk = k + (t >> 4) * 2 + j;
-                cw[j] = cs[j] = 0;
-                if (kk < p.K && w < p.words) {
-                    cw[j] = p.codes[(size_t)kk * p.words + w];
-                    cs[j] = p.scales[(size_t)kk * p.groups + (w * 8) / G];
-                }
-            }
-        }
+        for (int j = 0; j < LOADS; ++j)
+            if (ROWS % 64 == 0 || (j * 4 + wave) * 16 < ROWS)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base[j] + (size_t)k * 2 + off[j]),
+                                                 (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (j * 4 + wave) * 1024),
+                                                 16, 0, 0);
+        if constexpr (!PROD)
+            if (wave * 64 < 16 * MT)               // (by way of a register the wave would wait for it here)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)((const char*)(p.S + (size_t)(k / p.group) * p.M) + soff),
+                    (__attribute__((address_space(3))) void*)(lscale + buf * SROWS + wave * 64), 4, 0, 0);
     };
-    auto stage = [&](int buf) {
-        uint16_t* b = lb + buf * PX * LTILE;
+    float xr[8][2];
+    auto fetch_x = [&](int k) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float v0 = xv[0][j], v1 = xv[1][j], v2 = xv[2][j], v3 = xv[3][j];
+        for (int j = 0; j < 8; ++j)
+            load_two<T, VEC>((const T*)p.X + (size_t)min(k + kl + j, p.K - 1) * p.ldx, na, nb, xr[j][0], xr[j][1]);
+    };
+    uint4 fb[2][PX];
+    auto split_x = [&]() {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = xr[j][c];
 #pragma unroll
             for (int q = 0; q < PX; ++q) {
-                const uint32_t a = pack_bf16(v0, v1), c = pack_bf16(v2, v3);
-                *reinterpret_cast<uint2*>(b + q * LTILE + (xn + j) * LROW + xk) = make_uint2(a, c);
-                v0 -= bf16_lo(a); v1 -= bf16_hi(a); v2 -= bf16_lo(c); v3 -= bf16_hi(c);
-            }
-        }
-        uint16_t* a = la + buf * PW * LTILE;
-        if constexpr (!PROD) {
-            const float z = word_offset(cs[0]);
+                uint32_t u[4];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float q[8];
-                word_entries(cw[c], q);
-                uint4 v;
-                v.x = pack_bf16(q[0] + z, q[1] + z); v.y = pack_bf16(q[2] + z, q[3] + z);
-                v.z = pack_bf16(q[4] + z, q[5] + z); v.w = pack_bf16(q[6] + z, q[7] + z);
-                *reinterpret_cast<uint4*>(a + (t >> 1) * LROW + ((t & 1) * 2 + c) * 8) = v;
-            }
-            if ((t & 1) == 0) lscale[buf * 128 + (t >> 1)] = word_scale(cs[0]);
-        } else {
-            float q0[8], q1[8];
-            word_entries(cw[0], q0);
-            word_entries(cw[1], q1);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float v0 = word_scale(cs[0]) * (q0[j] + word_offset(cs[0]));
-                const float v1 = word_scale(cs[1]) * (q1[j] + word_offset(cs[1]));
-                const uint32_t hi = pack_bf16(v0, v1);
-                const uint32_t lo = pack_bf16(v0 - bf16_lo(hi), v1 - bf16_hi(hi));
-                *reinterpret_cast<uint32_t*>(a + ((t & 15) * 8 + j) * LROW + (t >> 4) * 2) = hi;
-                *reinterpret_cast<uint32_t*>(a + LTILE + ((t & 15) * 8 + j) * LROW + (t >> 4) * 2) = lo;
+                for (int j = 0; j < 4; ++j) {
+                    u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                    v[2 * j] -= bf16_lo(u[j]);
+                    v[2 * j + 1] -= bf16_hi(u[j]);
+                }
+                fb[c][q] = make_uint4(u[0], u[1], u[2], u[3]);
             }
         }
     };
 
-    f32x16 acc[2][2], part[2][2];
+    f32x4 acc[MT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = part[i][j][e] = 0.f;
-
-    fetch(0);
-    stage(0);
+    for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    fetch_a(kbeg, 0);
+    fetch_x(kbeg);
+    split_x();
+    const int op = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
     for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1;
-        __syncthreads();
-        if (s + 1 < steps) fetch(s + 1);
-        const uint16_t* a = la + buf * PW * LTILE;
-        const uint16_t* b = lb + buf * PX * LTILE;
-        const int at = (lane & 31) * LROW + (lane >> 5) * 8;
+        const int buf = s & 1, k = kbeg + s * BK;
+        __syncthreads();                               // (this step's weights have come, the last step's are done with)
+        if (s + 1 < steps) {
+            fetch_a(k + BK, buf ^ 1);
+            fetch_x(k + BK);
+        }
+        // the next tile's weights and scales are read while this one's are used
+        bf16x8 fa[2][PW];
+        f32x4 sc[2];
+        auto operand = [&](int i) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            bf16x8 fa[PW][2], fb[PX][2];
+            for (int q = 0; q < PW; ++q) fa[i & 1][q] = *reinterpret_cast<const bf16x8*>(lds + buf * STAGE + (q * MT + i) * 1024 + op);
+            if constexpr (!PROD) sc[i & 1] = *reinterpret_cast<const f32x4*>(lscale + buf * SROWS + 16 * i + 4 * (lane >> 4));
+        };
+        operand(0);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < MT; ++i) {
+            if (i + 1 < MT) operand(i + 1);
+            f32x4 part[2];
 #pragma unroll
-                for (int q = 0; q < PW; ++q)
-                    fa[q][i] = *reinterpret_cast<const bf16x8*>(a + q * LTILE + (wm + i * 32) * LROW + at + h * 16);
-#pragma unroll
-                for (int q = 0; q < PX; ++q)
-                    fb[q][i] = *reinterpret_cast<const bf16x8*>(b + q * LTILE + (wn + i * 32) * LROW + at + h * 16);
-            }
+            for (int c = 0; c < 2; ++c) part[c] = PROD ? acc[i][c] : f32x4{0.f, 0.f, 0.f, 0.f};
             // smallest products first
 #pragma unroll
             for (int qx = PX - 1; qx >= 0; --qx)
@@ -480,46 +521,38 @@ __global__ __launch_bounds__(256) void dict4_many_kernel(ManyParams p) {
                 for (int qw = PW - 1; qw >= 0; --qw) {
                     if (qx + qw > 2) continue;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            if constexpr (PROD)
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[qw][i], fb[qx][j], acc[i][j], 0, 0, 0);
-                            else
-                                part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[qw][i], fb[qx][j], part[i][j], 0, 0, 0);
-                        }
+                    for (int c = 0; c < 2; ++c)
+                        part[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1][qw], __builtin_bit_cast(bf16x8, fb[c][qx]), part[c], 0, 0, 0);
                 }
-        }
-        if constexpr (!PROD) {
-            const int k = kbeg + s * BK + BK;
-            if (k % G == 0 || s + 1 == steps) {           // the group ends: its scale
+            if constexpr (PROD) {
+                acc[i][0] = part[0];
+                acc[i][1] = part[1];
+            } else {
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float sc = lscale[buf * 128 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            acc[i][j][e] = fmaf(sc, part[i][j][e], acc[i][j][e]);
-                            part[i][j][e] = 0.f;
-                        }
-                    }
+                    for (int e = 0; e < 4; ++e) acc[i][c][e] = fmaf(sc[i & 1][e], part[c][e], acc[i][c][e]);
+                // (here and now: put off to the step's end, the tiles' sums would fill the registers)
+                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]));
             }
         }
-        if (s + 1 < steps) stage(buf ^ 1);
+        if (s + 1 < steps) split_x();
     }
+    const int n = n0 + 2 * (lane & 15);
+    if (n >= p.N) return;
+    float* out = p.slab ? p.slab + (size_t)blockIdx.y * p.M * p.N : p.out;
+    const int ldo = p.slab ? p.N : p.ldo;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int n = n0 + wn + j * 32 + (lane & 31);
-            if (n >= p.N) continue;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int m = m0 + wm + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-                if (m >= p.M) continue;
-                if (p.slab) p.slab[((size_t)blockIdx.y * p.M + m) * p.N + n] = acc[i][j][e];
-                else p.out[(size_t)m * p.ldo + n] = acc[i][j][e];
+        for (int e = 0; e < 4; ++e) {
+            const int m = m0 + 16 * i + 4 * (lane >> 4) + e;
+            if (m >= p.M) continue;
+            float* dst = out + (size_t)m * ldo + n;
+            if (p.vec_out && n + 1 < p.N) *reinterpret_cast<float2*>(dst) = make_float2(acc[i][0][e], acc[i][1][e]);
+            else {
+                dst[0] = acc[i][0][e];
+                if (n + 1 < p.N) dst[1] = acc[i][1][e];
             }
         }
 }
@@ -552,12 +585,35 @@ int product_few_splits(int d, int r, int ch) {
     splits = std::min(splits, (r + 63) / 64);                       // 16 atoms a wave at least
     return std::max(1, splits);
 }
-int many_splits(int M, int N, int steps, int least) {
-    const long long tiles = (long long)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-    if (tiles >= 256) return 1;
-    long long s = 512 / tiles;
-    s = std::min<long long>(s, steps / least);
-    return (int)std::max<long long>(1, s);
+// Rows of a workgroup's tile (in sixteens) and pieces of the contraction for a product with many columns.  A step
+// of a workgroup costs about 6 matrix instructions a row tile and, whatever its rows, what splitting its columns
+// does; two workgroups are resident per CU.
+struct ManyPlan { int mt, tiles_m, tiles_n, splits, per; size_t a_bytes, s_bytes, slab_bytes; };
+ManyPlan many_plan(bool prod, int d, int r, int b, int group) {
+    ManyPlan q;
+    const int M = prod ? d : r;
+    const int kp = prod ? (r + BK - 1) / BK * BK : (d + group - 1) / group * group;
+    const int steps = kp / BK;
+    q.tiles_n = (b + BN - 1) / BN;
+    long long best = -1;
+    for (int mt = prod ? 8 : 16; mt >= 2; mt /= 2) {       // (the product's weights are two pieces)
+        const long long tiles = (long long)((M + 16 * mt - 1) / (16 * mt)) * q.tiles_n;
+        const long long cost = ((tiles + 511) / 512) * (100 * mt + 400);
+        if (best < 0 || cost < best) {
+            best = cost;
+            q.mt = mt;
+        }
+    }
+    q.tiles_m = (M + 16 * q.mt - 1) / (16 * q.mt);
+    const long long tiles = (long long)q.tiles_m * q.tiles_n;
+    // (few tiles: the contraction is cut, into pieces of at least four steps, never inside a group's 32 features)
+    long long splits = tiles >= 256 ? 1 : std::max<long long>(1, std::min<long long>(512 / tiles, steps / 4));
+    q.per = (int)((steps + splits - 1) / splits);
+    q.splits = (steps + q.per - 1) / q.per;
+    q.a_bytes = ((size_t)(prod ? 2 : 1) * M * kp * 2 + 255) & ~(size_t)255;
+    q.s_bytes = prod ? 0 : ((size_t)(kp / group) * r * sizeof(float) + 255) & ~(size_t)255;
+    q.slab_bytes = q.splits > 1 ? (size_t)q.splits * M * b * sizeof(float) : 0;
+    return q;
 }
 
 template <int NB, int CH, typename T>
@@ -595,27 +651,43 @@ int product_few(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* cod
     return ONMF_OK;
 }
 
-template <bool PROD, typename T, int G>
-int many(onmf_ctx* c, ManyParams p, float* ws, hipStream_t s) {
-    constexpr int PX = sizeof(T) == 4 ? 3 : 1, PW = PROD ? 2 : 1;
-    const size_t bytes = sizeof(uint16_t) * 2 * (PX + PW) * LTILE + (PROD ? 0 : 2 * 128 * sizeof(float));
-    static LdsLimit lim;
-    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_many_kernel<PROD, T, G>, bytes));
-    const int unit = PROD ? BK : std::max(BK, G);                   // a split never cuts a group
-    const int units = ((PROD ? p.K : p.words * 8) + unit - 1) / unit;
-    int splits = many_splits(p.M, p.N, units, std::max(1, 128 / unit));
-    const int per = (units + splits - 1) / splits;
-    splits = (units + per - 1) / per;
-    p.k_per_split = per * unit;
-    p.tiles_m = (p.M + BM - 1) / BM;
-    p.slab = splits > 1 ? ws : nullptr;
-    const int tiles_n = (p.N + BN - 1) / BN;
-    hipLaunchKernelGGL((dict4_many_kernel<PROD, T, G>), dim3(p.tiles_m * tiles_n, splits), dim3(256), bytes, s, p);
+template <bool PROD, typename T>
+int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
+         float* out, int ldo, char* ws, hipStream_t s) {
+    const ManyPlan q = many_plan(PROD, d, r, b, group);
+    const int groups = (d + group - 1) / group, words = groups * (group / 8);
+    ManyParams p;
+    p.A = (const uint16_t*)ws;
+    p.S = (const float*)(ws + q.a_bytes);
+    p.slab = q.splits > 1 ? (float*)(ws + q.a_bytes + q.s_bytes) : nullptr;
+    p.X = X; p.out = out; p.ldx = ldx; p.ldo = ldo; p.group = group;
+    p.M = PROD ? d : r; p.N = b; p.K = PROD ? r : d;
+    p.kp = PROD ? (r + BK - 1) / BK * BK : words * 8;
+    p.tiles_m = q.tiles_m; p.tiles = q.tiles_m * q.tiles_n; p.k_per_split = q.per * BK;
+    p.vec = ((uintptr_t)X & (2 * sizeof(T) - 1)) == 0 && (ldx & 1) == 0 && b % 2 == 0;
+    p.vec_out = p.slab ? b % 2 == 0 : ((uintptr_t)out & 7) == 0 && ldo % 2 == 0;
+    if constexpr (PROD)
+        hipLaunchKernelGGL(dict4_lay_product_kernel, dim3((p.kp + 63) / 64, (words + 15) / 16), dim3(256), 0, s, d, r, words, group,
+                           groups, p.kp, codes, scales, (uint16_t*)ws);
+    else
+        hipLaunchKernelGGL(dict4_lay_correlate_kernel, dim3((unsigned)std::min<size_t>(((size_t)r * words + 255) / 256, 8192)),
+                           dim3(256), 0, s, d, r, words, group, groups, codes, scales, (uint4*)ws, (float*)(ws + q.a_bytes));
+    HIP_TRY(c, hipGetLastError());
+    const dim3 grid((p.tiles + 7) / 8 * 8, q.splits);
+#define MANY_CASE(MT)                                                                                                    \
+    if (q.mt == MT) {                                                                                                    \
+        const size_t bytes = 2 * ((PROD ? 2 : 1) * 16 * MT * 64 + (PROD ? 0 : (16 * MT + 63) / 64 * 64 * sizeof(float)));  \
+        if (p.vec) hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, true>), grid, dim3(256), bytes, s, p);             \
+        else hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, false>), grid, dim3(256), bytes, s, p);                  \
+    }
+    if constexpr (!PROD) { MANY_CASE(16) }
+    MANY_CASE(8) MANY_CASE(4) MANY_CASE(2)
+#undef MANY_CASE
     HIP_TRY(c, hipGetLastError());
     if (p.slab) {
         const size_t mn = (size_t)p.M * p.N;
         hipLaunchKernelGGL(dict4_many_reduce_kernel, dim3((unsigned)std::min<size_t>((mn + 255) / 256, 4096)), dim3(256), 0, s,
-                           mn, p.N, splits, p.slab, p.out, p.ldo);
+                           mn, p.N, q.splits, p.slab, p.out, p.ldo);
         HIP_TRY(c, hipGetLastError());
     }
     return ONMF_OK;
@@ -640,14 +712,7 @@ int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* cod
         FEW_CASE(4, 1); FEW_CASE(4, 2); FEW_CASE(8, 1);
 #undef FEW_CASE
     }
-    ManyParams p = {};
-    p.codes = codes; p.scales = scales; p.X = X; p.out = C;
-    p.M = r; p.N = b; p.K = d; p.ldx = ldx; p.ldo = b;
-    p.group = group; p.groups = (d + group - 1) / group; p.words = p.groups * (group / 8);
-    p.vec = ((uintptr_t)X & (4 * sizeof(T) - 1)) == 0 && (ldx & 3) == 0;
-    if (group == 32) return many<false, T, 32>(c, p, ws, s);
-    if (group == 64) return many<false, T, 64>(c, p, ws, s);
-    return many<false, T, 128>(c, p, ws, s);
+    return many<false, T>(c, d, r, b, group, codes, scales, X, ldx, C, b, (char*)ws, s);
 }
 
 template <typename T>
@@ -660,14 +725,7 @@ int product_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes
         FEW_CASE(4, 1); FEW_CASE(4, 2); FEW_CASE(8, 1);
 #undef FEW_CASE
     }
-    ManyParams p = {};
-    p.codes = codes; p.scales = scales; p.X = H; p.out = R;
-    p.M = d; p.N = b; p.K = r; p.ldx = ldh; p.ldo = ldr;
-    p.group = group; p.groups = (d + group - 1) / group; p.words = p.groups * (group / 8);
-    p.vec = ((uintptr_t)H & (4 * sizeof(T) - 1)) == 0 && (ldh & 3) == 0;
-    if (group == 32) return many<true, T, 32>(c, p, ws, s);
-    if (group == 64) return many<true, T, 64>(c, p, ws, s);
-    return many<true, T, 128>(c, p, ws, s);
+    return many<true, T>(c, d, r, b, group, codes, scales, H, ldh, R, ldr, (char*)ws, s);
 }
 
 }  // namespace
@@ -676,21 +734,12 @@ extern "C" {
 
 size_t onmf_dict4_workspace(int which, int d, int r, int b, int group) {
     if (d <= 0 || r <= 0 || b <= 0 || (group != 32 && group != 64 && group != 128)) return 0;
-    size_t floats = 0;
     if (b <= FEW) {
-        if (which == ONMF_DICT4_PRODUCT) {
-            const int splits = product_few_splits(d, r, few_plan(d, b).ch);
-            if (splits > 1) floats = (size_t)splits * d * b;
-        }
-    } else {
-        const bool prod = which == ONMF_DICT4_PRODUCT;
-        const int unit = prod ? BK : std::max(BK, group);
-        const int K = prod ? r : (d + group - 1) / group * group;
-        const int M = prod ? d : r;
-        const int splits = many_splits(M, b, (K + unit - 1) / unit, std::max(1, 128 / unit));
-        if (splits > 1) floats = (size_t)splits * M * b;
+        const int splits = which == ONMF_DICT4_PRODUCT ? product_few_splits(d, r, few_plan(d, b).ch) : 1;
+        return splits > 1 ? (size_t)splits * d * b * sizeof(float) : 0;
     }
-    return floats * sizeof(float);
+    const ManyPlan q = many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group);
+    return q.a_bytes + q.s_bytes + q.slab_bytes;
 }
 
 int onmf_dict4_pack(onmf_ctx* c, int d, int r, int group, const float* W, void* codes, int32_t* scales, void* stream) {
