@@ -32,9 +32,15 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 __device__ __forceinline__ float bf16_lo(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t p) { return __uint_as_float(p & 0xffff0000u); }
 
+// Bytes as they are: v_cvt_f32_ubyte<n> takes each where it lies (seeing through the mask, the compiler extracts
+// the four bits anew, an instruction more an entry).
+__device__ __forceinline__ void whole_bytes(uint32_t& v) { asm("" : "+v"(v)); }
+
 // the eight whole numbers q of a word
 __device__ __forceinline__ void word_entries(uint32_t w, float (&q)[8]) {
-    const uint32_t e = w & 0x0f0f0f0fu, o = (w >> 4) & 0x0f0f0f0fu;     // bytes of e: entries 0 4 1 5, of o: 2 6 3 7
+    uint32_t e = w & 0x0f0f0f0fu, o = (w >> 4) & 0x0f0f0f0fu;     // bytes of e: entries 0 4 1 5, of o: 2 6 3 7
+    whole_bytes(e);
+    whole_bytes(o);
     q[0] = (float)(e & 0xff);
     q[4] = (float)((e >> 8) & 0xff);
     q[1] = (float)((e >> 16) & 0xff);
@@ -222,20 +228,19 @@ __global__ __launch_bounds__(256) void dict4_correlate_few_kernel(int d, int r, 
 }
 
 // R = W H for up to NB columns: a lane owns F features of a segment and adds up its atoms' contributions
-// h (s q + s z) in registers; the waves of a workgroup and the workgroups of a segment take different atoms and
-// are added in a fixed order (LDS, then slabs).
-template <int NB, int CH, typename T>
-__global__ __launch_bounds__(256) void dict4_product_few_kernel(int d, int r, int b, int group, int groups,
-                                                                 const uint32_t* __restrict__ codes,
-                                                                 const uint32_t* __restrict__ scales,
-                                                                 const T* __restrict__ H, int ldh, float* __restrict__ R,
-                                                                 int ldr, int atoms_per_wg, float* __restrict__ slab) {
-    constexpr int F = 8 * CH, SEG = 64 * F;
-    __shared__ float part[3][NB][SEG];
+// h (s q + s z) in registers; the NW waves of a workgroup take different atoms, AT at a time, and are added in LDS,
+// workgroups of the same segment in slabs; both in a fixed order.
+template <int NB, int CH, int NW, typename T>
+__global__ __launch_bounds__(64 * NW) void dict4_product_few_kernel(int d, int r, int b, int group, int groups,
+                                                                     const uint32_t* __restrict__ codes,
+                                                                     const uint32_t* __restrict__ scales,
+                                                                     const T* __restrict__ H, int ldh, float* __restrict__ R,
+                                                                     int ldr, int atoms_per_wg, float* __restrict__ slab) {
+    constexpr int F = 8 * CH, SEG = 64 * F, AT = 8;
+    __shared__ float part[NW][NB][SEG];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int words = groups * (group / 8);
-    const int w0 = blockIdx.x * (SEG / 8) + lane * CH;
-    const bool there = w0 < words;
+    const int w0 = min((int)(blockIdx.x * (SEG / 8) + lane * CH), words - CH);      // (features behind the last are not stored)
     const int ka = blockIdx.y * atoms_per_wg, kb = min(r, ka + atoms_per_wg);
     float acc[F][NB], zacc[NB];
 #pragma unroll
@@ -244,75 +249,228 @@ __global__ __launch_bounds__(256) void dict4_product_few_kernel(int d, int r, in
 #pragma unroll
         for (int f = 0; f < F; ++f) acc[f][n] = 0.f;
     }
-    const int g = there ? (w0 * 8) / group : 0;
-    if (there)
-#pragma unroll 4
-        for (int k = ka + wave; k < kb; k += 4) {
-            uint32_t cw[CH];
+    const int g = w0 * 8 / group;
+    for (int k0 = ka + wave * AT; k0 < kb; k0 += NW * AT) {
+        uint32_t cw[AT][CH], sc[AT];
+        float h[AT][NB];
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
+            const int k = min(k0 + a, kb - 1);
             const uint32_t* src = codes + (size_t)k * words + w0;
             if constexpr (CH == 4) {
                 const uint4 v = *reinterpret_cast<const uint4*>(src);
-                cw[0] = v.x; cw[1] = v.y; cw[2] = v.z; cw[3] = v.w;
+                cw[a][0] = v.x; cw[a][1] = v.y; cw[a][2] = v.z; cw[a][3] = v.w;
             } else if constexpr (CH == 2) {
                 const uint2 v = *reinterpret_cast<const uint2*>(src);
-                cw[0] = v.x; cw[1] = v.y;
+                cw[a][0] = v.x; cw[a][1] = v.y;
             } else {
-                cw[0] = *src;
+                cw[a][0] = *src;
             }
-            const uint32_t sc = scales[(size_t)k * groups + g];
+            sc[a] = scales[(size_t)k * groups + g];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) h[a][n] = load_val(H + (size_t)k * ldh + min(n, b - 1));
+        }
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
             float hs[NB];
 #pragma unroll
+            for (int n = 0; n < NB; ++n) h[a][n] = k0 + a < kb ? h[a][n] : 0.f;
+#pragma unroll
             for (int n = 0; n < NB; ++n) {
-                hs[n] = word_scale(sc) * load_val(H + (size_t)k * ldh + min(n, b - 1));
-                zacc[n] = fmaf(word_offset(sc), hs[n], zacc[n]);
+                hs[n] = word_scale(sc[a]) * h[a][n];
+                zacc[n] = fmaf(word_offset(sc[a]), hs[n], zacc[n]);
             }
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 float q[8];
-                word_entries(cw[c], q);
+                word_entries(cw[a][c], q);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
                     for (int n = 0; n < NB; ++n) acc[8 * c + j][n] = fmaf(q[j], hs[n], acc[8 * c + j][n]);
             }
         }
-    if (wave > 0)
+    }
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int f = 0; f < F; ++f) part[wave - 1][n][f * 64 + lane] = acc[f][n] + zacc[n];
+        for (int f = 0; f < F; ++f) part[wave][n][f * 64 + lane] = acc[f][n] + zacc[n];
     __syncthreads();
-    if (wave == 0 && there) {
+    for (int e = threadIdx.x; e < NB * SEG; e += 64 * NW) {
+        const int n = e / SEG, at = e % SEG, i = blockIdx.x * SEG + (at & 63) * F + (at >> 6);
+        float v = 0.f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-#pragma unroll
-            for (int f = 0; f < F; ++f) {
-                const float v = ((acc[f][n] + zacc[n]) + part[0][n][f * 64 + lane]) + (part[1][n][f * 64 + lane] + part[2][n][f * 64 + lane]);
-                const int i = w0 * 8 + f;
-                if (i < d && n < b) {
-                    if (slab) slab[((size_t)blockIdx.y * b + n) * d + i] = v;
-                    else R[(size_t)i * ldr + n] = v;
-                }
-            }
+        for (int w = 0; w < NW; ++w) v += part[w][n][at];
+        if (i < d && n < b) {
+            if (slab) slab[((size_t)blockIdx.y * d + i) * b + n] = v;
+            else R[(size_t)i * ldr + n] = v;
         }
     }
 }
 
-// R[i][n] = sum over the slabs z of slab[z][n][i], in order
-__global__ __launch_bounds__(256) void dict4_product_few_reduce_kernel(int d, int b, int splits,
-                                                                        const float* __restrict__ slab,
-                                                                        float* __restrict__ R, int ldr) {
+// R = W H for 3 to 32 columns on the matrix pipe (16x16x32 bfloat16).  A lane takes the words of eight atoms: the
+// eight nibbles at one place are the operand of one row at eight consecutive steps of the contraction, so a tile's
+// 16 rows are the features at that place of the words of 16 lanes, and nothing has to be turned round.  An entry
+// s (q + z) has at most 16 significant bits: its upper half and the rest are bfloat16 values exactly.  Per weight
+// 5.4 vector instructions whatever the number of columns, against 1.4 + one a column on the vector pipe.
+// The waves of a workgroup take different atoms of the same 128 CW features and are added in LDS, workgroups of
+// the same features in slabs; both in a fixed order.
+template <int NT, int CW, typename T>
+__global__ __launch_bounds__(256, 2) void dict4_product_tile_kernel(int d, int r, int b, int group, int groups,
+                                                                  const uint32_t* __restrict__ codes,
+                                                                  const uint32_t* __restrict__ scales,
+                                                                  const T* __restrict__ H, int ldh, float* __restrict__ R,
+                                                                  int ldr, int atoms_per_wg, float* __restrict__ slab) {
+    constexpr int PX = sizeof(T) == 4 ? 3 : 1, TILES = 8 * CW * NT;
+    extern __shared__ __align__(16) float part[];             // [4 waves][TILES][64 lanes][4]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, kg = lane >> 4;
+    const int words = groups * (group / 8);
+    const int w0 = min((int)(blockIdx.x * 16 + m) * CW, words - CW);           // (rows behind the last are not stored)
+    const int g = w0 * 8 / group;
+    const int ka = blockIdx.y * atoms_per_wg, kb = min(r, ka + atoms_per_wg);
+    f32x4 acc[CW][8][NT];
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[c][j][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Raw { uint32_t cw[8][CW], sc[8]; float h[8][NT]; };
+    auto fetch = [&](int k0, Raw& x) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int k = min(k0 + kg * 8 + j, r - 1);
+            const uint32_t* src = codes + (size_t)k * words + w0;
+            if constexpr (CW == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(src);
+                x.cw[j][0] = v.x; x.cw[j][1] = v.y;
+            } else {
+                x.cw[j][0] = *src;
+            }
+            x.sc[j] = scales[(size_t)k * groups + g];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) x.h[j][n] = load_val(H + (size_t)k * ldh + min(16 * n + m, b - 1));
+        }
+    };
+    auto compute = [&](int k0, Raw& x) {
+        uint4 fb[NT][PX];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k0 + kg * 8 + j < kb ? x.h[j][n] : 0.f;
+#pragma unroll
+            for (int q = 0; q < PX; ++q) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                    v[2 * j] -= bf16_lo(u[j]);
+                    v[2 * j + 1] -= bf16_hi(u[j]);
+                }
+                fb[n][q] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+        }
+        float s[8], zs[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            s[j] = word_scale(x.sc[j]);
+            zs[j] = s[j] * word_offset(x.sc[j]);
+        }
+#pragma unroll
+        for (int c = 0; c < CW; ++c)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t nib[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    nib[j] = (half ? x.cw[j][c] >> 4 : x.cw[j][c]) & 0x0f0f0f0fu;
+                    whole_bytes(nib[j]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int entry = 2 * half + (q >> 1) + 4 * (q & 1);       // bytes: entries 0 4 1 5, then 2 6 3 7
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float v0 = fmaf((float)((nib[2 * j] >> (8 * q)) & 0xff), s[2 * j], zs[2 * j]);
+                        const float v1 = fmaf((float)((nib[2 * j + 1] >> (8 * q)) & 0xff), s[2 * j + 1], zs[2 * j + 1]);
+                        const uint32_t b0 = __float_as_uint(v0), b1 = __float_as_uint(v1);
+                        hi[j] = __builtin_amdgcn_perm(b1, b0, 0x07060302u);
+                        lo[j] = __builtin_amdgcn_perm(__float_as_uint(v1 - __uint_as_float(b1 & 0xffff0000u)),
+                                                      __float_as_uint(v0 - __uint_as_float(b0 & 0xffff0000u)), 0x07060302u);
+                    }
+                    const bf16x8 ahi = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                    const bf16x8 alo = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                    // smallest products first; of the six the last (2^-24) is left out
+#pragma unroll
+                    for (int qx = PX - 1; qx >= 0; --qx)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const bf16x8 f = __builtin_bit_cast(bf16x8, fb[n][qx]);
+                            if (qx < 2) acc[c][entry][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(alo, f, acc[c][entry][n], 0, 0, 0);
+                            acc[c][entry][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ahi, f, acc[c][entry][n], 0, 0, 0);
+                        }
+                    // (here and now: all entries unpacked first would fill the registers)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) asm volatile("" : "+v"(acc[c][entry][n]));
+                }
+            }
+    };
+    Raw even, odd;
+    int k0 = ka + wave * 32;
+    if (k0 < kb) fetch(k0, even);
+    while (k0 < kb) {
+        if (k0 + 128 < kb) fetch(k0 + 128, odd);
+        compute(k0, even);
+        k0 += 128;
+        if (k0 >= kb) break;
+        if (k0 + 128 < kb) fetch(k0 + 128, even);
+        compute(k0, odd);
+        k0 += 128;
+    }
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                *reinterpret_cast<f32x4*>(part + ((size_t)(wave * TILES + (c * 8 + j) * NT + n) * 64 + lane) * 4) = acc[c][j][n];
+    __syncthreads();
+#pragma unroll 4
+    for (int ti = wave; ti < TILES; ti += 4) {
+        f32x4 v = *reinterpret_cast<const f32x4*>(part + ((size_t)ti * 64 + lane) * 4);
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(part + ((size_t)(w * TILES + ti) * 64 + lane) * 4);
+        const int n = ti % NT * 16 + (lane & 15), j = ti / NT % 8, c = ti / NT / 8;
+        if (n >= b) continue;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = (((int)blockIdx.x * 16 + 4 * (lane >> 4) + e) * CW + c) * 8 + j;
+            if (i >= d) continue;
+            if (slab) slab[((size_t)blockIdx.y * d + i) * b + n] = v[e];
+            else R[(size_t)i * ldr + n] = v[e];
+        }
+    }
+}
+
+// out[m][n] = sum over the slabs z of slab[z][m][n], four threads an entry, in a fixed order
+__global__ __launch_bounds__(256) void dict4_reduce_kernel(size_t mn, int N, int splits, const float* __restrict__ slab,
+                                                            float* __restrict__ out, int ldo) {
     __shared__ float part[4][64];
     const int o = threadIdx.x & 63, g = threadIdx.x >> 6;
-    const size_t e = (size_t)blockIdx.x * 64 + o, all = (size_t)d * b;
-    float s = 0.f;
-    if (e < all)
-        for (int z = g; z < splits; z += 4) s += slab[(size_t)z * all + e];
-    part[g][o] = s;
-    __syncthreads();
-    if (g == 0 && e < all) {
-        const int n = (int)(e / d), i = (int)(e % d);
-        R[(size_t)i * ldr + n] = (part[0][o] + part[1][o]) + (part[2][o] + part[3][o]);
+    for (size_t base = (size_t)blockIdx.x * 64; base < mn; base += (size_t)gridDim.x * 64) {
+        const size_t e = base + o;
+        float s = 0.f;
+        if (e < mn) {
+#pragma unroll 8
+            for (int z = g; z < splits; z += 4) s += slab[(size_t)z * mn + e];
+        }
+        part[g][o] = s;
+        __syncthreads();
+        if (g == 0 && e < mn) out[(e / N) * (size_t)ldo + e % N] = (part[0][o] + part[1][o]) + (part[2][o] + part[3][o]);
+        __syncthreads();
     }
 }
 
@@ -557,19 +715,10 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
         }
 }
 
-__global__ __launch_bounds__(256) void dict4_many_reduce_kernel(size_t mn, int N, int splits,
-                                                                 const float* __restrict__ slab, float* __restrict__ out,
-                                                                 int ldo) {
-    for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < mn; e += (size_t)gridDim.x * 256) {
-        float s = 0.f;
-        for (int z = 0; z < splits; ++z) s += slab[(size_t)z * mn + e];
-        out[(e / N) * (size_t)ldo + e % N] = s;
-    }
-}
-
 // ------------------------------------------------------------------------------------------- launches
 constexpr int MOST_COLS = 2147483647 - 1024;    // tile arithmetic in int
-constexpr int FEW = 8;           // columns up to which the few-column kernels run
+constexpr int FEW = 8, FEW_PRODUCT = 2;     // columns up to which the vector kernels run
+constexpr int TILE_PRODUCT = 32;             // ... and the product's tile kernel
 
 struct FewPlan { int nb, ch; };
 FewPlan few_plan(int d, int b) {
@@ -579,11 +728,18 @@ FewPlan few_plan(int d, int b) {
     while (f.ch > 1 && d <= 64 * 8 * (f.ch / 2)) f.ch /= 2;         // one segment is enough with narrower lanes
     return f;
 }
-int product_few_splits(int d, int r, int ch) {
-    const int segs = (d + 512 * ch - 1) / (512 * ch);
-    int splits = std::max(1, 512 / segs);
-    splits = std::min(splits, (r + 63) / 64);                       // 16 atoms a wave at least
-    return std::max(1, splits);
+// The vector kernel's split of the atoms.  Up to 512 atoms one workgroup of 16 waves takes them all, in one launch
+// with nothing to add up behind it.
+struct FewProduct { bool one; int ch, segs, splits, per; };
+FewProduct product_few_plan(int d, int r, int b) {
+    FewProduct q;
+    q.one = r <= 512;
+    q.ch = q.one ? 1 : few_plan(d, b).ch;
+    q.segs = (d + 512 * q.ch - 1) / (512 * q.ch);
+    const int splits = q.one ? 1 : std::max(1, std::min(1024 / q.segs, r / 128));      // 32 atoms a wave at least
+    q.per = ((r + splits - 1) / splits + 31) / 32 * 32;
+    q.splits = (r + q.per - 1) / q.per;
+    return q;
 }
 // Rows of a workgroup's tile (in sixteens) and pieces of the contraction for a product with many columns.  A step
 // of a workgroup costs about 6 matrix instructions a row tile and, whatever its rows, what splitting its columns
@@ -616,6 +772,13 @@ ManyPlan many_plan(bool prod, int d, int r, int b, int group) {
     return q;
 }
 
+int add_slabs(onmf_ctx* c, size_t mn, int N, int splits, const float* slab, float* out, int ldo, hipStream_t s) {
+    hipLaunchKernelGGL(dict4_reduce_kernel, dim3((unsigned)std::min<size_t>((mn + 63) / 64, 16384)), dim3(256), 0, s, mn, N,
+                       splits, slab, out, ldo);
+    HIP_TRY(c, hipGetLastError());
+    return ONMF_OK;
+}
+
 template <int NB, int CH, typename T>
 int correlate_few(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales,
                   const T* X, int ldx, float* C, hipStream_t s) {
@@ -632,23 +795,40 @@ int correlate_few(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* c
     return ONMF_OK;
 }
 
-template <int NB, int CH, typename T>
-int product_few(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* H,
-                int ldh, float* R, int ldr, float* ws, hipStream_t s) {
-    const int groups = (d + group - 1) / group, segs = (d + 512 * CH - 1) / (512 * CH);
-    int splits = product_few_splits(d, r, CH);
-    const int per = (r + splits - 1) / splits;
-    splits = (r + per - 1) / per;
-    float* slab = splits > 1 ? ws : nullptr;
-    hipLaunchKernelGGL((dict4_product_few_kernel<NB, CH, T>), dim3(segs, splits), dim3(256), 0, s, d, r, b, group, groups,
-                       codes, scales, H, ldh, R, ldr, per, slab);
+template <int NB, int CH, int NW, typename T>
+int product_few(onmf_ctx* c, const FewProduct& q, int d, int r, int b, int group, const uint32_t* codes,
+                const uint32_t* scales, const T* H, int ldh, float* R, int ldr, float* ws, hipStream_t s) {
+    float* slab = q.splits > 1 ? ws : nullptr;
+    hipLaunchKernelGGL((dict4_product_few_kernel<NB, CH, NW, T>), dim3(q.segs, q.splits), dim3(64 * NW), 0, s, d, r, b, group,
+                       (d + group - 1) / group, codes, scales, H, ldh, R, ldr, q.per, slab);
     HIP_TRY(c, hipGetLastError());
-    if (slab) {
-        hipLaunchKernelGGL(dict4_product_few_reduce_kernel, dim3(((size_t)d * b + 63) / 64), dim3(256), 0, s, d, b, splits,
-                           slab, R, ldr);
-        HIP_TRY(c, hipGetLastError());
-    }
-    return ONMF_OK;
+    return slab ? add_slabs(c, (size_t)d * b, b, q.splits, slab, R, ldr, s) : ONMF_OK;
+}
+
+// The tile kernel's split of the atoms: two workgroups a CU (what its registers allow), 128 atoms (a step of each wave) at least.
+struct TilePlan { int nt, cw, blocks, splits, per; };
+TilePlan product_tile_plan(int d, int r, int b, int group) {
+    TilePlan q;
+    q.nt = b <= 16 ? 1 : 2;
+    q.cw = q.nt == 1 ? 2 : 1;
+    const int words = (d + group - 1) / group * (group / 8), steps = (r + 127) / 128;
+    q.blocks = (words + 16 * q.cw - 1) / (16 * q.cw);
+    const int splits = std::max(1, std::min(steps, 512 / q.blocks));
+    q.per = (steps + splits - 1) / splits * 128;
+    q.splits = (r + q.per - 1) / q.per;
+    return q;
+}
+template <int NT, int CW, typename T>
+int product_tile(onmf_ctx* c, const TilePlan& q, int d, int r, int b, int group, const uint32_t* codes,
+                 const uint32_t* scales, const T* H, int ldh, float* R, int ldr, float* ws, hipStream_t s) {
+    constexpr size_t bytes = 4 * 8 * CW * NT * 64 * 4 * sizeof(float);
+    static LdsLimit lim;
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_product_tile_kernel<NT, CW, T>, bytes));
+    float* slab = q.splits > 1 ? ws : nullptr;
+    hipLaunchKernelGGL((dict4_product_tile_kernel<NT, CW, T>), dim3(q.blocks, q.splits), dim3(256), bytes, s, d, r, b, group,
+                       (d + group - 1) / group, codes, scales, H, ldh, R, ldr, q.per, slab);
+    HIP_TRY(c, hipGetLastError());
+    return slab ? add_slabs(c, (size_t)d * b, b, q.splits, slab, R, ldr, s) : ONMF_OK;
 }
 
 template <bool PROD, typename T>
@@ -684,12 +864,7 @@ int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, con
     MANY_CASE(8) MANY_CASE(4) MANY_CASE(2)
 #undef MANY_CASE
     HIP_TRY(c, hipGetLastError());
-    if (p.slab) {
-        const size_t mn = (size_t)p.M * p.N;
-        hipLaunchKernelGGL(dict4_many_reduce_kernel, dim3((unsigned)std::min<size_t>((mn + 255) / 256, 4096)), dim3(256), 0, s,
-                           mn, p.N, q.splits, p.slab, p.out, p.ldo);
-        HIP_TRY(c, hipGetLastError());
-    }
+    if (p.slab) return add_slabs(c, (size_t)p.M * p.N, p.N, q.splits, p.slab, p.out, p.ldo, s);
     return ONMF_OK;
 }
 
@@ -718,12 +893,19 @@ int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* cod
 template <typename T>
 int product_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* H,
               int ldh, float* R, int ldr, float* ws, hipStream_t s) {
-    if (b <= FEW) {
-        const FewPlan f = few_plan(d, b);
-#define FEW_CASE(NB, CH) if (f.nb == NB && f.ch == CH) return product_few<NB, CH, T>(c, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s)
+    if (b <= FEW_PRODUCT) {
+        const FewProduct q = product_few_plan(d, r, b);
+#define FEW_CASE(NB, CH) \
+    if (b <= NB && q.ch == CH && !q.one) return product_few<NB, CH, 4, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s)
+        if (q.one && b == 1) return product_few<1, 1, 16, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
+        if (q.one) return product_few<2, 1, 16, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
         FEW_CASE(1, 1); FEW_CASE(1, 2); FEW_CASE(1, 4); FEW_CASE(2, 1); FEW_CASE(2, 2); FEW_CASE(2, 4);
-        FEW_CASE(4, 1); FEW_CASE(4, 2); FEW_CASE(8, 1);
 #undef FEW_CASE
+    }
+    if (b <= TILE_PRODUCT) {
+        const TilePlan q = product_tile_plan(d, r, b, group);
+        if (q.nt == 1) return product_tile<1, 2, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
+        return product_tile<2, 1, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
     }
     return many<true, T>(c, d, r, b, group, codes, scales, H, ldh, R, ldr, (char*)ws, s);
 }
@@ -734,10 +916,11 @@ extern "C" {
 
 size_t onmf_dict4_workspace(int which, int d, int r, int b, int group) {
     if (d <= 0 || r <= 0 || b <= 0 || (group != 32 && group != 64 && group != 128)) return 0;
-    if (b <= FEW) {
-        const int splits = which == ONMF_DICT4_PRODUCT ? product_few_splits(d, r, few_plan(d, b).ch) : 1;
+    if (which == ONMF_DICT4_PRODUCT && b <= TILE_PRODUCT) {
+        const int splits = b <= FEW_PRODUCT ? product_few_plan(d, r, b).splits : product_tile_plan(d, r, b, group).splits;
         return splits > 1 ? (size_t)splits * d * b * sizeof(float) : 0;
     }
+    if (which != ONMF_DICT4_PRODUCT && b <= FEW) return 0;
     const ManyPlan q = many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group);
     return q.a_bytes + q.s_bytes + q.slab_bytes;
 }
