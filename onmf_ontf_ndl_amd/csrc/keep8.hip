@@ -14,6 +14,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 namespace {
 
 constexpr int GROUP = 128;
+constexpr size_t MOST_GROUPS = (size_t)1 << 33;
 constexpr int MOST_COLS = 1 << 28;       // eight rows' codes lie within 32 bits
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
@@ -24,75 +25,132 @@ __device__ __forceinline__ float load_val(const uint16_t* p) { return bf16_to_f3
 // Whole q nearest to v / s with ties to even, decided exactly: the remainder v - s q is a multiple of half an
 // ulp of s and below 2^24 of them, so the fused multiply-add gives it without rounding and a quotient next to
 // a half falls on its own side whatever the reciprocal's rounding.
-__device__ __forceinline__ int nearest(float v, float s, float inv) {
-    float q = rintf(v * inv);
+__device__ __forceinline__ float nearest(float v, float s, float q) {
     const float rest = 2.f * fmaf(-q, s, v);
     const bool odd = ((int)q & 1) != 0;
     if (rest > s || (rest == s && odd)) q += 1.f;
     else if (rest < -s || (rest == -s && odd)) q -= 1.f;
-    return (int)q;
+    return q;
 }
 
-// 32 lanes per group, four columns a lane.
-template <typename T>
-__global__ __launch_bounds__(256) void keep8_kernel(int d, int n, int groups, const T* __restrict__ X, int ldx, int vec,
+// the largest value of 16 lanes, in all of them
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true));      // lanes 1 apart
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true));      // 2
+    v = max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true));     // the halves of 8
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, true));  // the halves of 16
+}
+
+// row and group of the first of the groups a thread handles, moved on one at a time (one division a thread)
+template <typename I>
+struct GroupAt {
+    I row, g, groups;
+    __device__ __forceinline__ GroupAt(I at, I n) : row(at / n), g(at % n), groups(n) {}
+    __device__ __forceinline__ void next() { if (++g == groups) { g = 0; ++row; } }
+};
+
+// 16 lanes per group, eight columns a lane, U groups a lane (their loads are on their way together).  Bound by
+// memory: 5 bytes a float32 entry, 3 a bfloat16 one.
+template <typename T, typename I, int U>
+__global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int groups, const T* __restrict__ X, int ldx, int vec,
                                                      int8_t* __restrict__ codes, float* __restrict__ scales) {
-    const size_t all = (size_t)d * groups;
-    for (size_t at = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); at < all; at += (size_t)gridDim.x * 8) {
-        const int row = (int)(at / groups), g = (int)(at % groups);
-        const int c = g * GROUP + (threadIdx.x & 31) * 4;
-        const T* src = X + (size_t)row * ldx + c;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (vec && c + 3 < n) {
+    const int lane = threadIdx.x & 15;
+    const size_t first = ((size_t)blockIdx.x * 16 + (threadIdx.x >> 4)) * U;
+    if (first >= all) return;
+    GroupAt<I> at((I)first, (I)groups);
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u, at.next()) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = 0.f;
+        if (first + u >= all) continue;
+        const int c = (int)at.g * GROUP + lane * 8;
+        const T* src = X + (size_t)at.row * ldx + c;
+        if (vec && c + 7 < n) {
             if constexpr (sizeof(T) == 4) {
-                const float4 f = *reinterpret_cast<const float4*>(src);
-                v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+                const float4 f = reinterpret_cast<const float4*>(src)[0], h = reinterpret_cast<const float4*>(src)[1];
+                v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w;
+                v[u][4] = h.x; v[u][5] = h.y; v[u][6] = h.z; v[u][7] = h.w;
             } else {
-                const uint2 u = *reinterpret_cast<const uint2*>(src);
-                v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-                v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
+                const uint4 w = *reinterpret_cast<const uint4*>(src);
+                const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[u][2 * j] = __uint_as_float(p[j] << 16);
+                    v[u][2 * j + 1] = __uint_as_float(p[j] & 0xffff0000u);
+                }
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c + j < n) v[j] = load_val(src + j);
+            for (int j = 0; j < 8; ++j)
+                if (c + j < n) v[u][j] = load_val(src + j);
         }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (first + u >= all) break;
         // the largest magnitude by its bits: a NaN's are above an infinity's, an infinity's above all others
         uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) most = max(most, __float_as_uint(v[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o, 64));
+        for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[u][j]) & 0x7fffffffu);
+        most = max16(most);
         float s = __uint_as_float(most) / 127.f;
-        int q[4] = {0, 0, 0, 0};
+        float q[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = 0.f;
         if (most >= 0x7f800000u) {
             s = __uint_as_float(0x7fc00000u);            // a NaN or an infinity: the whole group reads NaN
         } else if (s < 1.17549435e-38f) {
             s = 0.f;                                       // nothing but (next to) zeros
         } else {
-            const float inv = 1.f / s;
+            // v times the reciprocal (1 ulp) is within 127 (2^-23 + 2^-24) = 2.3e-5 of the quotient: only where it lies
+            // that near to a half is the remainder asked
+            const float inv = __builtin_amdgcn_rcpf(s);
+            float off = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = nearest(v[j], s, inv);
+            for (int j = 0; j < 8; ++j) {
+                const float f = v[u][j] * inv;
+                q[j] = rintf(f);
+                off = fmaxf(off, fabsf(f - q[j]));
+            }
+            if (off > 0.49997f) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = nearest(v[u][j], s, q[j]);
+            }
         }
-        *reinterpret_cast<uint32_t*>(codes + (size_t)row * groups * GROUP + c) =
-            (uint32_t)(q[0] & 0xff) | (uint32_t)(q[1] & 0xff) << 8 | (uint32_t)(q[2] & 0xff) << 16 | (uint32_t)(q[3] & 0xff) << 24;
-        if ((threadIdx.x & 31) == 0) scales[at] = s;
+        uint32_t word[2] = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) word[j >> 2] |= ((uint32_t)(int)q[j] & 0xff) << (8 * (j & 3));
+        // (a row's groups follow one another in both outputs: group `first + u` of all)
+        *reinterpret_cast<uint2*>(codes + (first + u) * GROUP + lane * 8) = make_uint2(word[0], word[1]);
+        if (lane == 0) scales[first + u] = s;
     }
 }
 
 // ------------------------------------------------------------------------------------------- bring back
-__global__ __launch_bounds__(256) void keep8_expand_kernel(int d, int n, int groups, const int8_t* __restrict__ codes,
+template <typename I, int U>
+__global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, int groups, const int8_t* __restrict__ codes,
                                                             const float* __restrict__ scales, float* __restrict__ X,
                                                             int ldx, int vec) {
-    const size_t all = (size_t)d * groups;
-    for (size_t at = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5); at < all; at += (size_t)gridDim.x * 8) {
-        const int row = (int)(at / groups), g = (int)(at % groups);
-        const int c = g * GROUP + (threadIdx.x & 31) * 4;
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + (size_t)row * groups * GROUP + c);
-        const float s = scales[at];
-        const float4 v = make_float4(s * (float)(int8_t)(w & 0xff), s * (float)(int8_t)((w >> 8) & 0xff),
-                                     s * (float)(int8_t)((w >> 16) & 0xff), s * (float)(int8_t)(w >> 24));
-        float* dst = X + (size_t)row * ldx + c;
+    const int lane = threadIdx.x & 31;
+    const size_t first = ((size_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
+    if (first >= all) return;
+    uint32_t w[U];
+    float s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const size_t at = min(first + u, all - 1);
+        w[u] = *reinterpret_cast<const uint32_t*>(codes + at * GROUP + lane * 4);
+        s[u] = scales[at];
+    }
+    GroupAt<I> at((I)first, (I)groups);
+#pragma unroll
+    for (int u = 0; u < U; ++u, at.next()) {
+        if (first + u >= all) break;
+        const int c = (int)at.g * GROUP + lane * 4;
+        const float4 v = make_float4(s[u] * (float)(int8_t)(w[u] & 0xff), s[u] * (float)(int8_t)((w[u] >> 8) & 0xff),
+                                     s[u] * (float)(int8_t)((w[u] >> 16) & 0xff), s[u] * (float)(int8_t)(w[u] >> 24));
+        float* dst = X + (size_t)at.row * ldx + c;
         if (vec && c + 3 < n) {
             *reinterpret_cast<float4*>(dst) = v;
         } else {
@@ -463,8 +521,31 @@ int run_reduce(onmf_ctx* c, const SumPlan& q, int d, int r, const float* slab, d
     return ONMF_OK;
 }
 
-unsigned group_blocks(int d, int n) {
-    return (unsigned)std::min<size_t>(((size_t)d * ((n + GROUP - 1) / GROUP) + 7) / 8, 8192);
+// Groups a thread handles: several where there are enough of them to fill the chip with.  32-bit group numbers where
+// they do (a division in 64 bits costs as much as everything else).
+template <typename T, typename I>
+void launch_keep_as(size_t all, int n, int groups, const T* X, int ldx, int vec, int8_t* codes, float* scales, hipStream_t s) {
+    if (all >= 65536)
+        hipLaunchKernelGGL((keep8_kernel<T, I, 2>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, X, ldx,
+                           vec, codes, scales);
+    else
+        hipLaunchKernelGGL((keep8_kernel<T, I, 1>), dim3((unsigned)((all + 15) / 16)), dim3(256), 0, s, all, n, groups, X, ldx,
+                           vec, codes, scales);
+}
+template <typename T>
+void launch_keep(size_t all, int n, int groups, const T* X, int ldx, int vec, int8_t* codes, float* scales, hipStream_t s) {
+    if (all < 0x7fffffffu) launch_keep_as<T, uint32_t>(all, n, groups, X, ldx, vec, codes, scales, s);
+    else launch_keep_as<T, uint64_t>(all, n, groups, X, ldx, vec, codes, scales, s);
+}
+template <typename I>
+void launch_expand(size_t all, int n, int groups, const int8_t* codes, const float* scales, float* X, int ldx, int vec,
+                   hipStream_t s) {
+    if (all >= 65536)
+        hipLaunchKernelGGL((keep8_expand_kernel<I, 4>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, codes,
+                           scales, X, ldx, vec);
+    else
+        hipLaunchKernelGGL((keep8_expand_kernel<I, 1>), dim3((unsigned)((all + 7) / 8)), dim3(256), 0, s, all, n, groups, codes,
+                           scales, X, ldx, vec);
 }
 
 }  // namespace
@@ -480,13 +561,11 @@ int onmf_keep8(onmf_ctx* c, int d, int n, const void* X, int x_type, int ldx, in
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
     const size_t es = x_type == ONMF_TYPE_F32 ? 4 : 2;
-    const int vec = ((uintptr_t)X & (4 * es - 1)) == 0 && (ldx & 3) == 0;
-    if (x_type == ONMF_TYPE_F32)
-        hipLaunchKernelGGL(keep8_kernel<float>, dim3(group_blocks(d, n)), dim3(256), 0, s, d, n, groups, (const float*)X, ldx,
-                           vec, codes, scales);
-    else
-        hipLaunchKernelGGL(keep8_kernel<uint16_t>, dim3(group_blocks(d, n)), dim3(256), 0, s, d, n, groups,
-                           (const uint16_t*)X, ldx, vec, codes, scales);
+    const int vec = ((uintptr_t)X & 15) == 0 && (ldx * es) % 16 == 0;
+    const size_t all = (size_t)d * groups;
+    if (all > MOST_GROUPS) return onmf_fail(c, ONMF_ERR_ARG, "keep8: %d x %d is more than 2^33 groups", d, n);
+    if (x_type == ONMF_TYPE_F32) launch_keep(all, n, groups, (const float*)X, ldx, vec, codes, scales, s);
+    else launch_keep(all, n, groups, (const uint16_t*)X, ldx, vec, codes, scales, s);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -500,12 +579,17 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
+    const size_t all = (size_t)d * groups;
+    const int vec = ((uintptr_t)X & 15) == 0 && (ldx & 3) == 0;
     if (idx)
         hipLaunchKernelGGL(keep8_gather_kernel, dim3((b + 255) / 256, std::min(d, 4096)), dim3(256), 0, s, d, n, groups, codes,
                            scales, (const long long*)idx, b, X, ldx);
+    else if (all > MOST_GROUPS)
+        return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: %d x %d is more than 2^33 groups", d, n);
+    else if (all < 0x7fffffffu)
+        launch_expand<uint32_t>(all, n, groups, codes, scales, X, ldx, vec, s);
     else
-        hipLaunchKernelGGL(keep8_expand_kernel, dim3(group_blocks(d, n)), dim3(256), 0, s, d, n, groups, codes, scales, X, ldx,
-                           (int)(((uintptr_t)X & 15) == 0 && (ldx & 3) == 0));
+        launch_expand<uint64_t>(all, n, groups, codes, scales, X, ldx, vec, s);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
