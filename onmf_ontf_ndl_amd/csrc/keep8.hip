@@ -193,7 +193,10 @@ template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
     static constexpr int mi = MI, nj = NJ, wm = WM_, wn = WN_, stages = STAGES;
     static constexpr int bm = 16 * MI * WM_, bn = 16 * NJ * WN_, waves = WM_ * WN_;
     static constexpr int rows = (bm + bn + 8 * waves - 1) / (8 * waves) * (8 * waves);     // of a stage: every wave loads as many
-    static constexpr int srows = (bm + bn + 16 * waves - 1) / (16 * waves) * (16 * waves);  // the same for the scales
+    // scales come sg groups at a time, sg lanes to a row (more groups than there are stages: see the waits)
+    static constexpr int sg = STAGES <= 4 ? 4 : 8, sper = 64 / sg * waves;
+    static constexpr int srows = (bm + bn + sper - 1) / sper * sper;
+    static_assert(STAGES <= sg && bm % (64 / sg) == 0 && bm % 8 == 0, "");
 };
 
 struct SumParams {
@@ -203,12 +206,17 @@ struct SumParams {
     int d, r, groups, per_split, splits;
     int tiles_m, tiles_h, tiles;     // tiles along r (rows); column tiles of the H H^T part; all tiles
     int cols_h, cols;         // columns of a slab row: the H H^T part's, all (both multiples of 4)
+    // one run holds everything: the results at once, A and B or (the gradient) Ad and Bd
+    double w, keep;
+    const float *A_in, *B_in;
+    float *A, *B;
+    double *Ad, *Bd;
 };
 
 template <typename S>
 __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) {
     constexpr int STAGES = S::stages, AHEAD = STAGES - 1, STAGE = S::rows * GROUP;
-    extern __shared__ __align__(16) int8_t lds[];            // [STAGES][STAGE], then float [2][S::srows][4]
+    extern __shared__ __align__(16) int8_t lds[];            // [STAGES][STAGE], then float [2][S::srows][SG]
     float* lsc = (float*)(lds + STAGES * STAGE);
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     // workgroups of one run share H's codes: they follow each other on one XCD (workgroups go to the XCDs in turn,
@@ -227,10 +235,10 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
     const int g0 = split * p.per_split, g1 = min(p.groups, g0 + p.per_split);
     const int wm = (wave % S::wm) * 16 * S::mi, wn = (wave / S::wm) * 16 * S::nj;
 
-    // A wave's loads are eight rows each, dealt out to the waves in turn; scales come four groups at a time, four
-    // lanes to a row (a row's are 4 bytes a group: taken one group at a time they were as many requests as the
-    // codes): [row][4].  Addresses: a base for the wave and 32 bits a lane.
-    constexpr int NW = S::waves, LOADS = S::rows / 8 / NW, SLOADS = S::srows / 16 / NW;
+    // A wave's loads are eight rows each, dealt out to the waves in turn; scales come SG groups at a time, SG lanes to
+    // a row (a row's are 4 bytes a group: taken one group at a time they were as many requests as the codes):
+    // [row][SG].  Addresses: a base for the wave and 32 bits a lane.
+    constexpr int NW = S::waves, LOADS = S::rows / 8 / NW, SLOADS = S::srows / S::sper, SG = S::sg;
     auto rows_of = [&](int row, int& first, int& last) {         // the matrix row at row `row` of a stage, and the last there is
         const bool of_h = row < S::bm;
         last = of_h ? p.r - 1 : N - 1;
@@ -253,9 +261,9 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
 #pragma unroll
     for (int j = 0; j < SLOADS; ++j) {
         int first, last;
-        sbase[j] = rows_of((j * NW + wave) * 16, first, last) ? p.hs : bs;
+        sbase[j] = rows_of((j * NW + wave) * (64 / SG), first, last) ? p.hs : bs;
         sbase[j] += (size_t)first * p.groups;
-        soff[j] = (uint32_t)(min(first + (lane >> 2), last) - first) * (uint32_t)p.groups * 4;
+        soff[j] = (uint32_t)(min(first + lane / SG, last) - first) * (uint32_t)p.groups * 4;
     }
     auto fetch = [&](int g, int buf) {
 #pragma unroll
@@ -265,11 +273,11 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
                                              16, 0, 0);
     };
     auto fetch_scales = [&](int g, int half) {
-        const uint32_t q = (uint32_t)min(lane & 3, p.groups - 1 - g) * 4;
+        const uint32_t q = (uint32_t)min(lane % SG, p.groups - 1 - g) * 4;
 #pragma unroll
         for (int j = 0; j < SLOADS; ++j)
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)((const char*)(sbase[j] + g) + (soff[j] + q)),
-                                             (__attribute__((address_space(3))) void*)(lsc + half * 4 * S::srows + (j * NW + wave) * 64),
+                                             (__attribute__((address_space(3))) void*)(lsc + half * SG * S::srows + (j * NW + wave) * 64),
                                              4, 0, 0);
     };
 
@@ -281,8 +289,8 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
     // where a lane's operands and scales lie in a stage (whole tiles of 16 rows further on the chunks lie alike)
     const int op0 = (wm + (lane & 15)) * GROUP + (((lane >> 4) ^ ((lane >> 1) & 7)) * 16), op1 = op0 ^ 64;
     const int ba = (S::bm + wn - wm) * GROUP;
-    const int sc_h = 4 * (wm + (lane & 15)), sc_x = 4 * (S::bm + wn + 4 * (lane >> 4));
-    // AHEAD groups are on their way while one is computed, and the scales of the next four.  Loads come back in order:
+    const int sc_h = SG * (wm + (lane & 15)), sc_x = SG * (S::bm + wn + 4 * (lane >> 4));
+    // AHEAD groups are on their way while one is computed, and the scales of the next SG.  Loads come back in order:
     // with only what was sent behind this group's codes still out - the codes of the AHEAD - 1 groups behind it, and
     // the scales where a fetch of them lies in between - this one's have arrived; behind the barrier those of all
     // waves have, and all waves are done with the group before, whose place the next one sent for takes.
@@ -293,18 +301,18 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
         if (k < n) fetch(g0 + k, k);
     int buf = 0;
     for (int k = 0; k < n; ++k) {
-        // (step i sent for scales where i is a multiple of four and group i + 4 is there)
-        const int i = (k - 1) & ~3;
-        const bool scales_out = i >= k - AHEAD && i >= 0 && i + 4 < n;
+        // (step i sent for scales where i is a multiple of SG and group i + SG is there)
+        const int i = (k - 1) & ~(SG - 1);
+        const bool scales_out = i >= k - AHEAD && i >= 0 && i + SG < n;
         if (k + AHEAD > n) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         else if (scales_out) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS + SLOADS) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS) : "memory");
         if (k + AHEAD < n) fetch(g0 + k + AHEAD, buf == 0 ? AHEAD : buf - 1);
-        if ((k & 3) == 0 && k + 4 < n) fetch_scales(g0 + k + 4, ((k >> 2) + 1) & 1);
+        if (k % SG == 0 && k + SG < n) fetch_scales(g0 + k + SG, (k / SG + 1) & 1);
         const int8_t* la0 = lds + buf * STAGE + op0;
         const int8_t* la1 = lds + buf * STAGE + op1;
-        const float* sa = lsc + ((k >> 2) & 1) * 4 * S::srows + (k & 3) + sc_h;
-        const float* sb = lsc + ((k >> 2) & 1) * 4 * S::srows + (k & 3) + sc_x;
+        const float* sa = lsc + (k / SG & 1) * SG * S::srows + k % SG + sc_h;
+        const float* sb = lsc + (k / SG & 1) * SG * S::srows + k % SG + sc_x;
         // (X's rows are the matrix instruction's rows and H's its columns: a lane's four values lie side by side in
         // the slab)
         i32x4 fa[S::mi][2];
@@ -313,7 +321,7 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
         for (int i = 0; i < S::mi; ++i) {
             fa[i][0] = *reinterpret_cast<const i32x4*>(la0 + 16 * i * GROUP);
             fa[i][1] = *reinterpret_cast<const i32x4*>(la1 + 16 * i * GROUP);
-            hs[i] = sa[4 * 16 * i];
+            hs[i] = sa[SG * 16 * i];
         }
 #pragma unroll
         for (int j = 0; j < S::nj; ++j) {
@@ -321,7 +329,7 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
             const i32x4 fb1 = *reinterpret_cast<const i32x4*>(la1 + ba + 16 * j * GROUP);
             float xs[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) xs[e] = sb[4 * (16 * j + e)];
+            for (int e = 0; e < 4; ++e) xs[e] = sb[SG * (16 * j + e)];
             i32x4 part[S::mi];
 #pragma unroll
             for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb0, fa[i][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
@@ -333,6 +341,27 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
                 for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(xs[e] * hs[i], (float)part[i][e], acc[i][j][e]);
         }
         buf = buf == AHEAD ? 0 : buf + 1;
+    }
+    if (p.splits == 1) {
+        const float* in = is_h ? p.A_in : p.B_in;
+        float* out = is_h ? p.A : p.B;
+        double* sums = is_h ? p.Ad : p.Bd;
+#pragma unroll
+        for (int i = 0; i < S::mi; ++i) {
+            const int m = m0 + wm + 16 * i + (lane & 15);
+            if (m >= p.r) continue;
+#pragma unroll
+            for (int j = 0; j < S::nj; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int n = n0 + wn + 16 * j + 4 * (lane >> 4) + e;
+                    if (n >= N) continue;
+                    const size_t at = (size_t)m * N + n;
+                    if (sums) sums[at] = (double)acc[i][j][e];
+                    else out[at] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at] : 0.0));
+                }
+        }
+        return;
     }
     float* out = p.slab + (size_t)split * p.r * p.cols + (is_h ? 0 : p.cols_h);
 #pragma unroll
@@ -450,8 +479,9 @@ __global__ __launch_bounds__(256) void keep8_gradient_kernel(int d, int r, const
 using Wide = Tile<4, 2, 4, 4, 3>;       // 256 x 128
 using Middle = Tile<4, 2, 2, 8, 3>;     // 128 x 256
 using Narrow = Tile<4, 2, 1, 8, 3>;     // 64 x 256
-using Slim = Tile<2, 2, 1, 8, 3>;       // 32 x 256
+using Slim = Tile<2, 2, 1, 4, 6>;       // 32 x 128
 
+constexpr int ONE_RUN = 8;
 struct SumPlan { int tile, bm, bn, tiles_m, tiles_h, tiles_x, cols_h, cols, splits, per; };
 SumPlan sum_plan(int d, int r, int n) {
     SumPlan q;
@@ -466,13 +496,17 @@ SumPlan sum_plan(int d, int r, int n) {
     q.cols_h = (r + 3) & ~3;
     q.cols = q.cols_h + ((d + 3) & ~3);
     const long long tiles = (long long)q.tiles_m * (q.tiles_h + q.tiles_x);
-    long long splits = std::max<long long>(1, 256 / tiles);
-    splits = std::min<long long>(splits, groups);
+    // A short contraction in one run, with nothing to add up behind it; otherwise a workgroup per CU and four groups
+    // a run at least (d=1200 r=100 n=8191: 17.3 us, with two groups a run and twice the slabs 20.3).
+    long long splits = groups <= ONE_RUN ? 1 : std::max<long long>(1, 256 / tiles);
+    splits = std::min<long long>(splits, (groups + 3) / 4);
     q.per = (int)((groups + splits - 1) / splits);
     q.splits = (groups + q.per - 1) / q.per;
     return q;
 }
-size_t sums_bytes(const SumPlan& q, int r) { return ((size_t)q.splits * r * q.cols * sizeof(float) + 255) & ~(size_t)255; }
+size_t sums_bytes(const SumPlan& q, int r) {
+    return q.splits == 1 ? 0 : ((size_t)q.splits * r * q.cols * sizeof(float) + 255) & ~(size_t)255;
+}
 
 int check8(onmf_ctx* c, const char* what, int d, int n, const void* codes, const void* scales) {
     if (d <= 0 || n <= 0 || !codes || !scales || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
@@ -483,7 +517,7 @@ int check8(onmf_ctx* c, const char* what, int d, int n, const void* codes, const
 
 template <typename S>
 int launch_sums(onmf_ctx* c, const SumParams& p, hipStream_t s) {
-    constexpr size_t bytes = S::stages * (size_t)S::rows * GROUP + 2 * (size_t)S::srows * 4 * sizeof(float);
+    constexpr size_t bytes = S::stages * (size_t)S::rows * GROUP + 2 * (size_t)S::srows * S::sg * sizeof(float);
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     static LdsLimit lim;
     ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_sums_kernel<S>, bytes));
@@ -492,24 +526,25 @@ int launch_sums(onmf_ctx* c, const SumParams& p, hipStream_t s) {
     return ONMF_OK;
 }
 
-int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* xc, const float* xs, const int8_t* hc,
-             const float* hs, float* slab, hipStream_t s) {
+// The sums of a minibatch into A and B, or as doubles into Ad and Bd.
+int run_sums(onmf_ctx* c, int d, int r, int n, const int8_t* xc, const float* xs, const int8_t* hc, const float* hs,
+             float* slab, double w, double keep, const float* A_in, const float* B_in, float* A, float* B, double* Ad,
+             double* Bd, hipStream_t s) {
+    const SumPlan q = sum_plan(d, r, n);
     SumParams p;
     p.hc = hc; p.xc = xc; p.hs = hs; p.xs = xs; p.slab = slab;
     p.d = d; p.r = r; p.groups = (n + GROUP - 1) / GROUP; p.per_split = q.per; p.splits = q.splits;
     p.tiles_m = q.tiles_m; p.tiles_h = q.tiles_h; p.tiles = q.tiles_m * (q.tiles_h + q.tiles_x);
     p.cols_h = q.cols_h; p.cols = q.cols;
+    p.w = w; p.keep = keep; p.A_in = A_in; p.B_in = B_in; p.A = A; p.B = B; p.Ad = Ad; p.Bd = Bd;
     switch (q.tile) {
-        case 0: return launch_sums<Slim>(c, p, s);
-        case 1: return launch_sums<Narrow>(c, p, s);
-        case 2: return launch_sums<Middle>(c, p, s);
-        default: return launch_sums<Wide>(c, p, s);
+        case 0: ONMF_TRY(launch_sums<Slim>(c, p, s)); break;
+        case 1: ONMF_TRY(launch_sums<Narrow>(c, p, s)); break;
+        case 2: ONMF_TRY(launch_sums<Middle>(c, p, s)); break;
+        default: ONMF_TRY(launch_sums<Wide>(c, p, s)); break;
     }
-}
-
-// (few entries with many slabs: more threads to an entry)
-int run_reduce(onmf_ctx* c, const SumPlan& q, int d, int r, const float* slab, double w, double keep, const float* A_in,
-               const float* B_in, float* A, float* B, double* Ad, double* Bd, hipStream_t s) {
+    if (q.splits == 1) return ONMF_OK;
+    // (few entries with many slabs: more threads to an entry)
     const size_t quads = (size_t)r * q.cols / 4;
     if (quads < 16384)
         hipLaunchKernelGGL(keep8_reduce_kernel<16>, dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, s, d, r, q.cols_h, q.cols,
@@ -607,13 +642,12 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
     ONMF_TRY(check8(c, "keep8_aggregate", r, n, h_codes, h_scales));
     if (!A_out || !B_out) return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: an output is null");
     const size_t need = onmf_keep8_workspace(d, r, n, 0);
-    if (!ws || ws_bytes < need)
+    if ((need && !ws) || ws_bytes < need)
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    const SumPlan q = sum_plan(d, r, n);
-    ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, s));
-    return run_reduce(c, q, d, r, (const float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr, nullptr, s);
+    return run_sums(c, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr,
+                    nullptr, s);
 }
 
 int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const int8_t* x_codes, const float* x_scales,
@@ -630,10 +664,9 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    const SumPlan q = sum_plan(d, r, n);
-    double* Ad = (double*)((char*)ws + sums_bytes(q, r));
-    ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, s));
-    ONMF_TRY(run_reduce(c, q, d, r, (const float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr, Ad, Ad + (size_t)r * r, s));
+    double* Ad = (double*)((char*)ws + sums_bytes(sum_plan(d, r, n), r));
+    ONMF_TRY(run_sums(c, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
+                      Ad, Ad + (size_t)r * r, s));
     hipLaunchKernelGGL(keep8_gradient_kernel, dim3((r + 31) / 32, (d + 31) / 32), dim3(256), 0, s, d, r, W, Ad,
                        Ad + (size_t)r * r, dW);
     HIP_TRY(c, hipGetLastError());

@@ -332,19 +332,21 @@ def test_gradient_is_the_losses_difference(eng, torch):
         assert abs(diff - g[i, k]) <= 1e-5 * np.abs(W).sum(1).max() * n
 
 
-def test_aggregates_in_place(eng, torch):
+@pytest.mark.parametrize("n", [500, 5000])          # one run of groups, and several that are added up
+def test_aggregates_in_place(eng, torch, n):
     from onmf_ontf_ndl_amd.engine import _ptr
     rs = np.random.RandomState(4)
-    d, r, n = 200, 30, 500
+    d, r = 200, 30
     X, H = eng.keep8(eng.dev(rs.rand(d, n))), eng.keep8(eng.dev(rs.rand(r, n)))
     A, B = eng.dev(rs.rand(r, r)), eng.dev(rs.rand(r, d))
     want = eng.keep8_aggregate(X, H, 0.25, A, B)
     nbytes = eng.lib.onmf_keep8_workspace(d, r, n, 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=eng.device)
+    assert (nbytes > 0) == (n > 1024)
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=eng.device)
     rc = eng.lib.onmf_keep8_aggregate(eng.ctx, d, r, n, _ptr(X.codes), _ptr(X.scales), _ptr(H.codes), _ptr(H.scales), 0.25,
                                       _ptr(A), _ptr(B), _ptr(A), _ptr(B), _ptr(ws), nbytes, eng.stream())
     assert rc == 0 and torch.equal(A, want[0]) and torch.equal(B, want[1])
-    for short, where in ((nbytes - 1, ws), (nbytes, None)):
+    for short, where in ((nbytes - 1, ws), (nbytes, None)) if nbytes else ():
         assert eng.lib.onmf_keep8_aggregate(eng.ctx, d, r, n, _ptr(X.codes), _ptr(X.scales), _ptr(H.codes), _ptr(H.scales), 0.25,
                                             _ptr(A), _ptr(B), _ptr(A), _ptr(B), _ptr(where), short, eng.stream()) == -1
     assert eng.lib.onmf_keep8(eng.ctx, d, n, _ptr(A), 0, n - 1, _ptr(X.codes), _ptr(X.scales), eng.stream()) == -1
