@@ -10,6 +10,9 @@
 #include <algorithm>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+// rows of any length: vectors that need no more alignment than their entries (the memory pipe takes them as they lie)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 namespace {
 
@@ -52,7 +55,7 @@ struct GroupAt {
 // 16 lanes per group, eight columns a lane, U groups a lane (their loads are on their way together).  Bound by
 // memory: 5 bytes a float32 entry, 3 a bfloat16 one.
 template <typename T, typename I, int U>
-__global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int groups, const T* __restrict__ X, int ldx, int vec,
+__global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int groups, const T* __restrict__ X, int ldx,
                                                      int8_t* __restrict__ codes, float* __restrict__ scales) {
     const int lane = threadIdx.x & 15;
     const size_t first = ((size_t)blockIdx.x * 16 + (threadIdx.x >> 4)) * U;
@@ -66,14 +69,13 @@ __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int group
         if (first + u >= all) continue;
         const int c = (int)at.g * GROUP + lane * 8;
         const T* src = X + (size_t)at.row * ldx + c;
-        if (vec && c + 7 < n) {
+        if (c + 7 < n) {
             if constexpr (sizeof(T) == 4) {
-                const float4 f = reinterpret_cast<const float4*>(src)[0], h = reinterpret_cast<const float4*>(src)[1];
+                const f32x4_any f = reinterpret_cast<const f32x4_any*>(src)[0], h = reinterpret_cast<const f32x4_any*>(src)[1];
                 v[u][0] = f.x; v[u][1] = f.y; v[u][2] = f.z; v[u][3] = f.w;
                 v[u][4] = h.x; v[u][5] = h.y; v[u][6] = h.z; v[u][7] = h.w;
             } else {
-                const uint4 w = *reinterpret_cast<const uint4*>(src);
-                const uint32_t p[4] = {w.x, w.y, w.z, w.w};
+                const u32x4_any p = *reinterpret_cast<const u32x4_any*>(src);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[u][2 * j] = __uint_as_float(p[j] << 16);
@@ -131,7 +133,7 @@ __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int group
 template <typename I, int U>
 __global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, int groups, const int8_t* __restrict__ codes,
                                                             const float* __restrict__ scales, float* __restrict__ X,
-                                                            int ldx, int vec) {
+                                                            int ldx) {
     const int lane = threadIdx.x & 31;
     const size_t first = ((size_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * U;
     if (first >= all) return;
@@ -148,11 +150,11 @@ __global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, in
     for (int u = 0; u < U; ++u, at.next()) {
         if (first + u >= all) break;
         const int c = (int)at.g * GROUP + lane * 4;
-        const float4 v = make_float4(s[u] * (float)(int8_t)(w[u] & 0xff), s[u] * (float)(int8_t)((w[u] >> 8) & 0xff),
-                                     s[u] * (float)(int8_t)((w[u] >> 16) & 0xff), s[u] * (float)(int8_t)(w[u] >> 24));
+        const f32x4_any v = {s[u] * (float)(int8_t)(w[u] & 0xff), s[u] * (float)(int8_t)((w[u] >> 8) & 0xff),
+                             s[u] * (float)(int8_t)((w[u] >> 16) & 0xff), s[u] * (float)(int8_t)(w[u] >> 24)};
         float* dst = X + (size_t)at.row * ldx + c;
-        if (vec && c + 3 < n) {
-            *reinterpret_cast<float4*>(dst) = v;
+        if (c + 3 < n) {
+            *reinterpret_cast<f32x4_any*>(dst) = v;
         } else {
             if (c + 0 < n) dst[0] = v.x;
             if (c + 1 < n) dst[1] = v.y;
@@ -351,15 +353,24 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
             const int m = m0 + wm + 16 * i + (lane & 15);
             if (m >= p.r) continue;
 #pragma unroll
-            for (int j = 0; j < S::nj; ++j)
+            for (int j = 0; j < S::nj; ++j) {
+                const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
+                const size_t at = (size_t)m * N + n;
+                if (n + 3 < N && !sums) {
+                    f32x4_any v = {0.f, 0.f, 0.f, 0.f};
+                    if (in) v = *reinterpret_cast<const f32x4_any*>(in + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = (float)(p.w * (double)acc[i][j][e] + p.keep * (double)v[e]);
+                    *reinterpret_cast<f32x4_any*>(out + at) = v;
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int n = n0 + wn + 16 * j + 4 * (lane >> 4) + e;
-                    if (n >= N) continue;
-                    const size_t at = (size_t)m * N + n;
-                    if (sums) sums[at] = (double)acc[i][j][e];
-                    else out[at] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at] : 0.0));
+                    if (n + e >= N) continue;
+                    if (sums) sums[at + e] = (double)acc[i][j][e];
+                    else out[at + e] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at + e] : 0.0));
                 }
+            }
         }
         return;
     }
@@ -426,12 +437,13 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // dW[i][k] = sum_j W[i][j] A[j][k] - B[k][i] in double, rounded once: near a stationary dictionary the two terms
 // nearly cancel.  32 x 32 tiles, a 16 x 16 one a wave on the double matrix pipe (16x16x4: row l % 16 and column
 // l % 16 of the operands at j + l / 16, output row 4 e + l / 16); the next 32 steps of j are loaded into registers
-// while these are computed.
+// while these are computed.  Rows of 36 and 48 doubles: an operand read's 64 lanes meet every bank alike.
+// (64 x 64 tiles leave too few waves to wait for memory: d=4096 r=256 20 -> 26 us.)
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(256) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
                                                               const double* __restrict__ A,
                                                               const double* __restrict__ B, float* __restrict__ dW) {
-    __shared__ double tw[32][33], ta[32][34], tb[32][33];
+    __shared__ double tw[32][36], ta[32][48], tb[32][33];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
     const int wi = (wave & 1) * 16, wk = (wave >> 1) * 16;
@@ -559,28 +571,28 @@ int run_sums(onmf_ctx* c, int d, int r, int n, const int8_t* xc, const float* xs
 // Groups a thread handles: several where there are enough of them to fill the chip with.  32-bit group numbers where
 // they do (a division in 64 bits costs as much as everything else).
 template <typename T, typename I>
-void launch_keep_as(size_t all, int n, int groups, const T* X, int ldx, int vec, int8_t* codes, float* scales, hipStream_t s) {
+void launch_keep_as(size_t all, int n, int groups, const T* X, int ldx, int8_t* codes, float* scales, hipStream_t s) {
     if (all >= 65536)
         hipLaunchKernelGGL((keep8_kernel<T, I, 2>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, X, ldx,
-                           vec, codes, scales);
+                           codes, scales);
     else
         hipLaunchKernelGGL((keep8_kernel<T, I, 1>), dim3((unsigned)((all + 15) / 16)), dim3(256), 0, s, all, n, groups, X, ldx,
-                           vec, codes, scales);
+                           codes, scales);
 }
 template <typename T>
-void launch_keep(size_t all, int n, int groups, const T* X, int ldx, int vec, int8_t* codes, float* scales, hipStream_t s) {
-    if (all < 0x7fffffffu) launch_keep_as<T, uint32_t>(all, n, groups, X, ldx, vec, codes, scales, s);
-    else launch_keep_as<T, uint64_t>(all, n, groups, X, ldx, vec, codes, scales, s);
+void launch_keep(size_t all, int n, int groups, const T* X, int ldx, int8_t* codes, float* scales, hipStream_t s) {
+    if (all < 0x7fffffffu) launch_keep_as<T, uint32_t>(all, n, groups, X, ldx, codes, scales, s);
+    else launch_keep_as<T, uint64_t>(all, n, groups, X, ldx, codes, scales, s);
 }
 template <typename I>
-void launch_expand(size_t all, int n, int groups, const int8_t* codes, const float* scales, float* X, int ldx, int vec,
+void launch_expand(size_t all, int n, int groups, const int8_t* codes, const float* scales, float* X, int ldx,
                    hipStream_t s) {
     if (all >= 65536)
         hipLaunchKernelGGL((keep8_expand_kernel<I, 4>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, codes,
-                           scales, X, ldx, vec);
+                           scales, X, ldx);
     else
         hipLaunchKernelGGL((keep8_expand_kernel<I, 1>), dim3((unsigned)((all + 7) / 8)), dim3(256), 0, s, all, n, groups, codes,
-                           scales, X, ldx, vec);
+                           scales, X, ldx);
 }
 
 }  // namespace
@@ -595,12 +607,10 @@ int onmf_keep8(onmf_ctx* c, int d, int n, const void* X, int x_type, int ldx, in
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
-    const size_t es = x_type == ONMF_TYPE_F32 ? 4 : 2;
-    const int vec = ((uintptr_t)X & 15) == 0 && (ldx * es) % 16 == 0;
     const size_t all = (size_t)d * groups;
     if (all > MOST_GROUPS) return onmf_fail(c, ONMF_ERR_ARG, "keep8: %d x %d is more than 2^33 groups", d, n);
-    if (x_type == ONMF_TYPE_F32) launch_keep(all, n, groups, (const float*)X, ldx, vec, codes, scales, s);
-    else launch_keep(all, n, groups, (const uint16_t*)X, ldx, vec, codes, scales, s);
+    if (x_type == ONMF_TYPE_F32) launch_keep(all, n, groups, (const float*)X, ldx, codes, scales, s);
+    else launch_keep(all, n, groups, (const uint16_t*)X, ldx, codes, scales, s);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -615,16 +625,15 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
     const size_t all = (size_t)d * groups;
-    const int vec = ((uintptr_t)X & 15) == 0 && (ldx & 3) == 0;
     if (idx)
         hipLaunchKernelGGL(keep8_gather_kernel, dim3((b + 255) / 256, std::min(d, 4096)), dim3(256), 0, s, d, n, groups, codes,
                            scales, (const long long*)idx, b, X, ldx);
     else if (all > MOST_GROUPS)
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: %d x %d is more than 2^33 groups", d, n);
     else if (all < 0x7fffffffu)
-        launch_expand<uint32_t>(all, n, groups, codes, scales, X, ldx, vec, s);
+        launch_expand<uint32_t>(all, n, groups, codes, scales, X, ldx, s);
     else
-        launch_expand<uint64_t>(all, n, groups, codes, scales, X, ldx, vec, s);
+        launch_expand<uint64_t>(all, n, groups, codes, scales, X, ldx, s);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
