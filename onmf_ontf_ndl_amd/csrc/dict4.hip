@@ -14,6 +14,9 @@
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+// rows of any length: pairs that need no more alignment than their entries (the memory pipe takes them as they lie)
+typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u32_any __attribute__((aligned(2)));
 
 namespace {
 
@@ -552,26 +555,20 @@ struct ManyParams {
     int M, N, K, kp;         // rows of the output, its columns, contraction length and that of A's rows
     int ldx, ldo, group;
     int tiles_m, tiles, k_per_split;
-    int vec;                 // two columns may be loaded at once
-    int vec_out;             // ... and stored
 };
 
-// columns n and n + 1 of row k
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_two(const T* row, int n, int n1, float& a, float& b) {
-    if constexpr (VEC && sizeof(T) == 4) {
-        const float2 v = *reinterpret_cast<const float2*>(row + n);
-        a = v.x; b = v.y;
-    } else if constexpr (VEC) {
-        const uint32_t v = *reinterpret_cast<const uint32_t*>(row + n);
-        a = bf16_lo(v); b = bf16_hi(v);
-    } else {
-        a = load_val(row + n);
-        b = load_val(row + n1);
-    }
+// two columns of a row, as they lie
+__device__ __forceinline__ void load_two(const float* p, float& a, float& b) {
+    const f32x2_any v = *reinterpret_cast<const f32x2_any*>(p);
+    a = v[0]; b = v[1];
+}
+__device__ __forceinline__ void load_two(const uint16_t* p, float& a, float& b) {
+    const uint32_t v = *reinterpret_cast<const u32_any*>(p);
+    a = bf16_lo(v); b = bf16_hi(v);
 }
 
-template <bool PROD, typename T, int MT, bool VEC>
+// OFF: 32 bits where 32 rows of X lie within them
+template <bool PROD, typename T, int MT, typename OFF>
 __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     constexpr int PX = sizeof(T) == 4 ? 3 : 1;        // pieces of the float operand
     constexpr int PW = PROD ? 2 : 1;                   // pieces of the weights
@@ -584,11 +581,12 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (at >= p.tiles) return;
     const int m0 = (at % p.tiles_m) * 16 * MT, n0 = (at / p.tiles_m) * BN + wave * 32;
-    const int kbeg = blockIdx.y * p.k_per_split, kend = min(p.kp, kbeg + p.k_per_split);
-    const int steps = (kend - kbeg) / BK;
-    // a column behind the last one reads the last one's (its results are not stored), a row behind the last one the
-    // last one (the weights are zero there)
-    const int na = min(n0 + 2 * (lane & 15), VEC ? max(p.N - 2, 0) : p.N - 1), nb = min(n0 + 2 * (lane & 15) + 1, p.N - 1);
+    const int kbeg = blockIdx.y * p.k_per_split, kend = min(p.K, kbeg + p.k_per_split);
+    const int steps = (kend - kbeg + BK - 1) / BK;
+    // Columns behind the last one read the last two (their results are not stored; where the last one is the first of
+    // its pair it is taken from the second place), rows behind the last one the last one (the weights are zero there).
+    const int na = min(n0 + 2 * (lane & 15), p.N - 2);
+    const bool second = n0 + 2 * (lane & 15) > na;
     const int kl = 8 * (lane >> 4);
 
     // 16 rows of weights a load: a base for the wave and 32 bits a lane
@@ -617,10 +615,11 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
                     (__attribute__((address_space(3))) void*)(lscale + buf * SROWS + wave * 64), 4, 0, 0);
     };
     float xr[8][2];
-    auto fetch_x = [&](int k) {
+    auto fetch_x = [&](int k) {                       // (k < K: the rows are counted from k's)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            load_two<T, VEC>((const T*)p.X + (size_t)min(k + kl + j, p.K - 1) * p.ldx, na, nb, xr[j][0], xr[j][1]);
+            load_two((const T*)((const char*)p.X + (size_t)k * p.ldx * sizeof(T) +
+                                ((OFF)min(kl + j, p.K - 1 - k) * (OFF)p.ldx + (OFF)na) * (OFF)sizeof(T)), xr[j][0], xr[j][1]);
     };
     uint4 fb[2][PX];
     auto split_x = [&]() {
@@ -628,7 +627,7 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
         for (int c = 0; c < 2; ++c) {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = xr[j][c];
+            for (int j = 0; j < 8; ++j) v[j] = c == 0 && second ? xr[j][1] : xr[j][c];
 #pragma unroll
             for (int q = 0; q < PX; ++q) {
                 uint32_t u[4];
@@ -646,10 +645,10 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     f32x4 acc[MT][2];
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int op = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
     fetch_a(kbeg, 0);
     fetch_x(kbeg);
     split_x();
-    const int op = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
     for (int s = 0; s < steps; ++s) {
         const int buf = s & 1, k = kbeg + s * BK;
         __syncthreads();                               // (this step's weights have come, the last step's are done with)
@@ -707,11 +706,8 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
             const int m = m0 + 16 * i + 4 * (lane >> 4) + e;
             if (m >= p.M) continue;
             float* dst = out + (size_t)m * ldo + n;
-            if (p.vec_out && n + 1 < p.N) *reinterpret_cast<float2*>(dst) = make_float2(acc[i][0][e], acc[i][1][e]);
-            else {
-                dst[0] = acc[i][0][e];
-                if (n + 1 < p.N) dst[1] = acc[i][1][e];
-            }
+            if (n + 1 < p.N) *reinterpret_cast<f32x2_any*>(dst) = f32x2_any{acc[i][0][e], acc[i][1][e]};
+            else dst[0] = acc[i][0][e];
         }
 }
 
@@ -749,7 +745,7 @@ ManyPlan many_plan(bool prod, int d, int r, int b, int group) {
     ManyPlan q;
     const int M = prod ? d : r;
     const int kp = prod ? (r + BK - 1) / BK * BK : (d + group - 1) / group * group;
-    const int steps = kp / BK;
+    const int steps = ((prod ? r : d) + BK - 1) / BK;
     q.tiles_n = (b + BN - 1) / BN;
     long long best = -1;
     for (int mt = prod ? 8 : 16; mt >= 2; mt /= 2) {       // (the product's weights are two pieces)
@@ -844,8 +840,6 @@ int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, con
     p.M = PROD ? d : r; p.N = b; p.K = PROD ? r : d;
     p.kp = PROD ? (r + BK - 1) / BK * BK : words * 8;
     p.tiles_m = q.tiles_m; p.tiles = q.tiles_m * q.tiles_n; p.k_per_split = q.per * BK;
-    p.vec = ((uintptr_t)X & (2 * sizeof(T) - 1)) == 0 && (ldx & 1) == 0 && b % 2 == 0;
-    p.vec_out = p.slab ? b % 2 == 0 : ((uintptr_t)out & 7) == 0 && ldo % 2 == 0;
     if constexpr (PROD)
         hipLaunchKernelGGL(dict4_lay_product_kernel, dim3((p.kp + 63) / 64, (words + 15) / 16), dim3(256), 0, s, d, r, words, group,
                            groups, p.kp, codes, scales, (uint16_t*)ws);
@@ -854,11 +848,12 @@ int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, con
                            dim3(256), 0, s, d, r, words, group, groups, codes, scales, (uint4*)ws, (float*)(ws + q.a_bytes));
     HIP_TRY(c, hipGetLastError());
     const dim3 grid((p.tiles + 7) / 8 * 8, q.splits);
+    const bool near = ((size_t)BK * ldx + b) * sizeof(T) < ((size_t)1 << 32);
 #define MANY_CASE(MT)                                                                                                    \
     if (q.mt == MT) {                                                                                                    \
         const size_t bytes = 2 * ((PROD ? 2 : 1) * 16 * MT * 64 + (PROD ? 0 : (16 * MT + 63) / 64 * 64 * sizeof(float)));  \
-        if (p.vec) hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, true>), grid, dim3(256), bytes, s, p);             \
-        else hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, false>), grid, dim3(256), bytes, s, p);                  \
+        if (near) hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, uint32_t>), grid, dim3(256), bytes, s, p);          \
+        else hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, uint64_t>), grid, dim3(256), bytes, s, p);               \
     }
     if constexpr (!PROD) { MANY_CASE(16) }
     MANY_CASE(8) MANY_CASE(4) MANY_CASE(2)

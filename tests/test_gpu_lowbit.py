@@ -141,6 +141,28 @@ def test_products_take_views(eng, torch, b):
             assert np.array_equal(host(eng.dict4_product(P, H)), W @ host(H))
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_rows_that_lie_far_apart(eng, torch, dtype):
+    """Offsets that pass 32 bits, in bytes and in elements: 40 rows of 2^26 + 1 values, of which the first few count."""
+    rs = np.random.RandomState(4)
+    d, ld = 40, 2 ** 26 + 1
+    held = torch.empty(d * ld, dtype=getattr(torch, dtype), device=eng.device)
+    wide = held.view(d, ld)
+    P, parts = whole_dictionary(eng, rs, d, 37, 32)
+    W = lo.values4(*parts, d)
+    Q, qarts = whole_dictionary(eng, rs, 37, d, 32)
+    V = lo.values4(*qarts, 37)
+    for b in (1, 2, 5, 20, 41):
+        X, Xh = as_type(torch, eng, rs.randint(-4, 5, size=(d, b)), dtype)
+        wide[:, 7:7 + b] = X
+        view = wide[:, 7:7 + b]
+        assert np.array_equal(host(eng.dict4_correlate(P, view)), W.T @ Xh)
+        assert np.array_equal(host(eng.dict4_product(Q, view)), V @ Xh)
+        K = eng.keep8(view)
+        q, s = lo.keep8(Xh)
+        assert np.array_equal(K.codes.cpu().numpy(), q) and np.array_equal(host(K.scales), s)
+
+
 @pytest.mark.parametrize("b", [1, 2, 4, 7, 8, 9, 100])
 def test_a_column_that_is_not_finite_touches_no_other(eng, torch, b):
     rs = np.random.RandomState(b)
