@@ -390,8 +390,10 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  *                       counts from the end as in NumPy, one out of range reads NaN) - X[:, idx], src/onmf.py:214
  * onmf_keep8_aggregate  onmf_aggregate's A_out and B_out (src/onmf.py:155-156) from a kept X (d x n) and H (r x n);
  *                       in/out pointers may alias, A_in / B_in NULL means zeros
- * onmf_keep8_gradient   dW (d x r) = W (H H^T) - X H^T, the gradient of 1/2 |X - W H|^2 to W; d, r <= 2^18
- * Products inside a group add up exactly in int32, groups in float32, runs of groups and what follows in double.
+ * onmf_keep8_gradient   dW (d x r) = W (H H^T) - X H^T, the gradient of 1/2 |X - W H|^2 to W; d, r <= 2^18;
+ *                       dW may not overlap W.  Up to 128 columns are taken as (W H - X) H^T where that is less work
+ * Products inside a group add up exactly in int32, groups in float32, runs of groups and what follows in double
+ * (the residual's products in double throughout).
  * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, in use until the call's work on
  * `stream` is done.  n <= 2^28.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
  */

@@ -486,6 +486,106 @@ __global__ __launch_bounds__(256) void keep8_gradient_kernel(int d, int r, const
     }
 }
 
+// The same gradient by way of the residual, dW = (W H - X) H^T, for up to 128 columns: with n < r / 2 of them it is
+// less work than W (H H^T), and one launch.  A workgroup owns 16 rows.  Its waves share the atoms of W H (double matrix
+// pipe: row l % 16 of W and 16 columns of H at k = 16 s + 4 (l / 16) + j in the j-th instruction, so that a lane
+// loads four neighbours of W and words of four codes; the scale of an atom goes with W, one exact double product),
+// add up in LDS and take X off; then they share the atoms of the result, with the residual's operands in registers and the
+// scale of an atom on its sum.  TILES sixteens of columns (1, 4 or 8), NW waves.
+template <int TILES, int NW>
+__global__ __launch_bounds__(64 * NW) void keep8_residual_kernel(int d, int r, const float* __restrict__ W,
+                                                                  const int8_t* __restrict__ xc, const float* __restrict__ xs,
+                                                                  const int8_t* __restrict__ hc, const float* __restrict__ hs,
+                                                                  float* __restrict__ dW) {
+    constexpr int N = 16 * TILES, WORDS = (TILES + 3) / 4, LINE = N + 2;
+    extern __shared__ __align__(16) double sums[];        // [NW][16][N], then the residual [16][LINE]
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, c = lane & 15, quad = lane >> 4;
+    const int i0 = blockIdx.x * 16;
+    const float* wrow = W + (size_t)min(i0 + c, d - 1) * r;
+    struct Step { float w[4], s[4]; uint32_t h[4][WORDS]; };
+    auto fetch = [&](int k0, Step& v) {                   // (atoms behind the last one: the last one's, with weight 0)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int k = min(k0 + 4 * quad + j, r - 1);
+            v.w[j] = wrow[k];
+            v.s[j] = hs[k];
+            const int8_t* code = hc + (size_t)k * GROUP;
+#pragma unroll
+            for (int u = 0; u < WORDS; ++u)
+                v.h[j][u] = TILES == 1 ? (uint32_t)(int)code[c] : *reinterpret_cast<const uint32_t*>(code + 64 * u + 4 * c);
+        }
+    };
+    f64x4 acc[TILES];
+#pragma unroll
+    for (int q = 0; q < TILES; ++q) acc[q] = f64x4{0.0, 0.0, 0.0, 0.0};
+    Step now, next;
+    if (wave * 16 < r) fetch(wave * 16, now);
+    for (int k0 = wave * 16; k0 < r; k0 += 16 * NW) {
+        if (k0 + 16 * NW < r) fetch(k0 + 16 * NW, next);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const double a = k0 + 4 * quad + j < r ? (double)now.w[j] * (double)now.s[j] : 0.0;
+#pragma unroll
+            for (int q = 0; q < TILES; ++q) {
+                const int code = TILES == 1 ? (int)now.h[j][0] : (int)(int8_t)(now.h[j][q / 4] >> (8 * (q % 4)));
+                acc[q] = __builtin_amdgcn_mfma_f64_16x16x4f64(a, (double)code, acc[q], 0, 0, 0);
+            }
+        }
+        if (k0 + 16 * NW < r) now = next;
+    }
+#pragma unroll
+    for (int q = 0; q < TILES; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            sums[(wave * 16 + 4 * e + quad) * N + (TILES == 1 ? c : 64 * (q / 4) + 4 * c + q % 4)] = acc[q][e];
+    __syncthreads();
+    constexpr int EACH = (16 * N + 64 * NW - 1) / (64 * NW);
+    double rest[EACH];
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) {
+        const int e = t + q * 64 * NW, row = min(i0 + e / N, d - 1);
+        if (e >= 16 * N) continue;
+        double v = sums[e];
+#pragma unroll
+        for (int z = 1; z < NW; ++z) v += sums[z * 16 * N + e];
+        rest[q] = v - (double)xs[row] * (double)xc[(size_t)row * GROUP + e % N];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < EACH; ++q) {
+        const int e = t + q * 64 * NW;
+        if (e < 16 * N) sums[e / N * LINE + e % N] = rest[q];
+    }
+    __syncthreads();
+    // instruction 16 u + j (one tile: j) contracts over the columns 64 u + 16 (l / 16) + j (4 (l / 16) + j)
+    constexpr int STEPS = N / 4, RUN = TILES == 1 ? 4 : 16;
+    double res[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) res[s] = sums[c * LINE + s / RUN * 64 + quad * RUN + s % RUN];
+    for (int k0 = wave * 16; k0 < r; k0 += 16 * NW) {
+        const int k = min(k0 + c, r - 1);
+        const int8_t* code = hc + (size_t)k * GROUP + quad * RUN;
+        const double scale = (double)hs[k];
+        uint32_t h[STEPS / 4];
+        if constexpr (TILES == 1) h[0] = *reinterpret_cast<const uint32_t*>(code);
+        else
+#pragma unroll
+            for (int u = 0; u < WORDS; ++u) {
+                const uint4 v = *reinterpret_cast<const uint4*>(code + 64 * u);
+                h[4 * u] = v.x; h[4 * u + 1] = v.y; h[4 * u + 2] = v.z; h[4 * u + 3] = v.w;
+            }
+        f64x4 sum = f64x4{0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+            sum = __builtin_amdgcn_mfma_f64_16x16x4f64(res[s], (double)(int)(int8_t)(h[s / 4] >> (8 * (s % 4))), sum, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = i0 + 4 * e + quad;
+            if (i < d && k0 + c < r) dW[(size_t)i * r + k0 + c] = (float)(scale * sum[e]);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------- launches
 // The tile follows r, so that X is read once: its columns are the wider the fewer rows there are.
 using Wide = Tile<4, 2, 4, 4, 3>;       // 256 x 128
@@ -568,6 +668,25 @@ int run_sums(onmf_ctx* c, int d, int r, int n, const int8_t* xc, const float* xs
     return ONMF_OK;
 }
 
+// The residual costs d r and the columns that its tiles hold, W (H H^T) costs d r^2 and a launch or two more.  Measured
+// (us, residual and sums): d=441 r=25 n=128 6.0 and 8.0; d=2372 r=581 n=2 9.6 and 73; d=8192 r=64 n=128 11.8 and 18;
+// d=65536 r=64 n=128 83 and 49, n=16 24 and 49.
+bool by_residual(int d, int r, int n) {
+    return n <= GROUP && (d <= 8192 || r >= (n <= 16 ? 16 : n <= 64 ? 64 : GROUP));
+}
+
+template <int TILES, int NW>
+int launch_residual(onmf_ctx* c, int d, int r, const float* W, const int8_t* xc, const float* xs, const int8_t* hc, const float* hs,
+                    float* dW, hipStream_t s) {
+    constexpr size_t bytes = (size_t)NW * 16 * 16 * TILES * sizeof(double);
+    static_assert(bytes <= 160 * 1024 && NW >= 2, "the residual, with its lines' padding, takes the sums' place");
+    static LdsLimit lim;
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_residual_kernel<TILES, NW>, bytes));
+    hipLaunchKernelGGL((keep8_residual_kernel<TILES, NW>), dim3((d + 15) / 16), dim3(64 * NW), bytes, s, d, r, W, xc, xs, hc, hs, dW);
+    HIP_TRY(c, hipGetLastError());
+    return ONMF_OK;
+}
+
 // Groups a thread handles: several where there are enough of them to fill the chip with.  32-bit group numbers where
 // they do (a division in 64 bits costs as much as everything else).
 template <typename T, typename I>
@@ -640,6 +759,7 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
 
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
     if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;
+    if (gradient && by_residual(d, r, n)) return 0;
     return sums_bytes(sum_plan(d, r, n), r) + (gradient ? sizeof(double) * (size_t)r * ((size_t)r + d) : 0);
 }
 
@@ -669,10 +789,15 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
     if (d > (1 << 18) || r > (1 << 18))
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: d=%d or r=%d is more than 2^18", d, r);
     const size_t need = onmf_keep8_workspace(d, r, n, 1);
-    if (!ws || ws_bytes < need)
+    if ((need && !ws) || ws_bytes < need)
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
+    if (by_residual(d, r, n)) {
+        if (n <= 16) return launch_residual<1, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
+        if (n <= 64) return launch_residual<4, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
+        return launch_residual<8, 8>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
+    }
     double* Ad = (double*)((char*)ws + sums_bytes(sum_plan(d, r, n), r));
     ONMF_TRY(run_sums(c, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
                       Ad, Ad + (size_t)r * r, s));

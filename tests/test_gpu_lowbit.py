@@ -291,7 +291,8 @@ def whole_columns(eng, rs, d, n, most=15):
 
 
 SUMS = [(1, 1, 1), (3, 2, 128), (441, 25, 1000), (100, 16, 127), (130, 129, 700), (1200, 100, 1500), (257, 300, 129),
-        (64, 1, 5000), (1, 64, 5000), (1024, 256, 2048), (40, 600, 257)]
+        (64, 1, 5000), (1, 64, 5000), (1024, 256, 2048), (40, 600, 257),
+        (300, 40, 9), (33, 333, 16), (200, 531, 17), (17, 15, 64), (1000, 70, 128), (8300, 20, 100), (8300, 129, 65), (1, 1000, 2)]
 
 
 @pytest.mark.parametrize("d,r,n", SUMS)
@@ -379,7 +380,8 @@ def test_aggregates_in_place(eng, torch, n):
 def every_operator(eng, P, X, H, KX, KH, W, A, B):
     kept = eng.keep8(X)
     return [eng.dict4_correlate(P, X), eng.dict4_correlate(P, X[:, :3]), eng.dict4_product(P, H), eng.dict4_product(P, H[:, :1]),
-            kept.codes, kept.scales, eng.keep8_expand(KX), *eng.keep8_aggregate(KX, KH, 0.5, A, B), eng.keep8_gradient(W, KX, KH)]
+            kept.codes, kept.scales, eng.keep8_expand(KX), *eng.keep8_aggregate(KX, KH, 0.5, A, B), eng.keep8_gradient(W, KX, KH),
+            eng.dict4_product(P, H[:, :9]), eng.keep8_gradient(W, eng.keep8(X[:, :100]), eng.keep8(H[:, :100]))]
 
 
 def state(eng, seed):
