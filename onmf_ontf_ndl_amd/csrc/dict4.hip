@@ -10,6 +10,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <cmath>
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -737,31 +738,40 @@ FewProduct product_few_plan(int d, int r, int b) {
     q.splits = (r + q.per - 1) / q.per;
     return q;
 }
-// Rows of a workgroup's tile (in sixteens) and pieces of the contraction for a product with many columns.  A step
-// of a workgroup costs about 6 matrix instructions a row tile and, whatever its rows, what splitting its columns
-// does; two workgroups are resident per CU.
+// Rows of a workgroup's tile (in sixteens) and pieces of the contraction for a product with many columns: the pair with
+// the least time by a model of what a step of 32 was measured to take with w workgroups a CU - 0.6 us until its loads
+// have come, for every set of workgroups that are resident together, and for every sixteen rows (and one for the
+// columns' split) 0.035 to 0.09 us of matrix and vector instructions - and of the pieces' way through memory at
+// 4 TB/s.  (W^T X, d=6492 r=9202 b=73 float32: tiles of 32, 64, 128, 256 rows in one piece 237, 194, 236, 382 us, in
+// pieces for two workgroups a CU 142, 98, 91, 119.)
 struct ManyPlan { int mt, tiles_m, tiles_n, splits, per; size_t a_bytes, s_bytes, slab_bytes; };
-ManyPlan many_plan(bool prod, int d, int r, int b, int group) {
+ManyPlan many_plan(bool prod, int d, int r, int b, int group, bool wide) {
     ManyPlan q;
     const int M = prod ? d : r;
     const int kp = prod ? (r + BK - 1) / BK * BK : (d + group - 1) / group * group;
     const int steps = ((prod ? r : d) + BK - 1) / BK;
     q.tiles_n = (b + BN - 1) / BN;
-    long long best = -1;
+    double best = -1;
     for (int mt = prod ? 8 : 16; mt >= 2; mt /= 2) {       // (the product's weights are two pieces)
-        const long long tiles = (long long)((M + 16 * mt - 1) / (16 * mt)) * q.tiles_n;
-        const long long cost = ((tiles + 511) / 512) * (100 * mt + 400);
-        if (best < 0 || cost < best) {
+        const int tiles_m = (M + 16 * mt - 1) / (16 * mt), resident = mt == 16 ? 2 : mt == 8 ? 3 : 4;
+        const double tiles = (double)tiles_m * q.tiles_n;
+        const double row = prod ? (wide ? 0.09 : 0.05) : (wide ? 0.07 : 0.035);
+        for (int target = 0; target <= 1024; target += 256) {
+            const int want = (int)std::max(1.0, std::min(target / tiles, steps / 2.0));
+            const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+            const double w = std::ceil(tiles * splits / 256);
+            // (256 rows alone on the chip: 0.01 more; with other sets behind it the columns that it saves count as much)
+            const double each = row + (mt == 16 && w <= 2 ? 0.01 : 0.0);
+            double cost = per * (0.6 * std::ceil(w / resident) + each * w * (mt + 1));
+            if (splits > 1) cost += 3.0 + 2e-6 * splits * M * b;
+            if (best >= 0 && cost >= best) continue;
             best = cost;
             q.mt = mt;
+            q.tiles_m = tiles_m;
+            q.per = per;
+            q.splits = splits;
         }
     }
-    q.tiles_m = (M + 16 * q.mt - 1) / (16 * q.mt);
-    const long long tiles = (long long)q.tiles_m * q.tiles_n;
-    // (few tiles: the contraction is cut, into pieces of at least four steps, never inside a group's 32 features)
-    long long splits = tiles >= 256 ? 1 : std::max<long long>(1, std::min<long long>(512 / tiles, steps / 4));
-    q.per = (int)((steps + splits - 1) / splits);
-    q.splits = (steps + q.per - 1) / q.per;
     q.a_bytes = ((size_t)(prod ? 2 : 1) * M * kp * 2 + 255) & ~(size_t)255;
     q.s_bytes = prod ? 0 : ((size_t)(kp / group) * r * sizeof(float) + 255) & ~(size_t)255;
     q.slab_bytes = q.splits > 1 ? (size_t)q.splits * M * b * sizeof(float) : 0;
@@ -830,7 +840,7 @@ int product_tile(onmf_ctx* c, const TilePlan& q, int d, int r, int b, int group,
 template <bool PROD, typename T>
 int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
          float* out, int ldo, char* ws, hipStream_t s) {
-    const ManyPlan q = many_plan(PROD, d, r, b, group);
+    const ManyPlan q = many_plan(PROD, d, r, b, group, sizeof(T) == 4);
     const int groups = (d + group - 1) / group, words = groups * (group / 8);
     ManyParams p;
     p.A = (const uint16_t*)ws;
@@ -916,8 +926,8 @@ size_t onmf_dict4_workspace(int which, int d, int r, int b, int group) {
         return splits > 1 ? (size_t)splits * d * b * sizeof(float) : 0;
     }
     if (which != ONMF_DICT4_PRODUCT && b <= FEW) return 0;
-    const ManyPlan q = many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group);
-    return q.a_bytes + q.s_bytes + q.slab_bytes;
+    const ManyPlan q = many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group, false);      // (enough for either type)
+    return q.a_bytes + q.s_bytes + std::max(q.slab_bytes, many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group, true).slab_bytes);
 }
 
 int onmf_dict4_pack(onmf_ctx* c, int d, int r, int group, const float* W, void* codes, int32_t* scales, void* stream) {

@@ -201,9 +201,11 @@ def test_workspaces_are_bounded():
         for d in (1, 31, 441, 4096, 8192):
             for r in (1, 25, 256, 32768):
                 for b in (1, 3, 8, 9, 64, 1000, 65536):
-                    out = 4 * b * (r if which == 0 else d)
+                    # the weights in bfloat16 (two pieces) with their scales, and 1024 pieces of a result's tile
+                    # of 256 x 128 - or, a column or a few of them, of 512 features
                     n = lib.onmf_dict4_workspace(which, d, r, b, 64)
-                    assert n % 4 == 0 and n <= max(768 * 128 * 128 * 4, 600 * out)
+                    laid = (4 * r + r // 8 + 128) * (d + 128) if b > 8 else 0
+                    assert n % 4 == 0 and n <= laid + 1024 * 256 * 128 * 4
         assert lib.onmf_dict4_workspace(which, 0, 4, 4, 64) == 0
         assert lib.onmf_dict4_workspace(which, 4, 4, 4, 48) == 0
     for d, r, n in ((441, 25, 128), (8192, 1024, 1), (60000, 300, 100)):     # by way of the residual: none
