@@ -17,6 +17,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 // rows of any length: pairs that need no more alignment than their entries (the memory pipe takes them as they lie)
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32_any __attribute__((aligned(2)));
 
 namespace {
@@ -478,6 +479,236 @@ __global__ __launch_bounds__(256) void dict4_reduce_kernel(size_t mn, int N, int
     }
 }
 
+// C = W^T X for a few to 64 columns on the matrix pipe (16x16x32 bfloat16), straight from the nibbles.  The result is
+// computed with X as the rows' operand and W as the columns': a lane's operand is one word (eight features of the atom
+// l % 16, at word l / 16 of a step's four), its part of the sum belongs to that same atom, and the group's scale, which
+// the lane has, is multiplied to it; the whole numbers q + z themselves are bfloat16 values.  A workgroup keeps
+// `per` features of X in LDS, already cut into bfloat16 pieces in the operand's order, and its waves take 32 atoms at a
+// time past it; ranges of features are added up in slabs.  A lane loads 16 bytes, four words of 128 features, two
+// blocks ahead; the 4 x 4 words of the lanes l % 16 + 16 j change places in four instructions.
+template <int NT, typename T>
+__global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r, int b, int group, int groups,
+                                                                      const uint32_t* __restrict__ codes,
+                                                                      const uint32_t* __restrict__ scales,
+                                                                      const T* __restrict__ X, int ldx, float* __restrict__ C,
+                                                                      int per, float* __restrict__ slab) {
+    constexpr int PX = sizeof(T) == 4 ? 3 : 1, AT = 2;
+    extern __shared__ __align__(16) uint4 xop[];              // [step of 32][NT][PX][64 lanes]
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, kq = lane >> 4;
+    const int words = groups * (group / 8);
+    const int f0 = blockIdx.y * per, f1 = min(d, f0 + per), blocks = (f1 - f0 + 127) / 128;
+#pragma unroll 2
+    for (int e = t; e < blocks * 4 * NT * 64; e += 512) {
+        const int at = e >> 6, n = at % NT * 16 + m, k0 = f0 + at / NT * 32 + 8 * kq;
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float x = load_val(X + (size_t)min(k0 + j, d - 1) * ldx + min(n, b - 1));
+            v[j] = k0 + j < d ? x : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < PX; ++q) {
+            uint32_t u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                v[2 * j] -= bf16_lo(u[j]);
+                v[2 * j + 1] -= bf16_hi(u[j]);
+            }
+            xop[(at * PX + q) * 64 + lane] = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+    __syncthreads();
+    const int tiles = (r + 16 * AT - 1) / (16 * AT), stride = gridDim.x * 8;
+    struct Raw { uint4 cw[AT]; uint32_t sc[AT][4]; };
+    // (atoms behind the last one are the last one, words behind a row's last one its last ones, where X is zero)
+    auto fetch = [&](int tile, int blk, Raw& x) {
+        const int f = f0 + blk * 128;
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
+            const int k = min(tile * 16 * AT + 16 * a + m, r - 1);
+            x.cw[a] = *reinterpret_cast<const uint4*>(codes + (size_t)k * words + min(f / 8 + 4 * kq, words - 4));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.sc[a][j] = scales[(size_t)k * groups + min((f + 32 * j) / group, groups - 1)];
+        }
+    };
+    f32x4 acc[AT][NT];
+    auto compute = [&](int tile, int blk, Raw& x) {
+        if (blk == 0)
+#pragma unroll
+            for (int a = 0; a < AT; ++a)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[a][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint32_t w[AT][4];
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
+            // word 4 row + j in place j of a row of lanes -> word 4 j + row
+            const auto p0 = __builtin_amdgcn_permlane32_swap(x.cw[a].x, x.cw[a].z, false, false);
+            const auto p1 = __builtin_amdgcn_permlane32_swap(x.cw[a].y, x.cw[a].w, false, false);
+            const auto q0 = __builtin_amdgcn_permlane16_swap(p0[0], p1[0], false, false);
+            const auto q1 = __builtin_amdgcn_permlane16_swap(p0[1], p1[1], false, false);
+            w[a][0] = q0[0]; w[a][1] = q0[1]; w[a][2] = q1[0]; w[a][3] = q1[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bf16x8 xo[NT][PX];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int q = 0; q < PX; ++q)
+                    xo[n][q] = __builtin_bit_cast(bf16x8, xop[(((blk * 4 + j) * NT + n) * PX + q) * 64 + lane]);
+#pragma unroll
+            for (int a = 0; a < AT; ++a) {
+                const float s = word_scale(x.sc[a][j]), z = word_offset(x.sc[a][j]);
+                float q[8];
+                word_entries(w[a][j], q);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] += z;
+                const bf16x8 wo = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]),
+                                                                        pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7])));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
+                    // smallest products first
+#pragma unroll
+                    for (int p = PX - 1; p >= 0; --p) part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xo[n][p], wo, part, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[a][n][e] = fmaf(s, part[e], acc[a][n][e]);
+                }
+            }
+        }
+        if (blk != blocks - 1) return;
+        float* out = slab ? slab + (size_t)blockIdx.y * r * b : C;
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
+            const int k = tile * 16 * AT + 16 * a + m;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int col = 16 * n + 4 * kq;
+                float* dst = out + (size_t)k * b + col;
+                if (k < r && col + 4 <= b) *reinterpret_cast<f32x4_any*>(dst) = acc[a][n];
+                else if (k < r)
+#pragma unroll
+                    for (int e = 0; e < 3; ++e)
+                        if (col + e < b) dst[e] = acc[a][n][e];
+            }
+        }
+    };
+    int tile = blockIdx.x * 8 + wave, blk = 0;                // ... of the loads that are sent for next
+    auto ahead = [&]() {
+        if (++blk == blocks) {
+            blk = 0;
+            tile += stride;
+        }
+    };
+    Raw even, odd;
+    int ct = tile, cb = 0;                                    // ... and of those that are computed
+    auto after = [&]() {
+        if (++cb == blocks) {
+            cb = 0;
+            ct += stride;
+        }
+    };
+    if (tile < tiles) fetch(tile, blk, even);
+    ahead();
+    if (tile < tiles) fetch(tile, blk, odd);
+    ahead();
+    while (ct < tiles) {
+        compute(ct, cb, even);
+        after();
+        if (tile < tiles) fetch(tile, blk, even);
+        ahead();
+        if (ct >= tiles) break;
+        compute(ct, cb, odd);
+        after();
+        if (tile < tiles) fetch(tile, blk, odd);
+        ahead();
+    }
+}
+
+// The same for results so small that a launch counts as much as the work: a workgroup owns 16 atoms, its NW waves share the
+// steps of 32 features, DEPTH of them on their way, each cutting its part of X into pieces itself, and add up in LDS.
+template <int NT, int NW, typename T>
+__global__ __launch_bounds__(64 * NW) void dict4_correlate_wave_kernel(int d, int r, int b, int group, int groups,
+                                                                       const uint32_t* __restrict__ codes,
+                                                                       const uint32_t* __restrict__ scales,
+                                                                       const T* __restrict__ X, int ldx, float* __restrict__ C) {
+    constexpr int PX = sizeof(T) == 4 ? 3 : 1, DEPTH = NT == 1 ? 4 : NT == 2 ? 3 : 2;
+    __shared__ __align__(16) f32x4 part[NW][NT][64];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, kq = lane >> 4;
+    const int words = groups * (group / 8), steps = (d + 31) / 32;
+    const int k = min((int)blockIdx.x * 16 + m, r - 1);                       // (atoms behind the last one are not stored)
+    const uint32_t* code = codes + (size_t)k * words + kq;
+    const uint32_t* scale = scales + (size_t)k * groups;
+    struct Raw { uint32_t w, sc; float x[NT][8]; };
+    auto fetch = [&](int s, Raw& v) {
+        v.w = code[4 * s];
+        v.sc = scale[32 * s / group];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v.x[n][j] = load_val(X + (size_t)min(32 * s + 8 * kq + j, d - 1) * ldx + min(16 * n + m, b - 1));
+    };
+    f32x4 acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int s, Raw& v) {
+        const float sc = word_scale(v.sc), z = word_offset(v.sc);
+        float q[8];
+        word_entries(v.w, q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] += z;
+        const bf16x8 wo = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]),
+                                                                pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7])));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float x[8];
+            uint4 xo[PX];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 32 * s + 8 * kq + j < d ? v.x[n][j] : 0.f;
+#pragma unroll
+            for (int p = 0; p < PX; ++p) {
+                uint32_t u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    u[j] = pack_bf16(x[2 * j], x[2 * j + 1]);
+                    x[2 * j] -= bf16_lo(u[j]);
+                    x[2 * j + 1] -= bf16_hi(u[j]);
+                }
+                xo[p] = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+            f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = PX - 1; p >= 0; --p)
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xo[p]), wo, sum, 0, 0, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[n][e] = fmaf(sc, sum[e], acc[n][e]);
+        }
+    };
+    Raw raw[DEPTH];
+#pragma unroll
+    for (int j = 0; j < DEPTH; ++j)
+        if (wave + j * NW < steps) fetch(wave + j * NW, raw[j]);
+    for (int s = wave; s < steps; s += DEPTH * NW)
+#pragma unroll
+        for (int j = 0; j < DEPTH; ++j)
+            if (s + j * NW < steps) {
+                compute(s + j * NW, raw[j]);
+                if (s + (j + DEPTH) * NW < steps) fetch(s + (j + DEPTH) * NW, raw[j]);
+            }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) part[wave][n][lane] = acc[n];
+    __syncthreads();
+    for (int e = t; e < NT * 256; e += 64 * NW) {
+        const int n = e >> 8, l = (e >> 2) & 63, atom = blockIdx.x * 16 + (l & 15), col = 16 * n + 4 * (l >> 4) + (e & 3);
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) v += part[w][n][l][e & 3];
+        if (atom < r && col < b) C[(size_t)atom * b + col] = v;
+    }
+}
+
 // ------------------------------------------------------------------------------------------- many columns
 // The bfloat16 matrix pipe (16x16x32), exact to float32's rounding: a float32 value is the sum of three bfloat16
 // pieces (8 + 8 + 8 bits), a bfloat16 one is its own piece.
@@ -714,7 +945,7 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
 
 // ------------------------------------------------------------------------------------------- launches
 constexpr int MOST_COLS = 2147483647 - 1024;    // tile arithmetic in int
-constexpr int FEW = 8, FEW_PRODUCT = 2;     // columns up to which the vector kernels run
+constexpr int FEW = 1, FEW_PRODUCT = 2, TILE_CORRELATE = 64;     // columns up to which the vector kernels run
 constexpr int TILE_PRODUCT = 32;             // ... and the product's tile kernel
 
 struct FewPlan { int nb, ch; };
@@ -837,6 +1068,49 @@ int product_tile(onmf_ctx* c, const TilePlan& q, int d, int r, int b, int group,
     return slab ? add_slabs(c, (size_t)d * b, b, q.splits, slab, R, ldr, s) : ONMF_OK;
 }
 
+// The correlate's tile kernel: a workgroup a CU, ranges of features that fit in its LDS and more of them (down to
+// 128 features) where there are not atoms enough.  `one`: little enough for the kernel with one launch, whose
+// workgroups take 1.2 us for 16 steps of 32 features and 16 columns (float32, three columns, us, one launch and ranges:
+// d=441 r=72 3.5 and 7.4, d=1024 r=4096 5.4 and 11.6, d=1024 r=16384 15.0 and 11.9, d=8192 r=72 21.4 and 10.8).
+struct RangePlan { bool one; int nt, per, splits, parts; };
+RangePlan correlate_tile_plan(int d, int r, int b, bool wide) {
+    RangePlan q;
+    q.nt = b <= 16 ? 1 : b <= 32 ? 2 : 4;
+    const int blocks = (d + 127) / 128, most = 144 * 1024 / (4 * 1024 * q.nt * (wide ? 3 : 1)), waves = (r + 255) / 256;
+    q.one = d <= 4096 / q.nt && (long long)((d + 31) / 32) * ((r + 15) / 16) <= 16384;
+    const int least = (blocks + most - 1) / most;
+    const int want = std::max(least, std::min(256 / waves, blocks));
+    const int each = (blocks + want - 1) / want;
+    q.per = each * 128;
+    q.splits = (blocks + each - 1) / each;
+    q.parts = std::max(1, std::min(waves, 256 / q.splits));
+    return q;
+}
+template <int NT, typename T>
+int correlate_wave(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
+                   float* C, hipStream_t s) {
+    const dim3 grid((r + 15) / 16);
+    const int groups = (d + group - 1) / group;
+    if (d <= 256)
+        hipLaunchKernelGGL((dict4_correlate_wave_kernel<NT, 4, T>), grid, dim3(256), 0, s, d, r, b, group, groups, codes, scales, X, ldx, C);
+    else
+        hipLaunchKernelGGL((dict4_correlate_wave_kernel<NT, 16, T>), grid, dim3(1024), 0, s, d, r, b, group, groups, codes, scales, X, ldx, C);
+    HIP_TRY(c, hipGetLastError());
+    return ONMF_OK;
+}
+template <int NT, typename T>
+int correlate_tile(onmf_ctx* c, const RangePlan& q, int d, int r, int b, int group, const uint32_t* codes,
+                   const uint32_t* scales, const T* X, int ldx, float* C, float* ws, hipStream_t s) {
+    const size_t bytes = (size_t)q.per / 32 * NT * (sizeof(T) == 4 ? 3 : 1) * 1024;
+    static LdsLimit lim;
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_correlate_tile_kernel<NT, T>, bytes));
+    float* slab = q.splits > 1 ? ws : nullptr;
+    hipLaunchKernelGGL((dict4_correlate_tile_kernel<NT, T>), dim3(q.parts, q.splits), dim3(512), bytes, s, d, r, b, group,
+                       (d + group - 1) / group, codes, scales, X, ldx, C, q.per, slab);
+    HIP_TRY(c, hipGetLastError());
+    return slab ? add_slabs(c, (size_t)r * b, b, q.splits, slab, C, b, s) : ONMF_OK;
+}
+
 template <bool PROD, typename T>
 int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
          float* out, int ldo, char* ws, hipStream_t s) {
@@ -892,6 +1166,15 @@ int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* cod
         FEW_CASE(4, 1); FEW_CASE(4, 2); FEW_CASE(8, 1);
 #undef FEW_CASE
     }
+    if (b <= TILE_CORRELATE) {
+        const RangePlan q = correlate_tile_plan(d, r, b, sizeof(T) == 4);
+        if (q.one && q.nt == 1) return correlate_wave<1, T>(c, d, r, b, group, codes, scales, X, ldx, C, s);
+        if (q.one && q.nt == 2) return correlate_wave<2, T>(c, d, r, b, group, codes, scales, X, ldx, C, s);
+        if (q.one) return correlate_wave<4, T>(c, d, r, b, group, codes, scales, X, ldx, C, s);
+        if (q.nt == 1) return correlate_tile<1, T>(c, q, d, r, b, group, codes, scales, X, ldx, C, ws, s);
+        if (q.nt == 2) return correlate_tile<2, T>(c, q, d, r, b, group, codes, scales, X, ldx, C, ws, s);
+        return correlate_tile<4, T>(c, q, d, r, b, group, codes, scales, X, ldx, C, ws, s);
+    }
     return many<false, T>(c, d, r, b, group, codes, scales, X, ldx, C, b, (char*)ws, s);
 }
 
@@ -926,6 +1209,11 @@ size_t onmf_dict4_workspace(int which, int d, int r, int b, int group) {
         return splits > 1 ? (size_t)splits * d * b * sizeof(float) : 0;
     }
     if (which != ONMF_DICT4_PRODUCT && b <= FEW) return 0;
+    if (which != ONMF_DICT4_PRODUCT && b <= TILE_CORRELATE) {                              // (enough for either type)
+        if (correlate_tile_plan(d, r, b, true).one) return 0;
+        const int splits = std::max(correlate_tile_plan(d, r, b, false).splits, correlate_tile_plan(d, r, b, true).splits);
+        return splits > 1 ? (size_t)splits * r * b * sizeof(float) : 0;
+    }
     const ManyPlan q = many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group, false);      // (enough for either type)
     return q.a_bytes + q.s_bytes + std::max(q.slab_bytes, many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group, true).slab_bytes);
 }
