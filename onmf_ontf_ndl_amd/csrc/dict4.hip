@@ -313,7 +313,7 @@ __global__ __launch_bounds__(64 * NW) void dict4_product_few_kernel(int d, int r
     }
 }
 
-// R = W H for 3 to 32 columns on the matrix pipe (16x16x32 bfloat16).  A lane takes the words of eight atoms: the
+// R = W H for a few to 1024 columns on the matrix pipe (16x16x32 bfloat16).  A lane takes the words of eight atoms: the
 // eight nibbles at one place are the operand of one row at eight consecutive steps of the contraction, so a tile's
 // 16 rows are the features at that place of the words of 16 lanes, and nothing has to be turned round.  An entry
 // s (q + z) has at most 16 significant bits: its upper half and the rest are bfloat16 values exactly.  Per weight
@@ -331,6 +331,7 @@ __global__ __launch_bounds__(256, 2) void dict4_product_tile_kernel(int d, int r
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, kg = lane >> 4;
     const int words = groups * (group / 8);
+    const int c0 = blockIdx.z * 16 * NT, cols = min(16 * NT, b - c0);
     const int w0 = min((int)(blockIdx.x * 16 + m) * CW, words - CW);           // (rows behind the last are not stored)
     const int g = w0 * 8 / group;
     const int ka = blockIdx.y * atoms_per_wg, kb = min(r, ka + atoms_per_wg);
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(256, 2) void dict4_product_tile_kernel(int d, int r
             }
             x.sc[j] = scales[(size_t)k * groups + g];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) x.h[j][n] = load_val(H + (size_t)k * ldh + min(16 * n + m, b - 1));
+            for (int n = 0; n < NT; ++n) x.h[j][n] = load_val(H + (size_t)k * ldh + c0 + min(16 * n + m, cols - 1));
         }
     };
     auto compute = [&](int k0, Raw& x) {
@@ -449,13 +450,13 @@ __global__ __launch_bounds__(256, 2) void dict4_product_tile_kernel(int d, int r
 #pragma unroll
         for (int w = 1; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(part + ((size_t)(w * TILES + ti) * 64 + lane) * 4);
         const int n = ti % NT * 16 + (lane & 15), j = ti / NT % 8, c = ti / NT / 8;
-        if (n >= b) continue;
+        if (n >= cols) continue;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = (((int)blockIdx.x * 16 + 4 * (lane >> 4) + e) * CW + c) * 8 + j;
             if (i >= d) continue;
-            if (slab) slab[((size_t)blockIdx.y * d + i) * b + n] = v[e];
-            else R[(size_t)i * ldr + n] = v[e];
+            if (slab) slab[((size_t)blockIdx.y * d + i) * b + c0 + n] = v[e];
+            else R[(size_t)i * ldr + c0 + n] = v[e];
         }
     }
 }
@@ -479,7 +480,7 @@ __global__ __launch_bounds__(256) void dict4_reduce_kernel(size_t mn, int N, int
     }
 }
 
-// C = W^T X for a few to 64 columns on the matrix pipe (16x16x32 bfloat16), straight from the nibbles.  The result is
+// C = W^T X for a few to 512 columns on the matrix pipe (16x16x32 bfloat16), straight from the nibbles.  The result is
 // computed with X as the rows' operand and W as the columns': a lane's operand is one word (eight features of the atom
 // l % 16, at word l / 16 of a step's four), its part of the sum belongs to that same atom, and the group's scale, which
 // the lane has, is multiplied to it; the whole numbers q + z themselves are bfloat16 values.  A workgroup keeps
@@ -496,6 +497,7 @@ __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r,
     extern __shared__ __align__(16) uint4 xop[];              // [step of 32][NT][PX][64 lanes]
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, kq = lane >> 4;
     const int words = groups * (group / 8);
+    const int c0 = blockIdx.z * 16 * NT, cols = min(16 * NT, b - c0);
     const int f0 = blockIdx.y * per, f1 = min(d, f0 + per), blocks = (f1 - f0 + 127) / 128;
 #pragma unroll 2
     for (int e = t; e < blocks * 4 * NT * 64; e += 512) {
@@ -503,7 +505,7 @@ __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r,
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const float x = load_val(X + (size_t)min(k0 + j, d - 1) * ldx + min(n, b - 1));
+            const float x = load_val(X + (size_t)min(k0 + j, d - 1) * ldx + c0 + min(n, cols - 1));
             v[j] = k0 + j < d ? x : 0.f;
         }
 #pragma unroll
@@ -585,12 +587,12 @@ __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r,
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int col = 16 * n + 4 * kq;
-                float* dst = out + (size_t)k * b + col;
-                if (k < r && col + 4 <= b) *reinterpret_cast<f32x4_any*>(dst) = acc[a][n];
+                float* dst = out + (size_t)k * b + c0 + col;
+                if (k < r && col + 4 <= cols) *reinterpret_cast<f32x4_any*>(dst) = acc[a][n];
                 else if (k < r)
 #pragma unroll
                     for (int e = 0; e < 3; ++e)
-                        if (col + e < b) dst[e] = acc[a][n][e];
+                        if (col + e < cols) dst[e] = acc[a][n][e];
             }
         }
     };
@@ -945,8 +947,13 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
 
 // ------------------------------------------------------------------------------------------- launches
 constexpr int MOST_COLS = 2147483647 - 1024;    // tile arithmetic in int
-constexpr int FEW = 1, FEW_PRODUCT = 2, TILE_CORRELATE = 64;     // columns up to which the vector kernels run
-constexpr int TILE_PRODUCT = 32;             // ... and the product's tile kernel
+constexpr int FEW = 1, FEW_PRODUCT = 2;     // columns up to which the vector kernels run
+// ... and the tile kernels, a block of columns in the grid for every 32 (product) or 64.  With more columns the weights
+// are better laid out once (us, tile and many columns' kernels: W H, d=8192 r=16384 b=192 340 and 507, b=1000 1337
+// and 1270, d=1024 r=1024 b=512 18.6 and 27.6; W^T X, float32, d=8192 r=16384 b=128 173 and 222, b=256 420 and
+// 314, d=4096 r=256 b=384 16.6 and 21.4, bfloat16, d=8192 r=16384 b=512 413 and 461).
+constexpr int TILE_PRODUCT = 1024;
+int most_tile_columns(int d, int r, bool wide) { return !wide || (long long)d * r <= 1 << 20 ? 512 : 192; }     // (the correlate's)
 
 struct FewPlan { int nb, ch; };
 FewPlan few_plan(int d, int b) {
@@ -1043,16 +1050,26 @@ int product_few(onmf_ctx* c, const FewProduct& q, int d, int r, int b, int group
 }
 
 // The tile kernel's split of the atoms: two workgroups a CU (what its registers allow), 128 atoms (a step of each wave) at least.
-struct TilePlan { int nt, cw, blocks, splits, per; };
+struct TilePlan { int nt, cw, blocks, splits, per, zs; };
 TilePlan product_tile_plan(int d, int r, int b, int group) {
     TilePlan q;
     q.nt = b <= 16 ? 1 : 2;
     q.cw = q.nt == 1 ? 2 : 1;
+    q.zs = (b + 16 * q.nt - 1) / (16 * q.nt);
     const int words = (d + group - 1) / group * (group / 8), steps = (r + 127) / 128;
     q.blocks = (words + 16 * q.cw - 1) / (16 * q.cw);
-    const int splits = std::max(1, std::min(steps, 512 / q.blocks));
-    q.per = (steps + splits - 1) / splits * 128;
-    q.splits = (r + q.per - 1) / q.per;
+    double best = -1;
+    for (int target = 0; target <= 512; target += 256) {
+        const int want = std::max(1, std::min(steps, target / (q.blocks * q.zs)));
+        const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+        const double w = (double)q.blocks * q.zs * splits;
+        double cost = std::ceil(w / 512) * per * (w > 256 ? 3.0 : 2.0);
+        if (splits > 1) cost += 4.0 + 2.5e-6 * splits * d * b;
+        if (best >= 0 && cost >= best) continue;
+        best = cost;
+        q.per = per * 128;
+        q.splits = splits;
+    }
     return q;
 }
 template <int NT, int CW, typename T>
@@ -1062,7 +1079,7 @@ int product_tile(onmf_ctx* c, const TilePlan& q, int d, int r, int b, int group,
     static LdsLimit lim;
     ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_product_tile_kernel<NT, CW, T>, bytes));
     float* slab = q.splits > 1 ? ws : nullptr;
-    hipLaunchKernelGGL((dict4_product_tile_kernel<NT, CW, T>), dim3(q.blocks, q.splits), dim3(256), bytes, s, d, r, b, group,
+    hipLaunchKernelGGL((dict4_product_tile_kernel<NT, CW, T>), dim3(q.blocks, q.splits, q.zs), dim3(256), bytes, s, d, r, b, group,
                        (d + group - 1) / group, codes, scales, H, ldh, R, ldr, q.per, slab);
     HIP_TRY(c, hipGetLastError());
     return slab ? add_slabs(c, (size_t)d * b, b, q.splits, slab, R, ldr, s) : ONMF_OK;
@@ -1072,18 +1089,19 @@ int product_tile(onmf_ctx* c, const TilePlan& q, int d, int r, int b, int group,
 // 128 features) where there are not atoms enough.  `one`: little enough for the kernel with one launch, whose
 // workgroups take 1.2 us for 16 steps of 32 features and 16 columns (float32, three columns, us, one launch and ranges:
 // d=441 r=72 3.5 and 7.4, d=1024 r=4096 5.4 and 11.6, d=1024 r=16384 15.0 and 11.9, d=8192 r=72 21.4 and 10.8).
-struct RangePlan { bool one; int nt, per, splits, parts; };
+struct RangePlan { bool one; int nt, per, splits, parts, zs; };
 RangePlan correlate_tile_plan(int d, int r, int b, bool wide) {
     RangePlan q;
     q.nt = b <= 16 ? 1 : b <= 32 ? 2 : 4;
+    q.zs = (b + 16 * q.nt - 1) / (16 * q.nt);
     const int blocks = (d + 127) / 128, most = 144 * 1024 / (4 * 1024 * q.nt * (wide ? 3 : 1)), waves = (r + 255) / 256;
-    q.one = d <= 4096 / q.nt && (long long)((d + 31) / 32) * ((r + 15) / 16) <= 16384;
+    q.one = b <= 64 && d <= 4096 / q.nt && (long long)((d + 31) / 32) * ((r + 15) / 16) <= 16384;
     const int least = (blocks + most - 1) / most;
-    const int want = std::max(least, std::min(256 / waves, blocks));
+    const int want = std::max(least, std::min(256 / (waves * q.zs), blocks));
     const int each = (blocks + want - 1) / want;
     q.per = each * 128;
     q.splits = (blocks + each - 1) / each;
-    q.parts = std::max(1, std::min(waves, 256 / q.splits));
+    q.parts = std::max(1, std::min(waves, 256 / (q.splits * q.zs)));
     return q;
 }
 template <int NT, typename T>
@@ -1105,7 +1123,7 @@ int correlate_tile(onmf_ctx* c, const RangePlan& q, int d, int r, int b, int gro
     static LdsLimit lim;
     ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_correlate_tile_kernel<NT, T>, bytes));
     float* slab = q.splits > 1 ? ws : nullptr;
-    hipLaunchKernelGGL((dict4_correlate_tile_kernel<NT, T>), dim3(q.parts, q.splits), dim3(512), bytes, s, d, r, b, group,
+    hipLaunchKernelGGL((dict4_correlate_tile_kernel<NT, T>), dim3(q.parts, q.splits, q.zs), dim3(512), bytes, s, d, r, b, group,
                        (d + group - 1) / group, codes, scales, X, ldx, C, q.per, slab);
     HIP_TRY(c, hipGetLastError());
     return slab ? add_slabs(c, (size_t)r * b, b, q.splits, slab, C, b, s) : ONMF_OK;
@@ -1156,6 +1174,21 @@ int check4(onmf_ctx* c, const char* what, int d, int r, int group, const void* c
     return ONMF_OK;
 }
 
+size_t workspace_of(bool prod, int d, int r, int b, int group, bool wide) {
+    int splits = 1;
+    if (prod && b <= FEW_PRODUCT) splits = product_few_plan(d, r, b).splits;
+    else if (prod && b <= TILE_PRODUCT) splits = product_tile_plan(d, r, b, group).splits;
+    else if (!prod && b <= FEW) splits = 1;
+    else if (!prod && b <= most_tile_columns(d, r, wide)) {
+        const RangePlan q = correlate_tile_plan(d, r, b, wide);
+        splits = q.one ? 1 : q.splits;
+    } else {
+        const ManyPlan q = many_plan(prod, d, r, b, group, wide);
+        return q.a_bytes + q.s_bytes + q.slab_bytes;
+    }
+    return splits > 1 ? (size_t)splits * (prod ? d : r) * b * sizeof(float) : 0;
+}
+
 template <typename T>
 int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X,
                 int ldx, float* C, float* ws, hipStream_t s) {
@@ -1166,7 +1199,7 @@ int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* cod
         FEW_CASE(4, 1); FEW_CASE(4, 2); FEW_CASE(8, 1);
 #undef FEW_CASE
     }
-    if (b <= TILE_CORRELATE) {
+    if (b <= most_tile_columns(d, r, sizeof(T) == 4)) {
         const RangePlan q = correlate_tile_plan(d, r, b, sizeof(T) == 4);
         if (q.one && q.nt == 1) return correlate_wave<1, T>(c, d, r, b, group, codes, scales, X, ldx, C, s);
         if (q.one && q.nt == 2) return correlate_wave<2, T>(c, d, r, b, group, codes, scales, X, ldx, C, s);
@@ -1204,18 +1237,9 @@ extern "C" {
 
 size_t onmf_dict4_workspace(int which, int d, int r, int b, int group) {
     if (d <= 0 || r <= 0 || b <= 0 || (group != 32 && group != 64 && group != 128)) return 0;
-    if (which == ONMF_DICT4_PRODUCT && b <= TILE_PRODUCT) {
-        const int splits = b <= FEW_PRODUCT ? product_few_plan(d, r, b).splits : product_tile_plan(d, r, b, group).splits;
-        return splits > 1 ? (size_t)splits * d * b * sizeof(float) : 0;
-    }
-    if (which != ONMF_DICT4_PRODUCT && b <= FEW) return 0;
-    if (which != ONMF_DICT4_PRODUCT && b <= TILE_CORRELATE) {                              // (enough for either type)
-        if (correlate_tile_plan(d, r, b, true).one) return 0;
-        const int splits = std::max(correlate_tile_plan(d, r, b, false).splits, correlate_tile_plan(d, r, b, true).splits);
-        return splits > 1 ? (size_t)splits * r * b * sizeof(float) : 0;
-    }
-    const ManyPlan q = many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group, false);      // (enough for either type)
-    return q.a_bytes + q.s_bytes + std::max(q.slab_bytes, many_plan(which == ONMF_DICT4_PRODUCT, d, r, b, group, true).slab_bytes);
+    size_t need = 0;                                    // enough for either type of the columns
+    for (const bool wide : {false, true}) need = std::max(need, workspace_of(which == ONMF_DICT4_PRODUCT, d, r, b, group, wide));
+    return need;
 }
 
 int onmf_dict4_pack(onmf_ctx* c, int d, int r, int group, const float* W, void* codes, int32_t* scales, void* stream) {

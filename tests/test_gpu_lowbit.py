@@ -88,6 +88,8 @@ SHAPES = [  # d, r, b, group: single columns, a few, many; ragged and whole; one
     (100, 16, 2, 64), (2100, 33, 2, 32), (441, 25, 3, 64), (1030, 130, 4, 128), (513, 257, 5, 32), (1500, 40, 8, 64),
     (9000, 5, 8, 128), (1, 1, 9, 32), (33, 129, 9, 32), (441, 25, 17, 64), (100, 16, 130, 64), (128, 128, 128, 128),
     (257, 300, 33, 32), (1200, 100, 257, 64), (1024, 256, 300, 128), (130, 2000, 65, 64), (4096, 40, 100, 64),
+    (8192, 20, 3, 64), (1100, 8200, 2, 32), (700, 9000, 31, 64), (2100, 4000, 64, 128), (3, 5000, 64, 32),
+    (60, 40, 1100, 32), (300, 70, 1501, 64), (200, 6001, 200, 32), (2100, 600, 601, 128), (33, 3, 1025, 32), (777, 1400, 1027, 64),
 ]
 
 
@@ -123,7 +125,7 @@ def test_products_of_real_values(eng, torch, d, r, b, group, dtype):
     assert (np.abs(R - Wq @ Hh) <= STEP * (r / 4 + 64) * (M @ np.abs(Hh))).all()
 
 
-@pytest.mark.parametrize("b", [1, 3, 8, 40])
+@pytest.mark.parametrize("b", [1, 3, 8, 40, 601, 1101])
 def test_products_take_views(eng, torch, b):
     """Columns of a wider matrix, a transposed one, every second column, one value for all."""
     rs = np.random.RandomState(b)
@@ -136,7 +138,7 @@ def test_products_take_views(eng, torch, b):
     for X in (wide[:, 1:b + 1], wide[:, 4:b + 4], tall.t(), wide[:, 0:2 * b:2], one.expand(d, b), wide.bfloat16()[:, 3:b + 3]):
         assert np.array_equal(host(eng.dict4_correlate(P, X)), W.T @ host(X))
     codes = eng.dev(rs.randint(-3, 4, size=(r, 2 * b + 7)).astype(np.float32))
-    for H in (codes[:, 1:b + 1], codes[:, 0:2 * b:2], codes.bfloat16()[:, 5:b + 5], codes[:b, :r].t()[:, :1] if b <= r else codes[:, :1]):
+    for H in (codes[:, 1:b + 1], codes.bfloat16()[:, 2:b + 2], codes[:, 0:2 * b:2], codes.bfloat16()[:, 5:b + 5], codes[:b, :r].t()[:, :1] if b <= r else codes[:, :1]):
         if H.shape[0] == r:
             assert np.array_equal(host(eng.dict4_product(P, H)), W @ host(H))
 
@@ -152,7 +154,7 @@ def test_rows_that_lie_far_apart(eng, torch, dtype):
     W = lo.values4(*parts, d)
     Q, qarts = whole_dictionary(eng, rs, 37, d, 32)
     V = lo.values4(*qarts, 37)
-    for b in (1, 2, 5, 20, 41):
+    for b in (1, 2, 5, 20, 41, 601, 1101):
         X, Xh = as_type(torch, eng, rs.randint(-4, 5, size=(d, b)), dtype)
         wide[:, 7:7 + b] = X
         view = wide[:, 7:7 + b]
@@ -163,7 +165,7 @@ def test_rows_that_lie_far_apart(eng, torch, dtype):
         assert np.array_equal(K.codes.cpu().numpy(), q) and np.array_equal(host(K.scales), s)
 
 
-@pytest.mark.parametrize("b", [1, 2, 4, 7, 8, 9, 100])
+@pytest.mark.parametrize("b", [1, 2, 4, 7, 8, 9, 100, 601, 1101])
 def test_a_column_that_is_not_finite_touches_no_other(eng, torch, b):
     rs = np.random.RandomState(b)
     d, r = 200, 150
@@ -179,7 +181,7 @@ def test_a_column_that_is_not_finite_touches_no_other(eng, torch, b):
     assert np.isnan(C_[:, bad]).all() and not np.isfinite(R[W[:, 5] != 0, bad]).any()
 
 
-@pytest.mark.parametrize("b", [1, 5, 40])
+@pytest.mark.parametrize("b", [1, 5, 40, 1101])
 def test_product_leaves_what_lies_behind_its_rows(eng, torch, b):
     from onmf_ontf_ndl_amd.engine import _ptr
     rs = np.random.RandomState(b)
