@@ -435,54 +435,75 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 }
 
 // dW[i][k] = sum_j W[i][j] A[j][k] - B[k][i] in double, rounded once: near a stationary dictionary the two terms
-// nearly cancel.  32 x 32 tiles, a 16 x 16 one a wave on the double matrix pipe (16x16x4: row l % 16 and column
-// l % 16 of the operands at j + l / 16, output row 4 e + l / 16); the next 32 steps of j are loaded into registers
-// while these are computed.  Rows of 36 and 48 doubles: an operand read's 64 lanes meet every bank alike.
-// (64 x 64 tiles leave too few waves to wait for memory: d=4096 r=256 20 -> 26 us.)
+// nearly cancel.  A workgroup owns a 32 x 32 tile, its NW waves share the sum over j in sixteens and add up in LDS.  A
+// wave loads the double matrix pipe's operands (16x16x4) straight into registers, the next sixteen while these are
+// computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
+// row 4 e + l / 16.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-__global__ __launch_bounds__(256) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
-                                                              const double* __restrict__ A,
-                                                              const double* __restrict__ B, float* __restrict__ dW) {
-    __shared__ double tw[32][36], ta[32][48], tb[32][33];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
+                                                                  const double* __restrict__ A,
+                                                                  const double* __restrict__ B, float* __restrict__ dW) {
+    __shared__ double part[NW][32][32], tb[32][33];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, quad = lane >> 4;
     const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
-    const int wi = (wave & 1) * 16, wk = (wave >> 1) * 16;
-    const int row = t >> 5, col = t & 31;                   // and the rows 8, 16, 24 behind it
-    float vw[4];
-    double va[4];
-    auto fetch = [&](int j0) {
+    for (int e = t; e < 1024; e += 64 * NW) {
+        const int k = k0 + (e >> 5), i = i0 + (e & 31);
+        tb[e & 31][e >> 5] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
+    }
+    // (rows and columns behind the last ones are the last ones and not stored, behind the last j the weight is zero)
+    const float* row[2] = {W + (size_t)min(i0 + m, d - 1) * r, W + (size_t)min(i0 + 16 + m, d - 1) * r};
+    const int col[2] = {min(k0 + m, r - 1), min(k0 + 16 + m, r - 1)};
+    struct Step { f32x4_any w[2]; double a[4][2]; };
+    auto fetch = [&](int j0, Step& v) {
+        const int j = j0 + 4 * quad;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int y = row + 8 * q;
-            vw[q] = (i0 + y < d && j0 + col < r) ? W[(size_t)(i0 + y) * r + j0 + col] : 0.f;
-            va[q] = (j0 + y < r && k0 + col < r) ? A[(size_t)(j0 + y) * r + k0 + col] : 0.0;
+        for (int h = 0; h < 2; ++h) {
+            if (j0 + 16 <= r) v.w[h] = *reinterpret_cast<const f32x4_any*>(row[h] + j);
+            else
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v.w[h][i] = j + i < r ? row[h][j + i] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v.a[i][h] = A[(size_t)min(j + i, r - 1) * r + col[h]];
         }
     };
-    fetch(0);
+    f64x4 acc[2][2];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int k = k0 + row + 8 * q, i = i0 + col;
-        tb[col][row + 8 * q] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
+    for (int h = 0; h < 2; ++h) acc[h][0] = acc[h][1] = f64x4{0.0, 0.0, 0.0, 0.0};
+    auto compute = [&](const Step& v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+                    acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v.w[h][i], v.a[i][c], acc[h][c], 0, 0, 0);
+    };
+    Step even, odd;
+    int j0 = wave * 16;
+    if (j0 < r) fetch(j0, even);
+    while (j0 < r) {
+        if (j0 + 16 * NW < r) fetch(j0 + 16 * NW, odd);
+        compute(even);
+        j0 += 16 * NW;
+        if (j0 >= r) break;
+        if (j0 + 16 * NW < r) fetch(j0 + 16 * NW, even);
+        compute(odd);
+        j0 += 16 * NW;
     }
-    f64x4 acc = f64x4{0.0, 0.0, 0.0, 0.0};
-    for (int j0 = 0; j0 < r; j0 += 32) {
-        __syncthreads();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            tw[row + 8 * q][col] = (double)vw[q];
-            ta[row + 8 * q][col] = va[q];
-        }
-        __syncthreads();
-        if (j0 + 32 < r) fetch(j0 + 32);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-            acc = __builtin_amdgcn_mfma_f64_16x16x4f64(tw[wi + (lane & 15)][j + (lane >> 4)],
-                                                       ta[j + (lane >> 4)][wk + (lane & 15)], acc, 0, 0, 0);
-    }
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const int i = wi + 4 * e + (lane >> 4), k = wk + (lane & 15);
-        if (i0 + i < d && k0 + k < r) dW[(size_t)(i0 + i) * r + k0 + k] = (float)(acc[e] - tb[i][k]);
+            for (int e = 0; e < 4; ++e) part[wave][16 * h + 4 * e + quad][16 * c + m] = acc[h][c][e];
+    __syncthreads();
+    for (int e = t; e < 1024; e += 64 * NW) {
+        const int i = e >> 5, k = e & 31;
+        double v = part[0][i][k];
+#pragma unroll
+        for (int z = 1; z < NW; ++z) v += part[z][i][k];
+        if (i0 + i < d && k0 + k < r) dW[(size_t)(i0 + i) * r + k0 + k] = (float)(v - tb[i][k]);
     }
 }
 
@@ -801,8 +822,13 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
     double* Ad = (double*)((char*)ws + sums_bytes(sum_plan(d, r, n), r));
     ONMF_TRY(run_sums(c, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
                       Ad, Ad + (size_t)r * r, s));
-    hipLaunchKernelGGL(keep8_gradient_kernel, dim3((r + 31) / 32, (d + 31) / 32), dim3(256), 0, s, d, r, W, Ad,
-                       Ad + (size_t)r * r, dW);
+    const dim3 grid((r + 31) / 32, (d + 31) / 32);
+    // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
+    // tiles the double matrix pipe is what counts: d=4096 r=1024 197 us, with eight waves 217)
+    if (r > 64 && (size_t)grid.x * grid.y <= 512)
+        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, Ad, Ad + (size_t)r * r, dW);
+    else
+        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, Ad, Ad + (size_t)r * r, dW);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
