@@ -8,6 +8,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <cmath>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 // rows of any length: vectors that need no more alignment than their entries (the memory pipe takes them as they lie)
@@ -208,11 +209,10 @@ struct SumParams {
     int d, r, groups, per_split, splits;
     int tiles_m, tiles_h, tiles;     // tiles along r (rows); column tiles of the H H^T part; all tiles
     int cols_h, cols;         // columns of a slab row: the H H^T part's, all (both multiples of 4)
-    // one run holds everything: the results at once, A and B or (the gradient) Ad and Bd
+    // one run holds everything: the results at once
     double w, keep;
     const float *A_in, *B_in;
     float *A, *B;
-    double *Ad, *Bd;
 };
 
 template <typename S>
@@ -347,7 +347,6 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
     if (p.splits == 1) {
         const float* in = is_h ? p.A_in : p.B_in;
         float* out = is_h ? p.A : p.B;
-        double* sums = is_h ? p.Ad : p.Bd;
 #pragma unroll
         for (int i = 0; i < S::mi; ++i) {
             const int m = m0 + wm + 16 * i + (lane & 15);
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
             for (int j = 0; j < S::nj; ++j) {
                 const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
                 const size_t at = (size_t)m * N + n;
-                if (n + 3 < N && !sums) {
+                if (n + 3 < N) {
                     f32x4_any v = {0.f, 0.f, 0.f, 0.f};
                     if (in) v = *reinterpret_cast<const f32x4_any*>(in + at);
 #pragma unroll
@@ -367,8 +366,7 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     if (n + e >= N) continue;
-                    if (sums) sums[at + e] = (double)acc[i][j][e];
-                    else out[at + e] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at + e] : 0.0));
+                    out[at + e] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at + e] : 0.0));
                 }
             }
         }
@@ -440,21 +438,21 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
 // row 4 e + l / 16.
 typedef double f64x4 __attribute__((ext_vector_type(4)));
-template <int NW>
+template <int NW, typename S>
 __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
-                                                                  const double* __restrict__ A,
-                                                                  const double* __restrict__ B, float* __restrict__ dW) {
+                                                                  const S* __restrict__ A, const S* __restrict__ B,
+                                                                  float* __restrict__ dW) {
     __shared__ double part[NW][32][32], tb[32][33];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, quad = lane >> 4;
     const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
     for (int e = t; e < 1024; e += 64 * NW) {
         const int k = k0 + (e >> 5), i = i0 + (e & 31);
-        tb[e & 31][e >> 5] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
+        tb[e & 31][e >> 5] = (k < r && i < d) ? (double)B[(size_t)k * d + i] : 0.0;
     }
     // (rows and columns behind the last ones are the last ones and not stored, behind the last j the weight is zero)
     const float* row[2] = {W + (size_t)min(i0 + m, d - 1) * r, W + (size_t)min(i0 + 16 + m, d - 1) * r};
     const int col[2] = {min(k0 + m, r - 1), min(k0 + 16 + m, r - 1)};
-    struct Step { f32x4_any w[2]; double a[4][2]; };
+    struct Step { f32x4_any w[2]; S a[4][2]; };
     auto fetch = [&](int j0, Step& v) {
         const int j = j0 + 4 * quad;
 #pragma unroll
@@ -477,7 +475,7 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                    acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v.w[h][i], v.a[i][c], acc[h][c], 0, 0, 0);
+                    acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v.w[h][i], (double)v.a[i][c], acc[h][c], 0, 0, 0);
     };
     Step even, odd;
     int j0 = wave * 16;
@@ -608,33 +606,51 @@ __global__ __launch_bounds__(64 * NW) void keep8_residual_kernel(int d, int r, c
 }
 
 // ------------------------------------------------------------------------------------------- launches
-// The tile follows r, so that X is read once: its columns are the wider the fewer rows there are.
 using Wide = Tile<4, 2, 4, 4, 3>;       // 256 x 128
 using Middle = Tile<4, 2, 2, 8, 3>;     // 128 x 256
 using Narrow = Tile<4, 2, 1, 8, 3>;     // 64 x 256
 using Slim = Tile<2, 2, 1, 4, 6>;       // 32 x 128
 
-constexpr int ONE_RUN = 8;
-struct SumPlan { int tile, bm, bn, tiles_m, tiles_h, tiles_x, cols_h, cols, splits, per; };
+struct SumPlan { int tile, bm, bn, tiles_m, tiles_h, tiles_x, cols_h, cols, splits, per; double cost; };
+// The tile and the number of runs with the least time by what was measured of them: a tile's own time (us: filling the ring,
+// writing the sums), what a group takes it - its operations, or with the chip full its codes' way from the caches at
+// 8 TB/s - and, with several runs, a second launch and the slabs' way through memory at 4 TB/s.  One workgroup a CU.
+// (us: d=8192 r=64 n=1000 64 x 256 13.2, 32 x 128 6.4; d=8192 r=256 n=1000 256 x 128 20, 64 x 256 12; d=4096 r=256
+// n=65536 256 x 128 125, 64 x 256 180; d=1200 r=100 n=8191 in runs of four groups 17.3, of two 20.3.)
 SumPlan sum_plan(int d, int r, int n) {
+    static constexpr struct { int bm, bn, rows; double own, group; } kind[4] = {{Slim::bm, Slim::bn, Slim::rows, 2.4, 0.5},
+                                                                                 {Narrow::bm, Narrow::bn, Narrow::rows, 5.0, 0.87},
+                                                                                 {Middle::bm, Middle::bn, Middle::rows, 7.0, 1.25},
+                                                                                 {Wide::bm, Wide::bn, Wide::rows, 9.6, 1.2}};
     SumPlan q;
     const int groups = (n + GROUP - 1) / GROUP;
-    const int tile[4][2] = {{Slim::bm, Slim::bn}, {Narrow::bm, Narrow::bn}, {Middle::bm, Middle::bn}, {Wide::bm, Wide::bn}};
-    q.tile = r <= Slim::bm ? 0 : r <= Narrow::bm ? 1 : r <= Middle::bm ? 2 : 3;
-    q.bm = tile[q.tile][0];
-    q.bn = tile[q.tile][1];
-    q.tiles_m = (r + q.bm - 1) / q.bm;
-    q.tiles_h = (r + q.bn - 1) / q.bn;
-    q.tiles_x = (d + q.bn - 1) / q.bn;
     q.cols_h = (r + 3) & ~3;
     q.cols = q.cols_h + ((d + 3) & ~3);
-    const long long tiles = (long long)q.tiles_m * (q.tiles_h + q.tiles_x);
-    // A short contraction in one run, with nothing to add up behind it; otherwise a workgroup per CU and four groups
-    // a run at least (d=1200 r=100 n=8191: 17.3 us, with two groups a run and twice the slabs 20.3).
-    long long splits = groups <= ONE_RUN ? 1 : std::max<long long>(1, 256 / tiles);
-    splits = std::min<long long>(splits, (groups + 3) / 4);
-    q.per = (int)((groups + splits - 1) / splits);
-    q.splits = (groups + q.per - 1) / q.per;
+    double best = -1;
+    for (int i = 0; i < 4; ++i) {
+        if (i > 0 && r <= kind[i - 1].bm) break;
+        const int tiles_m = (r + kind[i].bm - 1) / kind[i].bm, tiles_h = (r + kind[i].bn - 1) / kind[i].bn;
+        const int tiles_x = (d + kind[i].bn - 1) / kind[i].bn;
+        const double tiles = (double)tiles_m * (tiles_h + tiles_x);
+        for (int target = 0; target <= 512; target = target ? 2 * target : 64) {
+            const int want = (int)std::max(1.0, std::min(target / tiles, (double)groups));
+            const int per = (groups + want - 1) / want, splits = (groups + per - 1) / per;
+            const double w = tiles * splits;
+            double cost = std::ceil(w / 256) *
+                          (kind[i].own + per * std::max(kind[i].group, kind[i].rows * (double)GROUP * std::min(w, 256.0) / 8e6));
+            if (splits > 1) cost += 5.0 + 2e-6 * splits * r * q.cols;
+            if (best >= 0 && cost >= best) continue;
+            best = q.cost = cost;
+            q.tile = i;
+            q.bm = kind[i].bm;
+            q.bn = kind[i].bn;
+            q.tiles_m = tiles_m;
+            q.tiles_h = tiles_h;
+            q.tiles_x = tiles_x;
+            q.per = per;
+            q.splits = splits;
+        }
+    }
     return q;
 }
 size_t sums_bytes(const SumPlan& q, int r) {
@@ -660,16 +676,15 @@ int launch_sums(onmf_ctx* c, const SumParams& p, hipStream_t s) {
 }
 
 // The sums of a minibatch into A and B, or as doubles into Ad and Bd.
-int run_sums(onmf_ctx* c, int d, int r, int n, const int8_t* xc, const float* xs, const int8_t* hc, const float* hs,
+int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* xc, const float* xs, const int8_t* hc, const float* hs,
              float* slab, double w, double keep, const float* A_in, const float* B_in, float* A, float* B, double* Ad,
              double* Bd, hipStream_t s) {
-    const SumPlan q = sum_plan(d, r, n);
     SumParams p;
     p.hc = hc; p.xc = xc; p.hs = hs; p.xs = xs; p.slab = slab;
     p.d = d; p.r = r; p.groups = (n + GROUP - 1) / GROUP; p.per_split = q.per; p.splits = q.splits;
     p.tiles_m = q.tiles_m; p.tiles_h = q.tiles_h; p.tiles = q.tiles_m * (q.tiles_h + q.tiles_x);
     p.cols_h = q.cols_h; p.cols = q.cols;
-    p.w = w; p.keep = keep; p.A_in = A_in; p.B_in = B_in; p.A = A; p.B = B; p.Ad = Ad; p.Bd = Bd;
+    p.w = w; p.keep = keep; p.A_in = A_in; p.B_in = B_in; p.A = A; p.B = B;
     switch (q.tile) {
         case 0: ONMF_TRY(launch_sums<Slim>(c, p, s)); break;
         case 1: ONMF_TRY(launch_sums<Narrow>(c, p, s)); break;
@@ -689,11 +704,26 @@ int run_sums(onmf_ctx* c, int d, int r, int n, const int8_t* xc, const float* xs
     return ONMF_OK;
 }
 
-// The residual costs d r and the columns that its tiles hold, W (H H^T) costs d r^2 and a launch or two more.  Measured
-// (us, residual and sums): d=441 r=25 n=128 6.0 and 8.0; d=2372 r=581 n=2 9.6 and 73; d=8192 r=64 n=128 11.8 and 18;
-// d=65536 r=64 n=128 83 and 49, n=16 24 and 49.
-bool by_residual(int d, int r, int n) {
-    return n <= GROUP && (d <= 8192 || r >= (n <= 16 ? 16 : n <= 64 ? 64 : GROUP));
+template <typename S>
+int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const S* A, const S* B, float* dW, hipStream_t s) {
+    const dim3 grid((r + 31) / 32, (d + 31) / 32);
+    // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
+    // tiles the double matrix pipe is what counts: d=4096 r=1024 197 us, with eight waves 217)
+    if (r > 64 && (size_t)grid.x * grid.y <= 512)
+        hipLaunchKernelGGL((keep8_gradient_kernel<8, S>), grid, dim3(512), 0, s, d, r, W, A, B, dW);
+    else
+        hipLaunchKernelGGL((keep8_gradient_kernel<4, S>), grid, dim3(256), 0, s, d, r, W, A, B, dW);
+    HIP_TRY(c, hipGetLastError());
+    return ONMF_OK;
+}
+
+// The residual costs a workgroup r times the columns that its tiles hold; the sums a launch more and W (H H^T), d r^2
+// at 45 TFLOP/s.  In us, from measurements (residual and sums: d=441 r=25 n=128 6.0 and 9; d=2372 r=581 n=2 9.6 and
+// 60; d=60 r=1024 n=100 43 and 22; d=65536 r=64 n=128 83 and 49, n=16 24 and 49).
+bool by_residual(const SumPlan& q, int d, int r, int n) {
+    if (n > GROUP) return false;
+    const double residual = 2.5 + std::ceil(d / (n <= 16 ? 8192.0 : 4096.0)) * (1.0 + r * (n <= 16 ? 0.009 : n <= 64 ? 0.023 : 0.04));
+    return residual < q.cost + 6.0 + 0.011 * r + 2.0 * d * r * r / 45e6;
 }
 
 template <int TILES, int NW>
@@ -780,8 +810,9 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
 
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
     if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;
-    if (gradient && by_residual(d, r, n)) return 0;
-    return sums_bytes(sum_plan(d, r, n), r) + (gradient ? sizeof(double) * (size_t)r * ((size_t)r + d) : 0);
+    const SumPlan q = sum_plan(d, r, n);
+    if (gradient && by_residual(q, d, r, n)) return 0;
+    return sums_bytes(q, r) + (gradient ? (q.splits == 1 ? sizeof(float) : sizeof(double)) * (size_t)r * ((size_t)r + d) : 0);
 }
 
 int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes, const float* x_scales,
@@ -796,7 +827,7 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    return run_sums(c, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr,
+    return run_sums(c, sum_plan(d, r, n), d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr,
                     nullptr, s);
 }
 
@@ -814,23 +845,22 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    if (by_residual(d, r, n)) {
+    const SumPlan q = sum_plan(d, r, n);
+    if (by_residual(q, d, r, n)) {
         if (n <= 16) return launch_residual<1, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
         if (n <= 64) return launch_residual<4, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
         return launch_residual<8, 8>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
     }
-    double* Ad = (double*)((char*)ws + sums_bytes(sum_plan(d, r, n), r));
-    ONMF_TRY(run_sums(c, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
-                      Ad, Ad + (size_t)r * r, s));
-    const dim3 grid((r + 31) / 32, (d + 31) / 32);
-    // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
-    // tiles the double matrix pipe is what counts: d=4096 r=1024 197 us, with eight waves 217)
-    if (r > 64 && (size_t)grid.x * grid.y <= 512)
-        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, Ad, Ad + (size_t)r * r, dW);
-    else
-        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, Ad, Ad + (size_t)r * r, dW);
-    HIP_TRY(c, hipGetLastError());
-    return ONMF_OK;
+    if (q.splits == 1) {                    // (sums of one run are float32 values)
+        float* A = (float*)ws;
+        ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, nullptr, 1.0, 0.0, nullptr, nullptr, A,
+                          A + (size_t)r * r, nullptr, nullptr, s));
+        return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, s);
+    }
+    double* A = (double*)((char*)ws + sums_bytes(q, r));
+    ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
+                      A, A + (size_t)r * r, s));
+    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, s);
 }
 
 }  // extern "C"

@@ -208,9 +208,10 @@ def test_workspaces_are_bounded():
                     assert n % 4 == 0 and n <= laid + 1024 * 256 * 128 * 4
         assert lib.onmf_dict4_workspace(which, 0, 4, 4, 64) == 0
         assert lib.onmf_dict4_workspace(which, 4, 4, 4, 48) == 0
-    for d, r, n in ((441, 25, 128), (8192, 1024, 1), (60000, 300, 100)):     # by way of the residual: none
+    for d, r, n in ((441, 25, 128), (8192, 1024, 1), (4096, 300, 100)):     # by way of the residual: none
         assert lib.onmf_keep8_workspace(d, r, n, 1) == 0
-    for d, r, n in ((441, 25, 1000), (1024, 256, 65536), (8192, 1024, 129), (60000, 20, 100)):
+    # a slab for each run of groups (512 workgroups of 256 x 128 results at most), and the sums: doubles, with one run floats
+    for d, r, n in ((441, 25, 1000), (1024, 256, 65536), (8192, 1024, 129), (60000, 20, 100), (60, 1024, 100)):
         plain, with_gradient = lib.onmf_keep8_workspace(d, r, n, 0), lib.onmf_keep8_workspace(d, r, n, 1)
-        assert with_gradient == plain + 8 * r * (r + d) and plain <= 256 * 256 * 128 * 4 + 512 * 4 * r * 8
+        assert with_gradient == plain + (8 if plain else 4) * r * (r + d) and plain <= 512 * 256 * 128 * 4
     assert lib.onmf_keep8_workspace(0, 4, 4, 0) == 0
