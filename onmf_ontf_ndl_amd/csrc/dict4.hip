@@ -18,7 +18,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // rows of any length: pairs that need no more alignment than their entries (the memory pipe takes them as they lie)
 typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u32_any __attribute__((aligned(2)));
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 namespace {
 
@@ -720,11 +720,12 @@ __global__ __launch_bounds__(64 * NW) void dict4_correlate_wave_kernel(int d, in
 //             products of pieces the last (2^-24) is left out.
 // The weights are laid out as bfloat16 rows [piece][m][k] in the workspace first (unpacked in the product's kernel
 // itself they cost every 128 columns as many vector instructions as the columns' own split).
-// A workgroup owns 16 MT rows and 128 columns, a wave all its rows and 32 columns, so that every column is split
-// into its pieces once and in registers: lane l holds columns 2 (l % 16) and the next, at k = 8 (l / 16) .. + 7,
-// the operand of two tiles.  The weights go from memory to LDS, one step of 32 ahead, in rows of 64 bytes whose
+// A workgroup owns 16 MT rows and 128 (bfloat16: 256) columns, a wave all its rows and a quarter of its columns, so
+// that every column is split into its pieces once and in registers: lane l holds columns 2 (l % 16) and the next, at
+// k = 8 (l / 16) .. + 7, the operand of two tiles.  (bfloat16 columns need no split and a wave takes four tiles of
+// them, for half the reads of weights from LDS, which bound it before: d=1024 r=256 b=65536 66 -> 52 us.)  The weights go from memory to LDS, one step of 32 ahead, in rows of 64 bytes whose
 // 16-byte chunks are permuted by (row >> 2) & 3: the 16 rows of an operand read meet every bank once.
-constexpr int BK = 32, BN = 128;
+constexpr int BK = 32;
 
 // correlate's weights: [k][features, padded to whole groups with zeros] whole numbers, and the scales as floats [group][k]
 __global__ __launch_bounds__(256) void dict4_lay_correlate_kernel(int d, int r, int words, int group, int groups,
@@ -791,20 +792,14 @@ struct ManyParams {
     int tiles_m, tiles, k_per_split;
 };
 
-// two columns of a row, as they lie
-__device__ __forceinline__ void load_two(const float* p, float& a, float& b) {
-    const f32x2_any v = *reinterpret_cast<const f32x2_any*>(p);
-    a = v[0]; b = v[1];
-}
-__device__ __forceinline__ void load_two(const uint16_t* p, float& a, float& b) {
-    const uint32_t v = *reinterpret_cast<const u32_any*>(p);
-    a = bf16_lo(v); b = bf16_hi(v);
-}
+// a wave's columns in sixteens, as many as a lane loads at once: two float32 values or four bfloat16 ones
+template <typename T> constexpr int COLUMN_TILES = sizeof(T) == 4 ? 2 : 4;
 
 // OFF: 32 bits where 32 rows of X lie within them
 template <bool PROD, typename T, int MT, typename OFF>
 __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     constexpr int PX = sizeof(T) == 4 ? 3 : 1;        // pieces of the float operand
+    constexpr int CT = COLUMN_TILES<T>;
     constexpr int PW = PROD ? 2 : 1;                   // pieces of the weights
     constexpr int ROWS = PW * 16 * MT, STAGE = ROWS * 64;
     constexpr int SROWS = PROD ? 0 : (16 * MT + 63) / 64 * 64;
@@ -814,13 +809,13 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     // row tiles of the same columns follow each other on one XCD
     const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (at >= p.tiles) return;
-    const int m0 = (at % p.tiles_m) * 16 * MT, n0 = (at / p.tiles_m) * BN + wave * 32;
+    const int m0 = (at % p.tiles_m) * 16 * MT, n0 = (at / p.tiles_m) * 64 * CT + wave * 16 * CT;
     const int kbeg = blockIdx.y * p.k_per_split, kend = min(p.K, kbeg + p.k_per_split);
     const int steps = (kend - kbeg + BK - 1) / BK;
-    // Columns behind the last one read the last two (their results are not stored; where the last one is the first of
-    // its pair it is taken from the second place), rows behind the last one the last one (the weights are zero there).
-    const int na = min(n0 + 2 * (lane & 15), p.N - 2);
-    const bool second = n0 + 2 * (lane & 15) > na;
+    // Columns behind the last one are not stored.  A lane that has some reads the last CT columns, its own first among
+    // them at place `late`; rows behind the last one are the last one (the weights are zero there).
+    const int na = min(n0 + CT * (lane & 15), p.N - CT), late = min(n0 + CT * (lane & 15) - na, CT - 1);
+    const bool some_late = __any(late);
     const int kl = 8 * (lane >> 4);
 
     // 16 rows of weights a load: a base for the wave and 32 bits a lane
@@ -848,37 +843,53 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
                     (const __attribute__((address_space(1))) void*)((const char*)(p.S + (size_t)(k / p.group) * p.M) + soff),
                     (__attribute__((address_space(3))) void*)(lscale + buf * SROWS + wave * 64), 4, 0, 0);
     };
-    float xr[8][2];
+    u32x2_any xr[8];
     auto fetch_x = [&](int k) {                       // (k < K: the rows are counted from k's)
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            load_two((const T*)((const char*)p.X + (size_t)k * p.ldx * sizeof(T) +
-                                ((OFF)min(kl + j, p.K - 1 - k) * (OFF)p.ldx + (OFF)na) * (OFF)sizeof(T)), xr[j][0], xr[j][1]);
+            xr[j] = *reinterpret_cast<const u32x2_any*>((const char*)p.X + (size_t)k * p.ldx * sizeof(T) +
+                                                        ((OFF)min(kl + j, p.K - 1 - k) * (OFF)p.ldx + (OFF)na) * (OFF)sizeof(T));
     };
-    uint4 fb[2][PX];
+    uint4 fb[CT][PX];
     auto split_x = [&]() {
+        if (some_late)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float v[8];
+            for (int j = 0; j < 8; ++j) {
+                const uint64_t v = ((uint64_t)xr[j][1] << 32 | xr[j][0]) >> (late * (64 / CT));
+                xr[j][0] = (uint32_t)v;
+                xr[j][1] = (uint32_t)(v >> 32);
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c == 0 && second ? xr[j][1] : xr[j][c];
+        for (int c = 0; c < CT; ++c) {
+            uint32_t u[4];
+            if constexpr (PX == 1) {
 #pragma unroll
-            for (int q = 0; q < PX; ++q) {
-                uint32_t u[4];
+                for (int j = 0; j < 4; ++j)
+                    u[j] = __builtin_amdgcn_perm(xr[2 * j + 1][c / 2], xr[2 * j][c / 2], c % 2 ? 0x07060302u : 0x05040100u);
+                fb[c][0] = make_uint4(u[0], u[1], u[2], u[3]);
+            } else {
+                float v[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-                    v[2 * j] -= bf16_lo(u[j]);
-                    v[2 * j + 1] -= bf16_hi(u[j]);
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(xr[j][c]);
+#pragma unroll
+                for (int q = 0; q < PX; ++q) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        u[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                        v[2 * j] -= bf16_lo(u[j]);
+                        v[2 * j + 1] -= bf16_hi(u[j]);
+                    }
+                    fb[c][q] = make_uint4(u[0], u[1], u[2], u[3]);
                 }
-                fb[c][q] = make_uint4(u[0], u[1], u[2], u[3]);
             }
         }
     };
 
-    f32x4 acc[MT][2];
+    f32x4 acc[MT][CT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i][0] = acc[i][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     const int op = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
     fetch_a(kbeg, 0);
     fetch_x(kbeg);
@@ -902,9 +913,9 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             if (i + 1 < MT) operand(i + 1);
-            f32x4 part[2];
+            f32x4 part[CT];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) part[c] = PROD ? acc[i][c] : f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < CT; ++c) part[c] = PROD ? acc[i][c] : f32x4{0.f, 0.f, 0.f, 0.f};
             // smallest products first
 #pragma unroll
             for (int qx = PX - 1; qx >= 0; --qx)
@@ -912,24 +923,25 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
                 for (int qw = PW - 1; qw >= 0; --qw) {
                     if (qx + qw > 2) continue;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    for (int c = 0; c < CT; ++c)
                         part[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1][qw], __builtin_bit_cast(bf16x8, fb[c][qx]), part[c], 0, 0, 0);
                 }
             if constexpr (PROD) {
-                acc[i][0] = part[0];
-                acc[i][1] = part[1];
+#pragma unroll
+                for (int c = 0; c < CT; ++c) acc[i][c] = part[c];
             } else {
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+                for (int c = 0; c < CT; ++c)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][c][e] = fmaf(sc[i & 1][e], part[c][e], acc[i][c][e]);
                 // (here and now: put off to the step's end, the tiles' sums would fill the registers)
-                asm volatile("" : "+v"(acc[i][0]), "+v"(acc[i][1]));
+#pragma unroll
+                for (int c = 0; c < CT; ++c) asm volatile("" : "+v"(acc[i][c]));
             }
         }
         if (s + 1 < steps) split_x();
     }
-    const int n = n0 + 2 * (lane & 15);
+    const int n = n0 + CT * (lane & 15);
     if (n >= p.N) return;
     float* out = p.slab ? p.slab + (size_t)blockIdx.y * p.M * p.N : p.out;
     const int ldo = p.slab ? p.N : p.ldo;
@@ -940,8 +952,13 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
             const int m = m0 + 16 * i + 4 * (lane >> 4) + e;
             if (m >= p.M) continue;
             float* dst = out + (size_t)m * ldo + n;
-            if (n + 1 < p.N) *reinterpret_cast<f32x2_any*>(dst) = f32x2_any{acc[i][0][e], acc[i][1][e]};
-            else dst[0] = acc[i][0][e];
+            if (n + CT <= p.N) {
+                if constexpr (CT == 2) *reinterpret_cast<f32x2_any*>(dst) = f32x2_any{acc[i][0][e], acc[i][1][e]};
+                else *reinterpret_cast<f32x4_any*>(dst) = f32x4_any{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+            } else
+#pragma unroll
+                for (int c = 0; c < CT - 1; ++c)
+                    if (n + c < p.N) dst[c] = acc[i][c][e];
         }
 }
 
@@ -977,9 +994,9 @@ FewProduct product_few_plan(int d, int r, int b) {
     return q;
 }
 // Rows of a workgroup's tile (in sixteens) and pieces of the contraction for a product with many columns: the pair with
-// the least time by a model of what a step of 32 was measured to take with w workgroups a CU - 0.6 us until its loads
-// have come, for every set of workgroups that are resident together, and for every sixteen rows (and one for the
-// columns' split) 0.035 to 0.09 us of matrix and vector instructions - and of the pieces' way through memory at
+// the least time by a model of what a step of 32 was measured to take with w workgroups a CU - 0.45 to 0.6 us until its
+// loads have come, for every set of workgroups that are resident together, and for every sixteen rows (and one for the
+// columns' split) 0.05 to 0.09 us of matrix and vector instructions - and of the pieces' way through memory at
 // 4 TB/s.  (W^T X, d=6492 r=9202 b=73 float32: tiles of 32, 64, 128, 256 rows in one piece 237, 194, 236, 382 us, in
 // pieces for two workgroups a CU 142, 98, 91, 119.)
 struct ManyPlan { int mt, tiles_m, tiles_n, splits, per; size_t a_bytes, s_bytes, slab_bytes; };
@@ -988,19 +1005,20 @@ ManyPlan many_plan(bool prod, int d, int r, int b, int group, bool wide) {
     const int M = prod ? d : r;
     const int kp = prod ? (r + BK - 1) / BK * BK : (d + group - 1) / group * group;
     const int steps = ((prod ? r : d) + BK - 1) / BK;
-    q.tiles_n = (b + BN - 1) / BN;
+    const int cols = 64 * (wide ? COLUMN_TILES<float> : COLUMN_TILES<uint16_t>);
+    q.tiles_n = (b + cols - 1) / cols;
     double best = -1;
-    for (int mt = prod ? 8 : 16; mt >= 2; mt /= 2) {       // (the product's weights are two pieces)
-        const int tiles_m = (M + 16 * mt - 1) / (16 * mt), resident = mt == 16 ? 2 : mt == 8 ? 3 : 4;
+    for (int mt = prod || !wide ? 8 : 16; mt >= 2; mt /= 2) {       // (what LDS and the registers hold)
+        const int tiles_m = (M + 16 * mt - 1) / (16 * mt), resident = mt == 16 || (mt == 8 && !wide) ? 2 : mt == 8 || !wide ? 3 : 4;
         const double tiles = (double)tiles_m * q.tiles_n;
-        const double row = prod ? (wide ? 0.09 : 0.05) : (wide ? 0.07 : 0.035);
+        const double row = prod ? (wide ? 0.09 : 0.085) : (wide ? 0.07 : 0.05), own = wide ? 0.6 : 0.45;
         for (int target = 0; target <= 1024; target += 256) {
             const int want = (int)std::max(1.0, std::min(target / tiles, steps / 2.0));
             const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
             const double w = std::ceil(tiles * splits / 256);
             // (256 rows alone on the chip: 0.01 more; with other sets behind it the columns that it saves count as much)
             const double each = row + (mt == 16 && w <= 2 ? 0.01 : 0.0);
-            double cost = per * (0.6 * std::ceil(w / resident) + each * w * (mt + 1));
+            double cost = per * (own * std::ceil(w / resident) + each * w * (mt + 1));
             if (splits > 1) cost += 3.0 + 2e-6 * splits * M * b;
             if (best >= 0 && cost >= best) continue;
             best = cost;
@@ -1157,7 +1175,7 @@ int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, con
         if (near) hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, uint32_t>), grid, dim3(256), bytes, s, p);          \
         else hipLaunchKernelGGL((dict4_many_kernel<PROD, T, MT, uint64_t>), grid, dim3(256), bytes, s, p);               \
     }
-    if constexpr (!PROD) { MANY_CASE(16) }
+    if constexpr (!PROD && sizeof(T) == 4) { MANY_CASE(16) }
     MANY_CASE(8) MANY_CASE(4) MANY_CASE(2)
 #undef MANY_CASE
     HIP_TRY(c, hipGetLastError());

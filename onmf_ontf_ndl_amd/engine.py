@@ -574,7 +574,7 @@ class Engine:
                                  self._raw_stream())
         if rc:
             _lib.check(rc, self.ctx, "onmf_keep8")
-        return KeptColumns(codes, scales, n)
+        return KeptColumns._made(codes, scales, n)
 
     def keep8_expand(self, K, idx=None):
         """The float32 columns a store stands for: all (d x n), or those at ``idx`` (X[:, idx], src/onmf.py:214)."""

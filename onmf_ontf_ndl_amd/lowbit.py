@@ -76,6 +76,13 @@ class KeptColumns:
             raise ValueError("codes and scales must be contiguous")
         self.codes, self.scales, self.n = codes, scales, n
 
+    @classmethod
+    def _made(cls, codes, scales, n):
+        """What the engine has just made itself: nothing to check (1.5 us of a short call's 15)."""
+        K = object.__new__(cls)
+        K.codes, K.scales, K.n = codes, scales, n
+        return K
+
     @property
     def shape(self):
         return (self.codes.shape[0], self.n)

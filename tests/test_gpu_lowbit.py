@@ -89,7 +89,7 @@ SHAPES = [  # d, r, b, group: single columns, a few, many; ragged and whole; one
     (9000, 5, 8, 128), (1, 1, 9, 32), (33, 129, 9, 32), (441, 25, 17, 64), (100, 16, 130, 64), (128, 128, 128, 128),
     (257, 300, 33, 32), (1200, 100, 257, 64), (1024, 256, 300, 128), (130, 2000, 65, 64), (4096, 40, 100, 64),
     (8192, 20, 3, 64), (1100, 8200, 2, 32), (700, 9000, 31, 64), (2100, 4000, 64, 128), (3, 5000, 64, 32),
-    (60, 40, 1100, 32), (300, 70, 1501, 64), (200, 6001, 200, 32), (2100, 600, 601, 128), (33, 3, 1025, 32), (777, 1400, 1027, 64),
+    (60, 40, 1100, 32), (300, 70, 1501, 64), (200, 6001, 200, 32), (2100, 600, 601, 128), (33, 3, 1025, 32), (90, 33, 1030, 64), (777, 1400, 1027, 64),
 ]
 
 
