@@ -792,66 +792,36 @@ struct ManyParams {
     int tiles_m, tiles, k_per_split;
 };
 
-// a wave's columns in sixteens, as many as a lane loads at once: two float32 values or four bfloat16 ones
+// A wave's columns in sixteens, as many as a lane loads at once: two float32 values or four bfloat16 ones.
 template <typename T> constexpr int COLUMN_TILES = sizeof(T) == 4 ? 2 : 4;
+template <typename T> constexpr int COLUMN_PIECES = sizeof(T) == 4 ? 3 : 1;
 
-// OFF: 32 bits where 32 rows of X lie within them
-template <bool PROD, typename T, int MT, typename OFF>
-__global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
-    constexpr int PX = sizeof(T) == 4 ? 3 : 1;        // pieces of the float operand
-    constexpr int CT = COLUMN_TILES<T>;
-    constexpr int PW = PROD ? 2 : 1;                   // pieces of the weights
-    constexpr int ROWS = PW * 16 * MT, STAGE = ROWS * 64;
-    constexpr int SROWS = PROD ? 0 : (16 * MT + 63) / 64 * 64;
-    extern __shared__ __align__(16) char lds[];       // [2][STAGE], then float [2][SROWS]
-    float* lscale = (float*)(lds + 2 * STAGE);
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    // row tiles of the same columns follow each other on one XCD
-    const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
-    if (at >= p.tiles) return;
-    const int m0 = (at % p.tiles_m) * 16 * MT, n0 = (at / p.tiles_m) * 64 * CT + wave * 16 * CT;
-    const int kbeg = blockIdx.y * p.k_per_split, kend = min(p.K, kbeg + p.k_per_split);
-    const int steps = (kend - kbeg + BK - 1) / BK;
-    // Columns behind the last one are not stored.  A lane that has some reads the last CT columns, its own first among
-    // them at place `late`; rows behind the last one are the last one (the weights are zero there).
-    const int na = min(n0 + CT * (lane & 15), p.N - CT), late = min(n0 + CT * (lane & 15) - na, CT - 1);
-    const bool some_late = __any(late);
-    const int kl = 8 * (lane >> 4);
-
-    // 16 rows of weights a load: a base for the wave and 32 bits a lane
-    constexpr int LOADS = (ROWS / 16 + 3) / 4;
-    const char* base[LOADS];
-    uint32_t off[LOADS];
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-        const int row = (j * 4 + wave) * 16, piece = row / (16 * MT);
-        const int first = min(m0 + row - piece * 16 * MT, p.M - 1);
-        base[j] = (const char*)(p.A + ((size_t)piece * p.M + first) * p.kp);
-        off[j] = (uint32_t)(min(first + (lane >> 2), p.M - 1) - first) * (uint32_t)p.kp * 2 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16);
-    }
-    const uint32_t soff = PROD ? 0 : (uint32_t)min(m0 + t, p.M - 1) * 4;
-    auto fetch_a = [&](int k, int buf) {
-#pragma unroll
-        for (int j = 0; j < LOADS; ++j)
-            if (ROWS % 64 == 0 || (j * 4 + wave) * 16 < ROWS)
-                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base[j] + (size_t)k * 2 + off[j]),
-                                                 (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (j * 4 + wave) * 1024),
-                                                 16, 0, 0);
-        if constexpr (!PROD)
-            if (wave * 64 < 16 * MT)               // (by way of a register the wave would wait for it here)
-                __builtin_amdgcn_global_load_lds(
-                    (const __attribute__((address_space(1))) void*)((const char*)(p.S + (size_t)(k / p.group) * p.M) + soff),
-                    (__attribute__((address_space(3))) void*)(lscale + buf * SROWS + wave * 64), 4, 0, 0);
-    };
+// 32 rows of a wave's columns on their way to the matrix pipe.  OFF: 32 bits where 32 rows of X lie within them.
+template <typename T, typename OFF>
+struct Columns {
+    static constexpr int CT = COLUMN_TILES<T>, PX = COLUMN_PIECES<T>;
+    const char* X;
+    int N, K, ldx, kl, na, late;
+    bool some_late;
     u32x2_any xr[8];
-    auto fetch_x = [&](int k) {                       // (k < K: the rows are counted from k's)
+
+    __device__ __forceinline__ Columns(const void* X_, int N_, int K_, int ldx_, int lane)
+        : X((const char*)X_), N(N_), K(K_), ldx(ldx_), kl(8 * (lane >> 4)) {}
+    // Columns behind the last one are not stored.  A lane that has some reads the last CT columns, its own first among
+    // them at place `late`.
+    __device__ __forceinline__ void place(int n0, int lane) {
+        na = min(n0 + CT * (lane & 15), N - CT);
+        late = min(n0 + CT * (lane & 15) - na, CT - 1);
+        some_late = __any(late);
+    }
+    // rows k .. k + 31 (k < K); those behind the last one are the last one (the weights are zero there)
+    __device__ __forceinline__ void fetch(int k) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            xr[j] = *reinterpret_cast<const u32x2_any*>((const char*)p.X + (size_t)k * p.ldx * sizeof(T) +
-                                                        ((OFF)min(kl + j, p.K - 1 - k) * (OFF)p.ldx + (OFF)na) * (OFF)sizeof(T));
-    };
-    uint4 fb[CT][PX];
-    auto split_x = [&]() {
+            xr[j] = *reinterpret_cast<const u32x2_any*>(X + (size_t)k * ldx * sizeof(T) +
+                                                        ((OFF)min(kl + j, K - 1 - k) * (OFF)ldx + (OFF)na) * (OFF)sizeof(T));
+    }
+    __device__ __forceinline__ void split(uint4 (&fb)[CT][PX]) {
         if (some_late)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -883,83 +853,234 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
                 }
             }
         }
-    };
+    }
+};
 
-    f32x4 acc[MT][CT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+// A step of 32 of the contraction for 16 MT rows: the weights' operands at `a` (1024 bytes a piece and sixteen rows),
+// correlate's scales at `s`.
+template <bool PROD, int MT, int CT, int PX>
+__device__ __forceinline__ void row_tiles(const char* a, const float* s, int lane, const uint4 (&fb)[CT][PX], f32x4 (&acc)[MT][CT]) {
+    constexpr int PW = PROD ? 2 : 1;
     const int op = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
-    fetch_a(kbeg, 0);
-    fetch_x(kbeg);
-    split_x();
-    for (int s = 0; s < steps; ++s) {
-        const int buf = s & 1, k = kbeg + s * BK;
-        __syncthreads();                               // (this step's weights have come, the last step's are done with)
-        if (s + 1 < steps) {
-            fetch_a(k + BK, buf ^ 1);
-            fetch_x(k + BK);
-        }
-        // the next tile's weights and scales are read while this one's are used
-        bf16x8 fa[2][PW];
-        f32x4 sc[2];
-        auto operand = [&](int i) {
+    // the next tile's weights and scales are read while this one's are used
+    bf16x8 fa[2][PW];
+    f32x4 sc[2];
+    auto operand = [&](int i) {
 #pragma unroll
-            for (int q = 0; q < PW; ++q) fa[i & 1][q] = *reinterpret_cast<const bf16x8*>(lds + buf * STAGE + (q * MT + i) * 1024 + op);
-            if constexpr (!PROD) sc[i & 1] = *reinterpret_cast<const f32x4*>(lscale + buf * SROWS + 16 * i + 4 * (lane >> 4));
-        };
-        operand(0);
+        for (int q = 0; q < PW; ++q) fa[i & 1][q] = *reinterpret_cast<const bf16x8*>(a + (q * MT + i) * 1024 + op);
+        if constexpr (!PROD) sc[i & 1] = *reinterpret_cast<const f32x4*>(s + 16 * i + 4 * (lane >> 4));
+    };
+    operand(0);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            if (i + 1 < MT) operand(i + 1);
-            f32x4 part[CT];
+    for (int i = 0; i < MT; ++i) {
+        if (i + 1 < MT) operand(i + 1);
+        f32x4 part[CT];
 #pragma unroll
-            for (int c = 0; c < CT; ++c) part[c] = PROD ? acc[i][c] : f32x4{0.f, 0.f, 0.f, 0.f};
-            // smallest products first
+        for (int c = 0; c < CT; ++c) part[c] = PROD ? acc[i][c] : f32x4{0.f, 0.f, 0.f, 0.f};
+        // smallest products first
 #pragma unroll
-            for (int qx = PX - 1; qx >= 0; --qx)
+        for (int qx = PX - 1; qx >= 0; --qx)
 #pragma unroll
-                for (int qw = PW - 1; qw >= 0; --qw) {
-                    if (qx + qw > 2) continue;
-#pragma unroll
-                    for (int c = 0; c < CT; ++c)
-                        part[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1][qw], __builtin_bit_cast(bf16x8, fb[c][qx]), part[c], 0, 0, 0);
-                }
-            if constexpr (PROD) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c) acc[i][c] = part[c];
-            } else {
+            for (int qw = PW - 1; qw >= 0; --qw) {
+                if (qx + qw > 2) continue;
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][c][e] = fmaf(sc[i & 1][e], part[c][e], acc[i][c][e]);
-                // (here and now: put off to the step's end, the tiles' sums would fill the registers)
-#pragma unroll
-                for (int c = 0; c < CT; ++c) asm volatile("" : "+v"(acc[i][c]));
+                    part[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1][qw], __builtin_bit_cast(bf16x8, fb[c][qx]), part[c], 0, 0, 0);
             }
+        if constexpr (PROD) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[i][c] = part[c];
+        } else {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][c][e] = fmaf(sc[i & 1][e], part[c][e], acc[i][c][e]);
+            // (here and now: put off to the step's end, the tiles' sums would fill the registers)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) asm volatile("" : "+v"(acc[i][c]));
         }
-        if (s + 1 < steps) split_x();
     }
+}
+
+template <int MT, int CT>
+__device__ __forceinline__ void store_tiles(float* out, int ldo, int M, int N, int m0, int n0, int lane, const f32x4 (&acc)[MT][CT]) {
     const int n = n0 + CT * (lane & 15);
-    if (n >= p.N) return;
-    float* out = p.slab ? p.slab + (size_t)blockIdx.y * p.M * p.N : p.out;
-    const int ldo = p.slab ? p.N : p.ldo;
+    if (n >= N) return;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int m = m0 + 16 * i + 4 * (lane >> 4) + e;
-            if (m >= p.M) continue;
+            if (m >= M) continue;
             float* dst = out + (size_t)m * ldo + n;
-            if (n + CT <= p.N) {
+            if (n + CT <= N) {
                 if constexpr (CT == 2) *reinterpret_cast<f32x2_any*>(dst) = f32x2_any{acc[i][0][e], acc[i][1][e]};
                 else *reinterpret_cast<f32x4_any*>(dst) = f32x4_any{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
             } else
 #pragma unroll
                 for (int c = 0; c < CT - 1; ++c)
-                    if (n + c < p.N) dst[c] = acc[i][c][e];
+                    if (n + c < N) dst[c] = acc[i][c][e];
         }
+}
+
+template <bool PROD, typename T, int MT, typename OFF>
+__global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
+    constexpr int PX = COLUMN_PIECES<T>, CT = COLUMN_TILES<T>;
+    constexpr int PW = PROD ? 2 : 1;                   // pieces of the weights
+    constexpr int ROWS = PW * 16 * MT, STAGE = ROWS * 64;
+    constexpr int SROWS = PROD ? 0 : (16 * MT + 63) / 64 * 64;
+    extern __shared__ __align__(16) char lds[];       // [2][STAGE], then float [2][SROWS]
+    float* lscale = (float*)(lds + 2 * STAGE);
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // row tiles of the same columns follow each other on one XCD
+    const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= p.tiles) return;
+    const int m0 = (at % p.tiles_m) * 16 * MT, n0 = (at / p.tiles_m) * 64 * CT + wave * 16 * CT;
+    const int kbeg = blockIdx.y * p.k_per_split, kend = min(p.K, kbeg + p.k_per_split);
+    const int steps = (kend - kbeg + BK - 1) / BK;
+
+    // 16 rows of weights a load: a base for the wave and 32 bits a lane (rows behind the last one are the last one)
+    constexpr int LOADS = (ROWS / 16 + 3) / 4;
+    const char* base[LOADS];
+    uint32_t off[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const int row = (j * 4 + wave) * 16, piece = row / (16 * MT);
+        const int first = min(m0 + row - piece * 16 * MT, p.M - 1);
+        base[j] = (const char*)(p.A + ((size_t)piece * p.M + first) * p.kp);
+        off[j] = (uint32_t)(min(first + (lane >> 2), p.M - 1) - first) * (uint32_t)p.kp * 2 + (((lane & 3) ^ ((lane >> 4) & 3)) * 16);
+    }
+    const uint32_t soff = PROD ? 0 : (uint32_t)min(m0 + t, p.M - 1) * 4;
+    auto fetch_a = [&](int k, int buf) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            if (ROWS % 64 == 0 || (j * 4 + wave) * 16 < ROWS)
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base[j] + (size_t)k * 2 + off[j]),
+                                                 (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (j * 4 + wave) * 1024),
+                                                 16, 0, 0);
+        if constexpr (!PROD)
+            if (wave * 64 < 16 * MT)               // (by way of a register the wave would wait for it here)
+                __builtin_amdgcn_global_load_lds(
+                    (const __attribute__((address_space(1))) void*)((const char*)(p.S + (size_t)(k / p.group) * p.M) + soff),
+                    (__attribute__((address_space(3))) void*)(lscale + buf * SROWS + wave * 64), 4, 0, 0);
+    };
+    Columns<T, OFF> x(p.X, p.N, p.K, p.ldx, lane);
+    uint4 fb[CT][PX];
+    f32x4 acc[MT][CT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    x.place(n0, lane);
+    fetch_a(kbeg, 0);
+    x.fetch(kbeg);
+    x.split(fb);
+    for (int s = 0; s < steps; ++s) {
+        const int buf = s & 1, k = kbeg + s * BK;
+        __syncthreads();                               // (this step's weights have come, the last step's are done with)
+        if (s + 1 < steps) {
+            fetch_a(k + BK, buf ^ 1);
+            x.fetch(k + BK);
+        }
+        row_tiles<PROD, MT>(lds + buf * STAGE, lscale + buf * SROWS, lane, fb, acc);
+        if (s + 1 < steps) x.split(fb);
+    }
+    if (p.slab) store_tiles(p.slab + (size_t)blockIdx.y * p.M * p.N, p.N, p.M, p.N, m0, n0, lane, acc);
+    else store_tiles(p.out, p.ldo, p.M, p.N, m0, n0, lane, acc);
+}
+
+// The same for a contraction so short that a workgroup keeps all its rows' weights in LDS: it unpacks them there itself, and
+// its four waves take one set of columns after the other past them, each at its own pace, the next step's columns on
+// their way.  One launch, no workspace.
+struct ResidentParams {
+    const uint32_t *codes, *scales;
+    const void* X;
+    float* out;
+    int M, N, K, d, r;
+    int ldx, ldo, group, groups;
+    int tiles_m, parts;
+};
+template <bool PROD, typename T, int MT, typename OFF>
+__global__ __launch_bounds__(256, 2) void dict4_resident_kernel(ResidentParams p) {
+    constexpr int PX = COLUMN_PIECES<T>, CT = COLUMN_TILES<T>, PW = PROD ? 2 : 1, ROWS = 16 * MT, STAGE = PW * ROWS * 64;
+    extern __shared__ __align__(16) char lds[];       // [step][piece][row][32 values], then float [group][row]
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    // row tiles of the same columns follow each other on one XCD
+    const int at = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= p.tiles_m * p.parts) return;
+    const int m0 = at % p.tiles_m * ROWS, part = at / p.tiles_m;
+    const int steps = (p.K + BK - 1) / BK, words = p.groups * (p.group / 8);
+    float* lscale = (float*)(lds + steps * STAGE);
+    // a value's place: chunks of 8 are permuted by the row, as above
+    auto cell = [&](int piece, int row, int k) {
+        return lds + (k / BK) * STAGE + (piece * ROWS + row) * 64 + ((((k & 31) >> 3) ^ ((row >> 2) & 3)) * 16) + (k & 7) * 2;
+    };
+    if constexpr (PROD) {
+        // words of four atoms: eight rows, turned round
+        for (int e = t; e < steps * 8 * 2 * MT; e += 256) {
+            const int w = m0 / 8 + e % (2 * MT), k = e / (2 * MT) * 4;
+            float v[4][8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool there = k + j < p.r && w < words;
+                const uint32_t sc = there ? p.scales[(size_t)(k + j) * p.groups + w * 8 / p.group] : 0;
+                word_entries(there ? p.codes[(size_t)(k + j) * words + w] : 0, v[j]);
+#pragma unroll
+                for (int f = 0; f < 8; ++f) v[j][f] = word_scale(sc) * (v[j][f] + word_offset(sc));
+            }
+#pragma unroll
+            for (int f = 0; f < 8; ++f) {
+                const uint32_t a = pack_bf16(v[0][f], v[1][f]), b = pack_bf16(v[2][f], v[3][f]);
+                const int row = e % (2 * MT) * 8 + f;
+                *reinterpret_cast<uint2*>(cell(0, row, k)) = make_uint2(a, b);
+                *reinterpret_cast<uint2*>(cell(1, row, k)) = make_uint2(pack_bf16(v[0][f] - bf16_lo(a), v[1][f] - bf16_hi(a)),
+                                                                         pack_bf16(v[2][f] - bf16_lo(b), v[3][f] - bf16_hi(b)));
+            }
+        }
+    } else {
+        for (int e = t; e < ROWS * steps * 4; e += 256) {
+            const int row = e / (steps * 4), w = e % (steps * 4), k = m0 + row;
+            uint32_t u[4] = {0, 0, 0, 0};
+            if (k < p.r) {
+                const uint32_t sc = p.scales[(size_t)k * p.groups + w * 8 / p.group];
+                const float z = word_offset(sc);
+                float q[8];
+                word_entries(p.codes[(size_t)k * words + w], q);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) q[j] = w * 8 + j < p.d ? q[j] + z : 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = pack_bf16(q[2 * j], q[2 * j + 1]);
+                if (w * 8 % p.group == 0) lscale[w * 8 / p.group * ROWS + row] = word_scale(sc);
+            }
+            *reinterpret_cast<uint4*>(cell(0, row, w * 8)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+    }
+    __syncthreads();
+    const int sets = (p.N + 16 * CT - 1) / (16 * CT), stride = p.parts * 4;
+    int set = part * 4 + wave;
+    if (set >= sets) return;
+    Columns<T, OFF> x(p.X, p.N, p.K, p.ldx, lane);
+    x.place(set * 16 * CT, lane);
+    x.fetch(0);
+    for (; set < sets; set += stride) {
+        f32x4 acc[MT][CT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < steps; ++s) {
+            uint4 fb[CT][PX];
+            x.split(fb);
+            if (s + 1 < steps) {
+                x.fetch((s + 1) * BK);
+            } else if (set + stride < sets) {
+                x.place((set + stride) * 16 * CT, lane);
+                x.fetch(0);
+            }
+            row_tiles<PROD, MT>(lds + s * STAGE, lscale + s * BK / p.group * ROWS, lane, fb, acc);
+        }
+        store_tiles(p.out, p.ldo, p.M, p.N, m0, set * 16 * CT, lane, acc);
+    }
 }
 
 // ------------------------------------------------------------------------------------------- launches
@@ -970,6 +1091,7 @@ constexpr int FEW = 1, FEW_PRODUCT = 2;     // columns up to which the vector ke
 // and 1270, d=1024 r=1024 b=512 18.6 and 27.6; W^T X, float32, d=8192 r=16384 b=128 173 and 222, b=256 420 and
 // 314, d=4096 r=256 b=384 16.6 and 21.4, bfloat16, d=8192 r=16384 b=512 413 and 461).
 constexpr int TILE_PRODUCT = 1024;
+constexpr size_t RESIDENT_BYTES = 150 * 1024;
 int most_tile_columns(int d, int r, bool wide) { return !wide || (long long)d * r <= 1 << 20 ? 512 : 192; }     // (the correlate's)
 
 struct FewPlan { int nb, ch; };
@@ -999,7 +1121,7 @@ FewProduct product_few_plan(int d, int r, int b) {
 // columns' split) 0.05 to 0.09 us of matrix and vector instructions - and of the pieces' way through memory at
 // 4 TB/s.  (W^T X, d=6492 r=9202 b=73 float32: tiles of 32, 64, 128, 256 rows in one piece 237, 194, 236, 382 us, in
 // pieces for two workgroups a CU 142, 98, 91, 119.)
-struct ManyPlan { int mt, tiles_m, tiles_n, splits, per; size_t a_bytes, s_bytes, slab_bytes; };
+struct ManyPlan { int mt, tiles_m, tiles_n, splits, per; size_t a_bytes, s_bytes, slab_bytes; double cost; };
 ManyPlan many_plan(bool prod, int d, int r, int b, int group, bool wide) {
     ManyPlan q;
     const int M = prod ? d : r;
@@ -1021,7 +1143,7 @@ ManyPlan many_plan(bool prod, int d, int r, int b, int group, bool wide) {
             double cost = per * (own * std::ceil(w / resident) + each * w * (mt + 1));
             if (splits > 1) cost += 3.0 + 2e-6 * splits * M * b;
             if (best >= 0 && cost >= best) continue;
-            best = cost;
+            best = q.cost = cost;
             q.mt = mt;
             q.tiles_m = tiles_m;
             q.per = per;
@@ -1148,9 +1270,8 @@ int correlate_tile(onmf_ctx* c, const RangePlan& q, int d, int r, int b, int gro
 }
 
 template <bool PROD, typename T>
-int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
+int many(onmf_ctx* c, const ManyPlan& q, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
          float* out, int ldo, char* ws, hipStream_t s) {
-    const ManyPlan q = many_plan(PROD, d, r, b, group, sizeof(T) == 4);
     const int groups = (d + group - 1) / group, words = groups * (group / 8);
     ManyParams p;
     p.A = (const uint16_t*)ws;
@@ -1183,6 +1304,59 @@ int many(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, con
     return ONMF_OK;
 }
 
+// Rows of a resident workgroup's tile, or none where the two launches of the many columns' kernel take less by their model
+// (with 6.5 us for the first of them and its latency, the weights' way at 4 TB/s and the result's at 8).  A step takes
+// a wave `own` and `row` for every sixteen rows, half as long again with two workgroups a CU; before that come the
+// launch and the unpacking.  (us, resident and many: W H float32 d=1200 r=100 b=8192 22 and 25.5, d=1024 r=256
+// b=2000 13.3 and 18.4, b=60000 170 and 153; bfloat16 d=441 r=100 b=5001 8.7 and 13.6; W^T X bfloat16 d=441 r=100
+// b=16384 12.4 and 16.6, float32 d=1024 r=256 b=520 24 and 16.)
+struct ResidentPlan { int mt, tiles_m, parts; size_t bytes; };
+ResidentPlan resident_plan(const ManyPlan& many, bool prod, int d, int r, int b, int group, bool wide) {
+    ResidentPlan q;
+    q.mt = 0;
+    const int M = prod ? d : r, K = prod ? r : d, steps = (K + BK - 1) / BK, cols = 16 * (wide ? COLUMN_TILES<float> : COLUMN_TILES<uint16_t>);
+    const int sets = (b + cols - 1) / cols;
+    const double own = wide ? (prod ? 0.5 : 0.35) : 0.26, row = prod && !wide ? 0.16 : 0.145;
+    double best = many.cost + 6.5 + (prod ? 4.5 : 2.5) * d * r / 4e6 + 4.0 * M * b / 8e6;
+    for (int mt = wide ? 8 : 4; mt >= 2; mt /= 2) {            // (what the registers hold)
+        const size_t bytes = (size_t)steps * (prod ? 2 : 1) * 16 * mt * 64 + (prod ? 0 : sizeof(float) * ((steps * BK + group - 1) / group) * 16 * mt);
+        if (bytes > RESIDENT_BYTES) continue;
+        const int tiles_m = (M + 16 * mt - 1) / (16 * mt), resident = bytes > RESIDENT_BYTES / 2 ? 1 : 2;
+        const double waves = (double)sets * tiles_m, step = (own + row * mt) * (waves > 1024 && resident == 2 ? 1.5 : 1.0);
+        const double cost = 3.5 + bytes / 40e3 + std::ceil(waves / (1024 * resident)) * steps * step;
+        if (cost >= best) continue;
+        best = cost;
+        q.mt = mt;
+        q.bytes = bytes;
+        q.tiles_m = tiles_m;
+        q.parts = std::min((sets + 3) / 4, std::max(1, 256 * resident / tiles_m));
+    }
+    return q;
+}
+template <bool PROD, typename T>
+int resident(onmf_ctx* c, const ResidentPlan& q, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales,
+             const T* X, int ldx, float* out, int ldo, hipStream_t s) {
+    ResidentParams p;
+    p.codes = codes; p.scales = scales; p.X = X; p.out = out; p.ldx = ldx; p.ldo = ldo; p.group = group;
+    p.groups = (d + group - 1) / group; p.d = d; p.r = r;
+    p.M = PROD ? d : r; p.N = b; p.K = PROD ? r : d; p.tiles_m = q.tiles_m; p.parts = q.parts;
+    const dim3 grid((q.tiles_m * q.parts + 7) / 8 * 8);
+    const bool near = ((size_t)BK * ldx + b) * sizeof(T) < ((size_t)1 << 32);
+#define RESIDENT_CASE(MT, OFF)                                                                                           \
+    {                                                                                                                    \
+        static LdsLimit lim;                                                                                             \
+        ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_resident_kernel<PROD, T, MT, OFF>, q.bytes));            \
+        hipLaunchKernelGGL((dict4_resident_kernel<PROD, T, MT, OFF>), grid, dim3(256), q.bytes, s, p);                     \
+    }
+#define RESIDENT_CASES(MT) if (q.mt == MT) { if (near) RESIDENT_CASE(MT, uint32_t) else RESIDENT_CASE(MT, uint64_t) }
+    if constexpr (sizeof(T) == 4) { RESIDENT_CASES(8) }
+    RESIDENT_CASES(4) RESIDENT_CASES(2)
+#undef RESIDENT_CASES
+#undef RESIDENT_CASE
+    HIP_TRY(c, hipGetLastError());
+    return ONMF_OK;
+}
+
 int check4(onmf_ctx* c, const char* what, int d, int r, int group, const void* codes, const void* scales) {
     if (d <= 0 || r <= 0 || !codes || !scales || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
         return onmf_fail(c, ONMF_ERR_ARG, "%s: bad arguments (d=%d r=%d; codes must be aligned to 16 bytes)", what, d, r);
@@ -1202,7 +1376,7 @@ size_t workspace_of(bool prod, int d, int r, int b, int group, bool wide) {
         splits = q.one ? 1 : q.splits;
     } else {
         const ManyPlan q = many_plan(prod, d, r, b, group, wide);
-        return q.a_bytes + q.s_bytes + q.slab_bytes;
+        if (!resident_plan(q, prod, d, r, b, group, wide).mt) return q.a_bytes + q.s_bytes + q.slab_bytes;
     }
     return splits > 1 ? (size_t)splits * (prod ? d : r) * b * sizeof(float) : 0;
 }
@@ -1226,7 +1400,10 @@ int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* cod
         if (q.nt == 2) return correlate_tile<2, T>(c, q, d, r, b, group, codes, scales, X, ldx, C, ws, s);
         return correlate_tile<4, T>(c, q, d, r, b, group, codes, scales, X, ldx, C, ws, s);
     }
-    return many<false, T>(c, d, r, b, group, codes, scales, X, ldx, C, b, (char*)ws, s);
+    const ManyPlan m = many_plan(false, d, r, b, group, sizeof(T) == 4);
+    const ResidentPlan q = resident_plan(m, false, d, r, b, group, sizeof(T) == 4);
+    if (q.mt) return resident<false, T>(c, q, d, r, b, group, codes, scales, X, ldx, C, b, s);
+    return many<false, T>(c, m, d, r, b, group, codes, scales, X, ldx, C, b, (char*)ws, s);
 }
 
 template <typename T>
@@ -1246,7 +1423,10 @@ int product_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes
         if (q.nt == 1) return product_tile<1, 2, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
         return product_tile<2, 1, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
     }
-    return many<true, T>(c, d, r, b, group, codes, scales, H, ldh, R, ldr, (char*)ws, s);
+    const ManyPlan m = many_plan(true, d, r, b, group, sizeof(T) == 4);
+    const ResidentPlan q = resident_plan(m, true, d, r, b, group, sizeof(T) == 4);
+    if (q.mt) return resident<true, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, s);
+    return many<true, T>(c, m, d, r, b, group, codes, scales, H, ldh, R, ldr, (char*)ws, s);
 }
 
 }  // namespace
@@ -1291,7 +1471,7 @@ int onmf_dict4_correlate(onmf_ctx* c, int d, int r, int b, int group, const void
     ONMF_TRY(check4(c, "dict4_correlate", d, r, group, codes, scales));
     if (b <= 0 || b > MOST_COLS || !X || !C || ldx < b || (x_type != ONMF_TYPE_F32 && x_type != ONMF_TYPE_BF16))
         return onmf_fail(c, ONMF_ERR_ARG, "dict4_correlate: bad arguments (b=%d ldx=%d type=%d)", b, ldx, x_type);
-    const size_t need = onmf_dict4_workspace(ONMF_DICT4_CORRELATE, d, r, b, group);
+    const size_t need = workspace_of(false, d, r, b, group, x_type == T_F32);
     if (ws_bytes < need || (need && !ws))
         return onmf_fail(c, ONMF_ERR_ARG, "dict4_correlate: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
@@ -1307,7 +1487,7 @@ int onmf_dict4_product(onmf_ctx* c, int d, int r, int b, int group, const void* 
     ONMF_TRY(check4(c, "dict4_product", d, r, group, codes, scales));
     if (b <= 0 || b > MOST_COLS || !H || !R || ldh < b || ldr < b || (h_type != ONMF_TYPE_F32 && h_type != ONMF_TYPE_BF16))
         return onmf_fail(c, ONMF_ERR_ARG, "dict4_product: bad arguments (b=%d ldh=%d ldr=%d type=%d)", b, ldh, ldr, h_type);
-    const size_t need = onmf_dict4_workspace(ONMF_DICT4_PRODUCT, d, r, b, group);
+    const size_t need = workspace_of(true, d, r, b, group, h_type == T_F32);
     if (ws_bytes < need || (need && !ws))
         return onmf_fail(c, ONMF_ERR_ARG, "dict4_product: workspace of %zu bytes, %zu needed", ws_bytes, need);
     ONMF_ENTER(c);
