@@ -1305,7 +1305,7 @@ int many(onmf_ctx* c, const ManyPlan& q, int d, int r, int b, int group, const u
 }
 
 // Rows of a resident workgroup's tile, or none where the two launches of the many columns' kernel take less by their model
-// (with 6.5 us for the first of them and its latency, the weights' way at 4 TB/s and the result's at 8).  A step takes
+// (with 8 us for the first of them and its latency, the weights' way at 4 TB/s and the result's at 8).  A step takes
 // a wave `own` and `row` for every sixteen rows, half as long again with two workgroups a CU; before that come the
 // launch and the unpacking.  (us, resident and many: W H float32 d=1200 r=100 b=8192 22 and 25.5, d=1024 r=256
 // b=2000 13.3 and 18.4, b=60000 170 and 153; bfloat16 d=441 r=100 b=5001 8.7 and 13.6; W^T X bfloat16 d=441 r=100
@@ -1317,7 +1317,7 @@ ResidentPlan resident_plan(const ManyPlan& many, bool prod, int d, int r, int b,
     const int M = prod ? d : r, K = prod ? r : d, steps = (K + BK - 1) / BK, cols = 16 * (wide ? COLUMN_TILES<float> : COLUMN_TILES<uint16_t>);
     const int sets = (b + cols - 1) / cols;
     const double own = wide ? (prod ? 0.5 : 0.35) : 0.26, row = prod && !wide ? 0.16 : 0.145;
-    double best = many.cost + 6.5 + (prod ? 4.5 : 2.5) * d * r / 4e6 + 4.0 * M * b / 8e6;
+    double best = many.cost + 8.0 + (prod ? 4.5 : 2.5) * d * r / 4e6 + 4.0 * M * b / 8e6;
     for (int mt = wide ? 8 : 4; mt >= 2; mt /= 2) {            // (what the registers hold)
         const size_t bytes = (size_t)steps * (prod ? 2 : 1) * 16 * mt * 64 + (prod ? 0 : sizeof(float) * ((steps * BK + group - 1) / group) * 16 * mt);
         if (bytes > RESIDENT_BYTES) continue;
