@@ -357,8 +357,9 @@ int onmf_numpy_rand(onmf_ctx* ctx, const uint32_t* key, int pos, size_t n, float
  * Each is the other's gradient: dL/dX = W dL/dC, dL/dH = W^T dL/dR.
  * A column with a NaN or an infinity (or a float32 within 2^-8 of the largest one) has NaNs or infinities in its
  * result and touches no other column.  ws: at least onmf_dict4_workspace(which, d, r, b, group) bytes of device
- * memory, in use until the call's work on `stream` is done (so calls on different streams take different ones).
- * d <= 2^18.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
+ * memory, aligned to 16, in use until the call's work on `stream` is done (so calls on different streams take
+ * different ones).  d <= 2^18; results may not overlap what is read.  Asynchronous on `stream`, allocates nothing and
+ * can be captured into a graph.
  */
 #define ONMF_TYPE_F32 0
 #define ONMF_TYPE_BF16 1
@@ -394,8 +395,9 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  *                       dW may not overlap W.  Up to 128 columns are taken as (W H - X) H^T where that is less work
  * Products inside a group add up exactly in int32, groups in float32, runs of groups and what follows in double
  * (the residual's products in double throughout).
- * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, in use until the call's work on
- * `stream` is done.  n <= 2^28.  Asynchronous on `stream`, allocates nothing and can be captured into a graph.
+ * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, aligned to 16, in use until the call's
+ * work on `stream` is done.  n <= 2^28, at most 2^29 - 32 groups in a store.  Asynchronous on `stream`, allocates
+ * nothing and can be captured into a graph.
  */
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient);
 int onmf_keep8(onmf_ctx* ctx, int d, int n, const void* X, int x_type, int ldx, int8_t* codes, float* scales, void* stream);

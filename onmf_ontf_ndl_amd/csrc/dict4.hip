@@ -1364,7 +1364,8 @@ int check4(onmf_ctx* c, const char* what, int d, int r, int group, const void* c
         return onmf_fail(c, ONMF_ERR_ARG, "%s: bad arguments (d=%d r=%d; codes must be aligned to 16 bytes)", what, d, r);
     if (group != 32 && group != 64 && group != 128)
         return onmf_fail(c, ONMF_ERR_ARG, "%s: a group is 32, 64 or 128 features, not %d", what, group);
-    if (d > (1 << 18)) return onmf_fail(c, ONMF_ERR_ARG, "%s: d=%d is more than 2^18 features", what, d);
+    if (d > (1 << 18) || r > MOST_COLS)
+        return onmf_fail(c, ONMF_ERR_ARG, "%s: d=%d is more than 2^18 features, or r=%d more atoms than an int counts", what, d, r);
     return ONMF_OK;
 }
 
@@ -1475,8 +1476,8 @@ int onmf_dict4_correlate(onmf_ctx* c, int d, int r, int b, int group, const void
     if (b <= 0 || b > MOST_COLS || !X || !C || ldx < b || (x_type != ONMF_TYPE_F32 && x_type != ONMF_TYPE_BF16))
         return onmf_fail(c, ONMF_ERR_ARG, "dict4_correlate: bad arguments (b=%d ldx=%d type=%d)", b, ldx, x_type);
     const size_t need = workspace_of(false, d, r, b, group, x_type == T_F32);
-    if (ws_bytes < need || (need && !ws))
-        return onmf_fail(c, ONMF_ERR_ARG, "dict4_correlate: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    if (ws_bytes < need || (need && !ws) || ((uintptr_t)ws & 15))
+        return onmf_fail(c, ONMF_ERR_ARG, "dict4_correlate: workspace of %zu bytes, %zu needed, aligned to 16", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const uint32_t *cw = (const uint32_t*)codes, *sc = (const uint32_t*)scales;
@@ -1491,8 +1492,8 @@ int onmf_dict4_product(onmf_ctx* c, int d, int r, int b, int group, const void* 
     if (b <= 0 || b > MOST_COLS || !H || !R || ldh < b || ldr < b || (h_type != ONMF_TYPE_F32 && h_type != ONMF_TYPE_BF16))
         return onmf_fail(c, ONMF_ERR_ARG, "dict4_product: bad arguments (b=%d ldh=%d ldr=%d type=%d)", b, ldh, ldr, h_type);
     const size_t need = workspace_of(true, d, r, b, group, h_type == T_F32);
-    if (ws_bytes < need || (need && !ws))
-        return onmf_fail(c, ONMF_ERR_ARG, "dict4_product: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    if (ws_bytes < need || (need && !ws) || ((uintptr_t)ws & 15))
+        return onmf_fail(c, ONMF_ERR_ARG, "dict4_product: workspace of %zu bytes, %zu needed, aligned to 16", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const uint32_t *cw = (const uint32_t*)codes, *sc = (const uint32_t*)scales;

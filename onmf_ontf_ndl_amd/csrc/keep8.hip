@@ -18,7 +18,7 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 namespace {
 
 constexpr int GROUP = 128;
-constexpr size_t MOST_GROUPS = (size_t)1 << 33;
+constexpr size_t MOST_GROUPS = ((size_t)1 << 29) - 32;      // eight threads a group, fewer than 2^32 in a launch
 constexpr int MOST_COLS = 1 << 28;       // eight rows' codes lie within 32 bits
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
@@ -46,22 +46,21 @@ __device__ __forceinline__ uint32_t max16(uint32_t v) {
 }
 
 // row and group of the first of the groups a thread handles, moved on one at a time (one division a thread)
-template <typename I>
 struct GroupAt {
-    I row, g, groups;
-    __device__ __forceinline__ GroupAt(I at, I n) : row(at / n), g(at % n), groups(n) {}
+    uint32_t row, g, groups;
+    __device__ __forceinline__ GroupAt(uint32_t at, uint32_t n) : row(at / n), g(at % n), groups(n) {}
     __device__ __forceinline__ void next() { if (++g == groups) { g = 0; ++row; } }
 };
 
 // 16 lanes per group, eight columns a lane, U groups a lane (their loads are on their way together).  Bound by
 // memory: 5 bytes a float32 entry, 3 a bfloat16 one.
-template <typename T, typename I, int U>
+template <typename T, int U>
 __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int groups, const T* __restrict__ X, int ldx,
                                                      int8_t* __restrict__ codes, float* __restrict__ scales) {
     const int lane = threadIdx.x & 15;
     const size_t first = ((size_t)blockIdx.x * 16 + (threadIdx.x >> 4)) * U;
     if (first >= all) return;
-    GroupAt<I> at((I)first, (I)groups);
+    GroupAt at((uint32_t)first, (uint32_t)groups);
     float v[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u, at.next()) {
@@ -131,7 +130,7 @@ __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int group
 }
 
 // ------------------------------------------------------------------------------------------- bring back
-template <typename I, int U>
+template <int U>
 __global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, int groups, const int8_t* __restrict__ codes,
                                                             const float* __restrict__ scales, float* __restrict__ X,
                                                             int ldx) {
@@ -146,7 +145,7 @@ __global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, in
         w[u] = *reinterpret_cast<const uint32_t*>(codes + at * GROUP + lane * 4);
         s[u] = scales[at];
     }
-    GroupAt<I> at((I)first, (I)groups);
+    GroupAt at((uint32_t)first, (uint32_t)groups);
 #pragma unroll
     for (int u = 0; u < U; ++u, at.next()) {
         if (first + u >= all) break;
@@ -738,31 +737,23 @@ int launch_residual(onmf_ctx* c, int d, int r, const float* W, const int8_t* xc,
     return ONMF_OK;
 }
 
-// Groups a thread handles: several where there are enough of them to fill the chip with.  32-bit group numbers where
-// they do (a division in 64 bits costs as much as everything else).
-template <typename T, typename I>
-void launch_keep_as(size_t all, int n, int groups, const T* X, int ldx, int8_t* codes, float* scales, hipStream_t s) {
-    if (all >= 65536)
-        hipLaunchKernelGGL((keep8_kernel<T, I, 2>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, X, ldx,
-                           codes, scales);
-    else
-        hipLaunchKernelGGL((keep8_kernel<T, I, 1>), dim3((unsigned)((all + 15) / 16)), dim3(256), 0, s, all, n, groups, X, ldx,
-                           codes, scales);
-}
+// Groups a thread handles: several where there are enough of them to fill the chip with.
 template <typename T>
 void launch_keep(size_t all, int n, int groups, const T* X, int ldx, int8_t* codes, float* scales, hipStream_t s) {
-    if (all < 0x7fffffffu) launch_keep_as<T, uint32_t>(all, n, groups, X, ldx, codes, scales, s);
-    else launch_keep_as<T, uint64_t>(all, n, groups, X, ldx, codes, scales, s);
-}
-template <typename I>
-void launch_expand(size_t all, int n, int groups, const int8_t* codes, const float* scales, float* X, int ldx,
-                   hipStream_t s) {
     if (all >= 65536)
-        hipLaunchKernelGGL((keep8_expand_kernel<I, 4>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, codes,
-                           scales, X, ldx);
+        hipLaunchKernelGGL((keep8_kernel<T, 2>), dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, X, ldx, codes,
+                           scales);
     else
-        hipLaunchKernelGGL((keep8_expand_kernel<I, 1>), dim3((unsigned)((all + 7) / 8)), dim3(256), 0, s, all, n, groups, codes,
-                           scales, X, ldx);
+        hipLaunchKernelGGL((keep8_kernel<T, 1>), dim3((unsigned)((all + 15) / 16)), dim3(256), 0, s, all, n, groups, X, ldx, codes,
+                           scales);
+}
+void launch_expand(size_t all, int n, int groups, const int8_t* codes, const float* scales, float* X, int ldx, hipStream_t s) {
+    if (all >= 65536)
+        hipLaunchKernelGGL(keep8_expand_kernel<4>, dim3((unsigned)((all + 31) / 32)), dim3(256), 0, s, all, n, groups, codes, scales,
+                           X, ldx);
+    else
+        hipLaunchKernelGGL(keep8_expand_kernel<1>, dim3((unsigned)((all + 7) / 8)), dim3(256), 0, s, all, n, groups, codes, scales, X,
+                           ldx);
 }
 
 }  // namespace
@@ -778,7 +769,7 @@ int onmf_keep8(onmf_ctx* c, int d, int n, const void* X, int x_type, int ldx, in
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
     const size_t all = (size_t)d * groups;
-    if (all > MOST_GROUPS) return onmf_fail(c, ONMF_ERR_ARG, "keep8: %d x %d is more than 2^33 groups", d, n);
+    if (all > MOST_GROUPS) return onmf_fail(c, ONMF_ERR_ARG, "keep8: %d x %d is more than 2^29 - 32 groups of 128", d, n);
     if (x_type == ONMF_TYPE_F32) launch_keep(all, n, groups, (const float*)X, ldx, codes, scales, s);
     else launch_keep(all, n, groups, (const uint16_t*)X, ldx, codes, scales, s);
     HIP_TRY(c, hipGetLastError());
@@ -790,7 +781,7 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
     if (!c) return ONMF_ERR_ARG;
     ONMF_TRY(check8(c, "keep8_expand", d, n, codes, scales));
     const int cols = idx ? b : n;
-    if (!X || cols <= 0 || ldx < cols) return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: bad arguments (b=%d ldx=%d)", b, ldx);
+    if (!X || cols <= 0 || cols > 2147483647 - 1024 || ldx < cols) return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: bad arguments (b=%d ldx=%d)", b, ldx);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
@@ -799,11 +790,9 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
         hipLaunchKernelGGL(keep8_gather_kernel, dim3((b + 255) / 256, std::min(d, 4096)), dim3(256), 0, s, d, n, groups, codes,
                            scales, (const long long*)idx, b, X, ldx);
     else if (all > MOST_GROUPS)
-        return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: %d x %d is more than 2^33 groups", d, n);
-    else if (all < 0x7fffffffu)
-        launch_expand<uint32_t>(all, n, groups, codes, scales, X, ldx, s);
+        return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: %d x %d is more than 2^29 - 32 groups of 128", d, n);
     else
-        launch_expand<uint64_t>(all, n, groups, codes, scales, X, ldx, s);
+        launch_expand(all, n, groups, codes, scales, X, ldx, s);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -823,8 +812,8 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
     ONMF_TRY(check8(c, "keep8_aggregate", r, n, h_codes, h_scales));
     if (!A_out || !B_out) return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: an output is null");
     const size_t need = onmf_keep8_workspace(d, r, n, 0);
-    if ((need && !ws) || ws_bytes < need)
-        return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    if ((need && !ws) || ws_bytes < need || ((uintptr_t)ws & 15))
+        return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: workspace of %zu bytes, %zu needed, aligned to 16", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     return run_sums(c, sum_plan(d, r, n), d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr,
@@ -841,8 +830,10 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
     if (d > (1 << 18) || r > (1 << 18))
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: d=%d or r=%d is more than 2^18", d, r);
     const size_t need = onmf_keep8_workspace(d, r, n, 1);
-    if ((need && !ws) || ws_bytes < need)
-        return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: workspace of %zu bytes, %zu needed", ws_bytes, need);
+    if ((need && !ws) || ws_bytes < need || ((uintptr_t)ws & 15))
+        return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: workspace of %zu bytes, %zu needed, aligned to 16", ws_bytes, need);
+    if (dW < W + (size_t)d * r && W < dW + (size_t)d * r)
+        return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: dW lies over W, which all of it is computed from");
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const SumPlan q = sum_plan(d, r, n);

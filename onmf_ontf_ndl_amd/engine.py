@@ -13,7 +13,7 @@ import warnings
 import numpy as np
 
 from . import _lib
-from .lowbit import GROUP8, GROUPS4, KeptColumns, PackedDictionary
+from .lowbit import GROUP8, GROUPS4, MOST, KeptColumns, PackedDictionary
 
 _engines = {}
 
@@ -480,8 +480,10 @@ class Engine:
         else:
             raise ValueError("%s: the columns must be float32 or bfloat16, not %s" % (what, a.dtype))
         b = shape[1]
+        if b > MOST or shape[0] > MOST:
+            raise ValueError("%s: at most 2^31 - 1 rows and columns, not %s" % (what, tuple(shape)))
         ld = a.stride(0)
-        if (b > 1 and a.stride(1) != 1) or ld < b:         # a transposed, broadcast or reversed view
+        if (b > 1 and a.stride(1) != 1) or ld < b or ld > MOST:         # a transposed or broadcast view, rows far apart
             a = a.contiguous()
             ld = b
         return a, kind, max(ld, b)
@@ -513,6 +515,8 @@ class Engine:
             raise ValueError("dict4_pack: a group is 32, 64 or 128 features, not %s" % (group,))
         if not isinstance(W, self.torch.Tensor) or W.dim() != 2 or W.numel() == 0:
             raise ValueError("dict4_pack: W must be a (d, r) tensor with entries")
+        if max(W.shape) > MOST:
+            raise ValueError("dict4_pack: at most 2^31 - 1 atoms and features, not %s" % (tuple(W.shape),))
         d, r = W.shape
         W = self._matrix(W, (d, r), "dict4_pack: W")
         groups = -(-d // int(group))
@@ -583,9 +587,9 @@ class Engine:
         if idx is None:
             b, ip = n, None
         else:
+            if np.ndim(idx) != 1 or not 0 < len(idx) <= MOST:
+                raise ValueError("keep8_expand: idx must be a vector with entries, at most 2^31 - 1")
             idx = self.dev(idx, self.torch.int64)
-            if idx.dim() != 1 or idx.numel() == 0:
-                raise ValueError("keep8_expand: idx must be a vector with entries")
             self._check_index(idx, n, "keep8_expand")
             b, ip = idx.numel(), _ptr(idx)
         out = self.empty(d, b)

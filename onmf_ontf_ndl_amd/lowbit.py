@@ -18,6 +18,8 @@ __all__ = ["PackedDictionary", "KeptColumns", "pack_dictionary", "keep_columns",
 
 GROUPS4 = (32, 64, 128)      # features that may share a scale in a 4-bit dictionary
 GROUP8 = 128                 # columns that share a scale in an 8-bit store
+MOST = 2 ** 31 - 1           # what the library's sizes hold
+MOST8 = 2 ** 28              # columns of an 8-bit store
 
 
 class PackedDictionary:
@@ -35,6 +37,8 @@ class PackedDictionary:
                 scales.shape != (shape[0], groups):
             raise ValueError("codes must be (r, %d) and scales (r, %d) for d=%d, group=%d"
                              % (groups * group // 2, groups, d, group))
+        if shape[0] > MOST or d > MOST:
+            raise ValueError("a dictionary has at most 2^31 - 1 atoms and features")
         if str(codes.dtype) != "torch.uint8" or str(scales.dtype) != "torch.int32" or codes.device != scales.device:
             raise ValueError("codes must be uint8 and scales int32, on one device")
         if not (codes.is_contiguous() and scales.is_contiguous()):
@@ -70,6 +74,8 @@ class KeptColumns:
         if n <= 0 or len(shape) != 2 or shape[0] == 0 or shape[1] != groups * GROUP8 or \
                 scales.shape != (shape[0], groups):
             raise ValueError("codes must be (d, %d) and scales (d, %d) for n=%d" % (groups * GROUP8, groups, n))
+        if shape[0] > MOST or n > MOST8:
+            raise ValueError("a store has at most 2^31 - 1 rows and 2^28 columns")
         if str(codes.dtype) != "torch.int8" or str(scales.dtype) != "torch.float32" or codes.device != scales.device:
             raise ValueError("codes must be int8 and scales float32, on one device")
         if not (codes.is_contiguous() and scales.is_contiguous()):

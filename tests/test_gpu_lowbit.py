@@ -90,6 +90,7 @@ SHAPES = [  # d, r, b, group: single columns, a few, many; ragged and whole; one
     (257, 300, 33, 32), (1200, 100, 257, 64), (1024, 256, 300, 128), (130, 2000, 65, 64), (4096, 40, 100, 64),
     (8192, 20, 3, 64), (1100, 8200, 2, 32), (700, 9000, 31, 64), (2100, 4000, 64, 128), (3, 5000, 64, 32),
     (60, 40, 1100, 32), (300, 70, 1501, 64), (200, 6001, 200, 32), (2100, 600, 601, 128), (33, 3, 1025, 32), (90, 33, 1030, 64), (777, 1400, 1027, 64),
+    (1300, 900, 1031, 32), (3000, 300, 1026, 128), (700, 4000, 1025, 64),
 ]
 
 
@@ -163,6 +164,14 @@ def test_rows_that_lie_far_apart(eng, torch, dtype):
         K = eng.keep8(view)
         q, s = lo.keep8(Xh)
         assert np.array_equal(K.codes.cpu().numpy(), q) and np.array_equal(host(K.scales), s)
+    # ... and by way of the workspace
+    P, parts = whole_dictionary(eng, rs, d, 20000, 32)
+    Q, qarts = whole_dictionary(eng, rs, 5000, d, 32)
+    b = 1101
+    X, Xh = as_type(torch, eng, rs.randint(-4, 5, size=(d, b)), dtype)
+    wide[:, 7:7 + b] = X
+    assert np.array_equal(host(eng.dict4_correlate(P, wide[:, 7:7 + b])), lo.values4(*parts, d).T @ Xh)
+    assert np.array_equal(host(eng.dict4_product(Q, wide[:, 7:7 + b])), lo.values4(*qarts, 5000) @ Xh)
 
 
 @pytest.mark.parametrize("b", [1, 2, 4, 7, 8, 9, 100, 601, 1101])
@@ -226,15 +235,23 @@ def test_library_refuses_what_the_engine_would_not_send(eng, torch):
                 dict(x=None), dict(c=None), dict(codes=None), dict(b=2 ** 31 - 5, ld=2 ** 31 - 1)):
         assert call(**bad) == -1, bad
         assert b"dict4_correlate" in lib.onmf_last_error(ctx)
-    need = lib.onmf_dict4_workspace(0, 4096, 25, 16, 64)
-    if need:
-        big, _ = whole_dictionary(eng, np.random.RandomState(0), 4096, 25, 64)
-        xx = eng.zeros(4096, 16)
-        ws = torch.empty(need, dtype=torch.uint8, device=eng.device)
-        assert lib.onmf_dict4_correlate(ctx, 4096, 25, 16, 64, _ptr(big.codes), _ptr(big.scales), _ptr(xx), 0, 16, _ptr(out),
-                                        _ptr(ws), need - 1, eng.stream()) == -1
-        assert lib.onmf_dict4_correlate(ctx, 4096, 25, 16, 64, _ptr(big.codes), _ptr(big.scales), _ptr(xx), 0, 16, _ptr(out),
-                                        None, need, eng.stream()) == -1
+    need = lib.onmf_dict4_workspace(0, 8192, 25, 16, 64)
+    assert need > 0
+    big, _ = whole_dictionary(eng, np.random.RandomState(0), 8192, 25, 64)
+    xx, c = eng.zeros(8192, 16), eng.zeros(25, 16)
+    ws = torch.empty(need + 16, dtype=torch.uint8, device=eng.device)
+    for where, n in ((_ptr(ws), need - 1), (None, need), (ws.data_ptr() + 4, need)):
+        assert call(d=8192, r=25, codes=big.codes, x=xx, c=c, ws=None, n=0) == -1
+        assert lib.onmf_dict4_correlate(ctx, 8192, 25, 16, 64, _ptr(big.codes), _ptr(big.scales), _ptr(xx), 0, 16, _ptr(c), where, n,
+                                        eng.stream()) == -1
+    need = lib.onmf_dict4_workspace(1, 64, 5000, 16, 64)
+    assert need > 0
+    big, _ = whole_dictionary(eng, np.random.RandomState(0), 64, 5000, 64)
+    h, out, ws = eng.zeros(5000, 16), eng.zeros(64, 16), torch.empty(need, dtype=torch.uint8, device=eng.device)
+    for bad in (dict(ldr=15), dict(ldh=15), dict(n=need - 1), dict(kind=7), dict(b=0)):
+        a = dict(dict(b=16, kind=0, ldh=16, ldr=16, n=need), **bad)
+        assert lib.onmf_dict4_product(ctx, 64, 5000, a["b"], 64, _ptr(big.codes), _ptr(big.scales), _ptr(h), a["kind"], a["ldh"], _ptr(out),
+                                      a["ldr"], _ptr(ws), a["n"], eng.stream()) == -1, bad
 
 
 # ------------------------------------------------------------------------------------------------- columns in 8 bits
@@ -376,6 +393,28 @@ def test_aggregates_in_place(eng, torch, n):
                                             _ptr(A), _ptr(B), _ptr(A), _ptr(B), _ptr(where), short, eng.stream()) == -1
     assert eng.lib.onmf_keep8(eng.ctx, d, n, _ptr(A), 0, n - 1, _ptr(X.codes), _ptr(X.scales), eng.stream()) == -1
     assert eng.lib.onmf_keep8(eng.ctx, d, n, _ptr(A), 5, n, _ptr(X.codes), _ptr(X.scales), eng.stream()) == -1
+
+
+def test_gradient_refuses_results_over_its_input_and_a_workspace_askew(eng, torch):
+    from onmf_ontf_ndl_amd.engine import _ptr
+    rs = np.random.RandomState(1)
+    d, r = 64, 16
+    both = eng.dev(rs.rand(2 * d, r))
+    for n in (50, 3000):
+        X, H = eng.keep8(eng.dev(rs.rand(d, n))), eng.keep8(eng.dev(rs.rand(r, n)))
+        need = eng.lib.onmf_keep8_workspace(d, r, n, 1)
+        ws = torch.empty(need + 32, dtype=torch.uint8, device=eng.device)
+
+        def call(dW, shift=0, nbytes=need):
+            return eng.lib.onmf_keep8_gradient(eng.ctx, d, r, n, both.data_ptr(), _ptr(X.codes), _ptr(X.scales), _ptr(H.codes),
+                                               _ptr(H.scales), dW, ws.data_ptr() + shift, nbytes, eng.stream())
+        for row in (0, 1, d - 1):
+            assert call(both[row].data_ptr()) == -1
+        assert call(both[d:].data_ptr(), 8) == -1
+        assert call(both[d:].data_ptr()) == 0
+        assert torch.equal(both[d:], eng.keep8_gradient(both[:d], X, H))
+        if need:
+            assert call(both[d:].data_ptr(), 0, need - 1) == -1
 
 
 # ------------------------------------------------------------------------------------------------- streams and graphs

@@ -185,6 +185,33 @@ def test_stores_refuse_before_the_library_is_called(host_side):
             eng.keep8_gradient(W, K, H)
 
 
+def test_sizes_that_no_int_holds_are_refused(host_side):
+    """The library counts in ints: a view of more columns, rows or atoms than one holds (it takes no memory) is refused here
+    and not cut off on the way."""
+    from onmf_ontf_ndl_amd import KeptColumns, PackedDictionary
+    eng, one = host_side, torch.zeros(1, 1)
+    far = 2 ** 32 + 5
+    P = packed()
+    for bad in (one.expand(1, far), one.expand(far, 1), one.bfloat16().expand(1, far)):
+        with pytest.raises(ValueError):
+            eng.keep8(bad)
+    with pytest.raises(ValueError):
+        eng.dict4_correlate(P, one.expand(P.shape[0], far))
+    with pytest.raises(ValueError):
+        eng.dict4_product(P, one.expand(P.shape[1], far))
+    for bad in (one.expand(1, far), one.expand(far, 1)):
+        with pytest.raises(ValueError):
+            eng.dict4_pack(bad)
+    with pytest.raises(ValueError):
+        eng.keep8_expand(kept(), torch.zeros(1, dtype=torch.int64).expand(far))
+    with pytest.raises(ValueError):
+        KeptColumns(torch.zeros(1, 1, dtype=torch.int8).expand(1, 2 ** 28 + 128), torch.zeros(1, 1).expand(1, 2 ** 21 + 1), 2 ** 28 + 1)
+    with pytest.raises(ValueError):
+        KeptColumns(torch.zeros(1, 1, dtype=torch.int8).expand(far, 128), torch.zeros(1, 1).expand(far, 1), 3)
+    with pytest.raises(ValueError):
+        PackedDictionary(torch.zeros(1, 1, dtype=torch.uint8).expand(far, 16), torch.zeros(1, 1, dtype=torch.int32).expand(far, 1), 3, 32)
+
+
 # ------------------------------------------------------------------------------------------------- the library's host side
 def test_entry_points_refuse_a_null_context():
     lib = _lib.load()
