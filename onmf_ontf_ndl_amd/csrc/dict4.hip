@@ -66,77 +66,100 @@ __device__ __forceinline__ float bf16_up(double v) {
     return __uint_as_float(u);
 }
 
-// One thread per group: neighbouring threads take neighbouring atoms, so that reads of W (row-major) coalesce.
-// The scale spans the group's range in 15 steps (14 where rounding both ends to the grid would need a 16th) and
-// is rounded UP to bfloat16, so no entry is clipped and the error is at most s / 2.  Quotients in double: an
-// entry next to a rounding border falls on its own side.
-__global__ __launch_bounds__(256) void dict4_pack_kernel(int d, int r, int group, int groups,
-                                                          const float* __restrict__ W, uint32_t* __restrict__ codes,
-                                                          uint32_t* __restrict__ scales) {
-    const int k = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y;
-    if (k >= r) return;
-    const int i0 = g * group, n = min(group, d - i0);
-    float lo = __int_as_float(0x7f800000), hi = -lo;
-    bool fine = true;
-    for (int i = 0; i < n; ++i) {
-        const float v = W[(size_t)(i0 + i) * r + k];
-        fine = fine && (fabsf(v) < __int_as_float(0x7f800000));
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
-    }
-    uint32_t* out = codes + ((size_t)k * groups + g) * (group / 8);
-    if (!fine) {                       // a NaN or an infinity: the whole group reads NaN
-        scales[(size_t)k * groups + g] = 0x7fc00000u;
-        for (int w = 0; w < group / 8; ++w) out[w] = 0;
-        return;
-    }
-    const double range = (double)hi - (double)lo;
-    const double floor_ = fmax(fabs((double)lo), fabs((double)hi)) / 255.0;
-    float s = bf16_up(fmax(range / 15.0, floor_));
-    if (rint((double)hi / (double)s) - rint((double)lo / (double)s) > 15.0) s = bf16_up(fmax(range / 14.0, floor_));
-    if (!(s >= 1.17549435e-38f)) {     // nothing but (next to) zeros
-        scales[(size_t)k * groups + g] = 0;
-        for (int w = 0; w < group / 8; ++w) out[w] = 0;
-        return;
-    }
-    const double sd = (double)s, z = rint((double)lo / sd);
-    scales[(size_t)k * groups + g] = __float_as_uint(s) | ((uint32_t)(int)z & 0xffffu);
-    for (int w = 0; w < group / 8; ++w) {
-        uint32_t word = 0;
+// 64 atoms of a group a workgroup: a lane an atom, so that reads of W (row-major) coalesce, and a quarter of its features
+// a wave, all on their way together.  The scale spans the group's range in 15 steps (14 where rounding both ends to the
+// grid would need a 16th) and is rounded UP to bfloat16, so no entry is clipped and the error is at most s / 2.  An
+// entry next to a rounding border falls on its own side: v times the reciprocal (1 ulp) is within 255.5 (2^-23 + 2^-24)
+// = 4.6e-5 of the quotient, and only where it lies that near to a half is the quotient itself taken, in double.
+// Bound by memory (d=4096 r=32768, 606 MB: 140 us; one thread a group and all quotients in double 585).
+template <int FEATURES>
+__global__ __launch_bounds__(256) void dict4_pack_kernel(int d, int r, int groups, const float* __restrict__ W,
+                                                          uint32_t* __restrict__ codes, uint32_t* __restrict__ scales) {
+    constexpr int EACH = FEATURES / 4;
+    __shared__ float ends[2][4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = blockIdx.x * 64 + lane, g = blockIdx.y;
+    const int i0 = g * FEATURES + wave * EACH, n = min(EACH, d - i0);        // (n: this wave's, or none)
+    const float most = __int_as_float(0x7f800000);
+    const float* src = W + (size_t)i0 * r + min(k, r - 1);
+    float v[EACH], lo = most, hi = -most;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = w * 8 + j;
-            if (i < n) {
-                const double q = rint((double)W[(size_t)(i0 + i) * r + k] / sd) - z;
-                word |= (uint32_t)(int)q << (4 * ((j >> 1) + 4 * (j & 1)));
+    for (int j = 0; j < EACH; ++j) v[j] = j < n ? src[(size_t)j * r] : 0.f;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j)
+        if (j < n) {
+            if (!(fabsf(v[j]) < most)) lo = -most;       // a NaN or an infinity: the whole group reads NaN
+            lo = fminf(lo, v[j]);
+            hi = fmaxf(hi, v[j]);
+        }
+    ends[0][wave][lane] = lo;
+    ends[1][wave][lane] = hi;
+    __syncthreads();
+    if (k >= r) return;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        lo = fminf(lo, ends[0][w][lane]);
+        hi = fmaxf(hi, ends[1][w][lane]);
+    }
+    uint32_t word[EACH / 8], sc;
+#pragma unroll
+    for (int w = 0; w < EACH / 8; ++w) word[w] = 0;
+    if (lo == -most) {
+        sc = 0x7fc00000u;
+    } else {
+        const double range = (double)hi - (double)lo;
+        const double floor_ = fmax(fabs((double)lo), fabs((double)hi)) / 255.0;
+        float s = bf16_up(fmax(range / 15.0, floor_));
+        if (rint((double)hi / (double)s) - rint((double)lo / (double)s) > 15.0) s = bf16_up(fmax(range / 14.0, floor_));
+        if (!(s >= 1.17549435e-38f)) {     // nothing but (next to) zeros
+            sc = 0;
+        } else {
+            const float z = (float)rint((double)lo / (double)s), inv = __builtin_amdgcn_rcpf(s);
+            sc = __float_as_uint(s) | ((uint32_t)(int)z & 0xffffu);
+#pragma unroll
+            for (int j = 0; j < EACH; ++j) {
+                const float f = v[j] * inv;
+                float q = rintf(f);
+                if (fabsf(f - q) > 0.4999f) q = (float)rint((double)v[j] / (double)s);
+                if (j < n) word[j / 8] |= (uint32_t)(int)(q - z) << (4 * ((j % 8 >> 1) + 4 * (j & 1)));
             }
         }
-        out[w] = word;
     }
+    uint32_t* out = codes + ((size_t)k * groups + g) * (FEATURES / 8) + wave * (EACH / 8);
+    if constexpr (EACH == 32) *reinterpret_cast<uint4*>(out) = make_uint4(word[0], word[1], word[2], word[3]);
+    else if constexpr (EACH == 16) *reinterpret_cast<uint2*>(out) = make_uint2(word[0], word[1]);
+    else out[0] = word[0];
+    if (wave == 0) scales[(size_t)k * groups + g] = sc;
 }
 
-// One thread per word of eight features; neighbouring threads take neighbouring atoms (W's fast index).
+// One thread per four words (32 features, of one group); neighbouring threads take neighbouring atoms (W's fast index).
+// Bound by memory (d=4096 r=32768, 606 MB: 149 us).
 __global__ __launch_bounds__(256) void dict4_unpack_kernel(int d, int r, int group, int groups,
                                                             const uint32_t* __restrict__ codes,
                                                             const uint32_t* __restrict__ scales, float* __restrict__ W) {
-    const int k = blockIdx.x * 256 + threadIdx.x, w = blockIdx.y;
+    const int k = blockIdx.x * 256 + threadIdx.x, w = blockIdx.y * 4;
     if (k >= r) return;
     const uint32_t sc = scales[(size_t)k * groups + (w * 8) / group];
     const float s = word_scale(sc), z = word_offset(sc);
-    float q[8];
-    word_entries(codes[(size_t)k * groups * (group / 8) + w], q);
+    const uint4 v = *reinterpret_cast<const uint4*>(codes + (size_t)k * groups * (group / 8) + w);
+    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (w * 8 + j < d) W[(size_t)(w * 8 + j) * r + k] = s * (q[j] + z);
+    for (int u = 0; u < 4; ++u) {
+        float q[8];
+        word_entries(words[u], q);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if ((w + u) * 8 + j < d) W[(size_t)((w + u) * 8 + j) * r + k] = s * (q[j] + z);
+    }
 }
 
 // ------------------------------------------------------------------------------------------- few columns
-// C = W^T X for up to NB columns: bound by reading the codes once.  A lane owns F = 8 CH consecutive features
-// of a segment of 64 F; X is staged in LDS as float and a segment's F x NB values are held in registers while AT
-// atoms stream past.  One code costs an extraction (0.4), a conversion and NB fused multiply-adds.
-// LDS: quad q (of F / 4) of lane l of segment g and column n at [((g * F/4 + q) * 64 + l) * 4] of plane n.
-template <int NB, int CH, int AT, typename T>
-__global__ __launch_bounds__(256) void dict4_correlate_few_kernel(int d, int r, int b, int group, int groups,
+// C = W^T x for one column: bound by reading the codes once (d=4096 r=32768, 71 MB: 18 us, 3.9 TB/s; d=441 r=25 3 us, a
+// launch).  A lane owns F = 8 CH consecutive features of a segment of 64 F; x is staged in LDS as float and a
+// segment's F values are held in registers while AT atoms stream past.  An entry costs an extraction (0.4), a
+// conversion and a fused multiply-add; z is taken once a group, with the sum of its features.
+// LDS: quad q (of F / 4) of lane l of segment g at [((g * F/4 + q) * 64 + l) * 4].
+template <int CH, int AT, typename T>
+__global__ __launch_bounds__(256) void dict4_correlate_one_kernel(int d, int r, int group, int groups,
                                                                    const uint32_t* __restrict__ codes,
                                                                    const uint32_t* __restrict__ scales,
                                                                    const T* __restrict__ X, int ldx,
@@ -146,26 +169,21 @@ __global__ __launch_bounds__(256) void dict4_correlate_few_kernel(int d, int r, 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int segs = (d + SEG - 1) / SEG;
     const int words = groups * (group / 8);
-    const int plane = segs_staged * SEG;
     const int chunks = (r + 4 * AT - 1) / (4 * AT);
     bool first = true;
     for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
         const int k0 = chunk * 4 * AT + wave * AT;
-        float acc[AT][NB];
+        float acc[AT];
 #pragma unroll
-        for (int a = 0; a < AT; ++a)
-#pragma unroll
-            for (int n = 0; n < NB; ++n) acc[a][n] = 0.f;
+        for (int a = 0; a < AT; ++a) acc[a] = 0.f;
         for (int s0 = 0; s0 < segs; s0 += segs_staged) {
-            if (first || segs_staged < segs) {          // the whole of X fits: staged once
+            if (first || segs_staged < segs) {          // the whole of x fits: staged once
                 __syncthreads();
-                const int i0 = s0 * SEG, in = min(plane, segs * SEG - i0);
-                for (int e = threadIdx.x; e < in * NB; e += 256) {
-                    const int n = NB == 1 ? 0 : e % NB, i = NB == 1 ? e : e / NB;
-                    float v = 0.f;
-                    if (i0 + i < d && n < b) v = load_val(X + (size_t)(i0 + i) * ldx + n);
+                const int i0 = s0 * SEG, in = min(segs_staged, segs - s0) * SEG;
+                for (int i = threadIdx.x; i < in; i += 256) {
+                    const float v = i0 + i < d ? load_val(X + (size_t)(i0 + i) * ldx) : 0.f;
                     const int g = i / SEG, l = (i % SEG) / F, f = i % F;
-                    xs[n * plane + ((g * (F / 4) + (f >> 2)) * 64 + l) * 4 + (f & 3)] = v;
+                    xs[((g * (F / 4) + (f >> 2)) * 64 + l) * 4 + (f & 3)] = v;
                 }
                 __syncthreads();
                 first = false;
@@ -174,16 +192,12 @@ __global__ __launch_bounds__(256) void dict4_correlate_few_kernel(int d, int r, 
             for (int g = 0; g < sn; ++g) {
                 const int w0 = (s0 + g) * (SEG / 8) + lane * CH;       // this lane's first word
                 if (w0 >= words) continue;                               // padding of the last segment
-                float x[F][NB], sum[NB];
+                float x[F], sum = 0.f;
 #pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    sum[n] = 0.f;
-#pragma unroll
-                    for (int q = 0; q < F / 4; ++q) {
-                        const float4 v = *reinterpret_cast<const float4*>(&xs[n * plane + ((g * (F / 4) + q) * 64 + lane) * 4]);
-                        x[4 * q + 0][n] = v.x; x[4 * q + 1][n] = v.y; x[4 * q + 2][n] = v.z; x[4 * q + 3][n] = v.w;
-                        sum[n] += (v.x + v.y) + (v.z + v.w);
-                    }
+                for (int q = 0; q < F / 4; ++q) {
+                    const float4 v = *reinterpret_cast<const float4*>(&xs[((g * (F / 4) + q) * 64 + lane) * 4]);
+                    x[4 * q + 0] = v.x; x[4 * q + 1] = v.y; x[4 * q + 2] = v.z; x[4 * q + 3] = v.w;
+                    sum += (v.x + v.y) + (v.z + v.w);
                 }
                 uint32_t cw[AT][CH], sc[AT];
 #pragma unroll
@@ -203,38 +217,32 @@ __global__ __launch_bounds__(256) void dict4_correlate_few_kernel(int d, int r, 
                 }
 #pragma unroll
                 for (int a = 0; a < AT; ++a) {
-                    float t[NB];
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) t[n] = word_offset(sc[a]) * sum[n];
+                    float t = word_offset(sc[a]) * sum;
 #pragma unroll
                     for (int c = 0; c < CH; ++c) {
                         float q[8];
                         word_entries(cw[a][c], q);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-#pragma unroll
-                            for (int n = 0; n < NB; ++n) t[n] = fmaf(q[j], x[8 * c + j][n], t[n]);
+                        for (int j = 0; j < 8; ++j) t = fmaf(q[j], x[8 * c + j], t);
                     }
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) acc[a][n] = fmaf(word_scale(sc[a]), t[n], acc[a][n]);
+                    acc[a] = fmaf(word_scale(sc[a]), t, acc[a]);
                 }
             }
         }
 #pragma unroll
-        for (int a = 0; a < AT; ++a)
+        for (int a = 0; a < AT; ++a) {
+            float v = acc[a];
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                float v = acc[a][n];
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-                if (lane == 0 && k0 + a < r && n < b) C[(size_t)(k0 + a) * b + n] = v;
-            }
+            for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+            if (lane == 0 && k0 + a < r) C[k0 + a] = v;
+        }
     }
 }
 
-// R = W H for up to NB columns: a lane owns F features of a segment and adds up its atoms' contributions
-// h (s q + s z) in registers; the NW waves of a workgroup take different atoms, AT at a time, and are added in LDS,
-// workgroups of the same segment in slabs; both in a fixed order.
+// R = W H for one or two columns (d=8192 r=16384, 75 MB with the scales: 20 and 27 us; d=1024 r=256 5 us, one launch):
+// bound by instructions, 1.4 + NB an entry, and by the codes' way from memory.  A lane owns F features of a segment and
+// adds up its atoms' contributions h (s q + s z) in registers; the NW waves of a workgroup take different atoms, AT at
+// a time, and are added in LDS, workgroups of the same segment in slabs; both in a fixed order.
 template <int NB, int CH, int NW, typename T>
 __global__ __launch_bounds__(64 * NW) void dict4_product_few_kernel(int d, int r, int b, int group, int groups,
                                                                      const uint32_t* __restrict__ codes,
@@ -317,7 +325,8 @@ __global__ __launch_bounds__(64 * NW) void dict4_product_few_kernel(int d, int r
 // eight nibbles at one place are the operand of one row at eight consecutive steps of the contraction, so a tile's
 // 16 rows are the features at that place of the words of 16 lanes, and nothing has to be turned round.  An entry
 // s (q + z) has at most 16 significant bits: its upper half and the rest are bfloat16 values exactly.  Per weight
-// 5.4 vector instructions whatever the number of columns, against 1.4 + one a column on the vector pipe.
+// 5.4 vector instructions whatever the number of columns, against 1.4 + one a column on the vector pipe: they are
+// the bound (d=8192 r=16384 b=7 39 us, b=32 56 us; the codes and scales are 75 MB).
 // The waves of a workgroup take different atoms of the same 128 CW features and are added in LDS, workgroups of
 // the same features in slabs; both in a fixed order.
 template <int NT, int CW, typename T>
@@ -461,7 +470,8 @@ __global__ __launch_bounds__(256, 2) void dict4_product_tile_kernel(int d, int r
     }
 }
 
-// out[m][n] = sum over the slabs z of slab[z][m][n], four threads an entry, in a fixed order
+// out[m][n] = sum over the slabs z of slab[z][m][n], four threads an entry, in a fixed order; bound by reading them
+// (22 slabs of 16384 x 64: 22 us, 4.2 TB/s)
 __global__ __launch_bounds__(256) void dict4_reduce_kernel(size_t mn, int N, int splits, const float* __restrict__ slab,
                                                             float* __restrict__ out, int ldo) {
     __shared__ float part[4][64];
@@ -486,7 +496,9 @@ __global__ __launch_bounds__(256) void dict4_reduce_kernel(size_t mn, int N, int
 // the lane has, is multiplied to it; the whole numbers q + z themselves are bfloat16 values.  A workgroup keeps
 // `per` features of X in LDS, already cut into bfloat16 pieces in the operand's order, and its waves take 32 atoms at a
 // time past it; ranges of features are added up in slabs.  A lane loads 16 bytes, four words of 128 features, two
-// blocks ahead; the 4 x 4 words of the lanes l % 16 + 16 j change places in four instructions.
+// blocks ahead; the 4 x 4 words of the lanes l % 16 + 16 j change places in four instructions.  Bound by its vector
+// instructions (3 an entry for up to 16 columns) and, with more columns, the operand reads from LDS and the slabs
+// (float32, d=8192 r=16384: b=8 58 us and 5 for adding up, b=32 54 and 8, b=64 69 and 22).
 template <int NT, typename T>
 __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r, int b, int group, int groups,
                                                                       const uint32_t* __restrict__ codes,
@@ -629,7 +641,8 @@ __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r,
 }
 
 // The same for results so small that a launch counts as much as the work: a workgroup owns 16 atoms, its NW waves share the
-// steps of 32 features, DEPTH of them on their way, each cutting its part of X into pieces itself, and add up in LDS.
+// steps of 32 features, DEPTH of them on their way, each cutting its part of X into pieces itself, and add up in LDS
+// (d=441 r=72 b=3 3.4 us, of which a launch is 2.5; by ranges and slabs 7.4).
 template <int NT, int NW, typename T>
 __global__ __launch_bounds__(64 * NW) void dict4_correlate_wave_kernel(int d, int r, int b, int group, int groups,
                                                                        const uint32_t* __restrict__ codes,
@@ -723,11 +736,15 @@ __global__ __launch_bounds__(64 * NW) void dict4_correlate_wave_kernel(int d, in
 // A workgroup owns 16 MT rows and 128 (bfloat16: 256) columns, a wave all its rows and a quarter of its columns, so
 // that every column is split into its pieces once and in registers: lane l holds columns 2 (l % 16) and the next, at
 // k = 8 (l / 16) .. + 7, the operand of two tiles.  (bfloat16 columns need no split and a wave takes four tiles of
-// them, for half the reads of weights from LDS, which bound it before: d=1024 r=256 b=65536 66 -> 52 us.)  The weights go from memory to LDS, one step of 32 ahead, in rows of 64 bytes whose
-// 16-byte chunks are permuted by (row >> 2) & 3: the 16 rows of an operand read meet every bank once.
+// them, for half the reads of weights from LDS, which bound it before: d=1024 r=256 b=65536 66 -> 54 us.)  The weights
+// go from memory to LDS, one step of 32 ahead, in rows of 64 bytes whose 16-byte chunks are permuted by
+// (row >> 2) & 3: the 16 rows of an operand read meet every bank once.
+// Bound by the matrix pipe: W^T X d=1024 r=256 b=65536 float32 100 us, 1.03 PFLOP/s of the three products; W H 162 us,
+// 1.06 of five; with few columns by what a step waits for its loads.
 constexpr int BK = 32;
 
-// correlate's weights: [k][features, padded to whole groups with zeros] whole numbers, and the scales as floats [group][k]
+// correlate's weights: [k][features, padded to whole groups with zeros] whole numbers, and the scales as floats [group][k];
+// bound by writing them (d=6492 r=9202, 157 MB: 35 us)
 __global__ __launch_bounds__(256) void dict4_lay_correlate_kernel(int d, int r, int words, int group, int groups,
                                                                    const uint32_t* __restrict__ codes,
                                                                    const uint32_t* __restrict__ scales,
@@ -747,7 +764,7 @@ __global__ __launch_bounds__(256) void dict4_lay_correlate_kernel(int d, int r, 
 }
 
 // the product's weights: [piece][feature][atoms, padded to kp with zeros]; 128 features x 64 atoms a workgroup,
-// turned round in LDS
+// turned round in LDS (d=1200 r=100 6 us; bound by writing them where they are many, 4 bytes a weight)
 __global__ __launch_bounds__(256) void dict4_lay_product_kernel(int d, int r, int words, int group, int groups, int kp,
                                                                  const uint32_t* __restrict__ codes,
                                                                  const uint32_t* __restrict__ scales,
@@ -885,7 +902,8 @@ __device__ __forceinline__ void row_tiles(const char* a, const float* s, int lan
                 if (qx + qw > 2) continue;
 #pragma unroll
                 for (int c = 0; c < CT; ++c)
-                    part[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1][qw], __builtin_bit_cast(bf16x8, fb[c][qx]), part[c], 0, 0, 0);
+                    part[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa[i & 1][qw], __builtin_bit_cast(bf16x8, fb[c][qx]),
+                                                                      part[c], 0, 0, 0);
             }
         if constexpr (PROD) {
 #pragma unroll
@@ -991,7 +1009,8 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
 
 // The same for a contraction so short that a workgroup keeps all its rows' weights in LDS: it unpacks them there itself, and
 // its four waves take one set of columns after the other past them, each at its own pace, the next step's columns on
-// their way.  One launch, no workspace.
+// their way.  One launch, no workspace.  (W H float32 d=1200 r=100 b=8192 22 us, 39 MB of results; laid out
+// first and multiplied in a second launch 26.)
 struct ResidentParams {
     const uint32_t *codes, *scales;
     const void* X;
@@ -1085,7 +1104,7 @@ __global__ __launch_bounds__(256, 2) void dict4_resident_kernel(ResidentParams p
 
 // ------------------------------------------------------------------------------------------- launches
 constexpr int MOST_COLS = 2147483647 - 1024;    // tile arithmetic in int
-constexpr int FEW = 1, FEW_PRODUCT = 2;     // columns up to which the vector kernels run
+constexpr int FEW_PRODUCT = 2;              // columns up to which the product's vector kernel runs
 // ... and the tile kernels, a block of columns in the grid for every 32 (product) or 64.  With more columns the weights
 // are better laid out once (us, tile and many columns' kernels: W H, d=8192 r=16384 b=192 340 and 507, b=1000 1337
 // and 1270, d=1024 r=1024 b=512 18.6 and 27.6; W^T X, float32, d=8192 r=16384 b=128 173 and 222, b=256 420 and
@@ -1094,21 +1113,15 @@ constexpr int TILE_PRODUCT = 1024;
 constexpr size_t RESIDENT_BYTES = 150 * 1024;
 int most_tile_columns(int d, int r, bool wide) { return !wide || (long long)d * r <= 1 << 20 ? 512 : 192; }     // (the correlate's)
 
-struct FewPlan { int nb, ch; };
-FewPlan few_plan(int d, int b) {
-    FewPlan f;
-    f.nb = b <= 1 ? 1 : b <= 2 ? 2 : b <= 4 ? 4 : 8;
-    f.ch = f.nb <= 2 ? 4 : f.nb == 4 ? 2 : 1;
-    while (f.ch > 1 && d <= 64 * 8 * (f.ch / 2)) f.ch /= 2;         // one segment is enough with narrower lanes
-    return f;
-}
+// words a lane of the vector kernels: one segment is enough with narrower lanes where there are few features
+int words_a_lane(int d) { return d <= 512 ? 1 : d <= 1024 ? 2 : 4; }
 // The vector kernel's split of the atoms.  Up to 512 atoms one workgroup of 16 waves takes them all, in one launch
 // with nothing to add up behind it.
 struct FewProduct { bool one; int ch, segs, splits, per; };
-FewProduct product_few_plan(int d, int r, int b) {
+FewProduct product_few_plan(int d, int r) {
     FewProduct q;
     q.one = r <= 512;
-    q.ch = q.one ? 1 : few_plan(d, b).ch;
+    q.ch = q.one ? 1 : words_a_lane(d);
     q.segs = (d + 512 * q.ch - 1) / (512 * q.ch);
     const int splits = q.one ? 1 : std::max(1, std::min(1024 / q.segs, r / 128));      // 32 atoms a wave at least
     q.per = ((r + splits - 1) / splits + 31) / 32 * 32;
@@ -1163,18 +1176,15 @@ int add_slabs(onmf_ctx* c, size_t mn, int N, int splits, const float* slab, floa
     return ONMF_OK;
 }
 
-template <int NB, int CH, typename T>
-int correlate_few(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales,
-                  const T* X, int ldx, float* C, hipStream_t s) {
+template <int CH, typename T>
+int correlate_one(onmf_ctx* c, int d, int r, int group, const uint32_t* codes, const uint32_t* scales, const T* X, int ldx,
+                  float* C, hipStream_t s) {
     constexpr int AT = 4, SEG = 512 * CH;
     const int segs = (d + SEG - 1) / SEG, groups = (d + group - 1) / group;
-    const int staged = std::min(segs, std::max(1, (int)(65536 / (sizeof(float) * SEG * NB))));
-    const size_t bytes = sizeof(float) * (size_t)staged * SEG * NB;
-    static LdsLimit lim;
-    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)dict4_correlate_few_kernel<NB, CH, AT, T>, bytes));
+    const int staged = std::min(segs, (int)(65536 / (sizeof(float) * SEG)));
     const int chunks = (r + 4 * AT - 1) / (4 * AT);
-    hipLaunchKernelGGL((dict4_correlate_few_kernel<NB, CH, AT, T>), dim3(std::min(chunks, 1024)), dim3(256), bytes, s, d, r,
-                       b, group, groups, codes, scales, X, ldx, C, staged);
+    hipLaunchKernelGGL((dict4_correlate_one_kernel<CH, AT, T>), dim3(std::min(chunks, 1024)), dim3(256),
+                       sizeof(float) * (size_t)staged * SEG, s, d, r, group, groups, codes, scales, X, ldx, C, staged);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -1252,9 +1262,11 @@ int correlate_wave(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* 
     const dim3 grid((r + 15) / 16);
     const int groups = (d + group - 1) / group;
     if (d <= 256)
-        hipLaunchKernelGGL((dict4_correlate_wave_kernel<NT, 4, T>), grid, dim3(256), 0, s, d, r, b, group, groups, codes, scales, X, ldx, C);
+        hipLaunchKernelGGL((dict4_correlate_wave_kernel<NT, 4, T>), grid, dim3(256), 0, s, d, r, b, group, groups, codes, scales,
+                           X, ldx, C);
     else
-        hipLaunchKernelGGL((dict4_correlate_wave_kernel<NT, 16, T>), grid, dim3(1024), 0, s, d, r, b, group, groups, codes, scales, X, ldx, C);
+        hipLaunchKernelGGL((dict4_correlate_wave_kernel<NT, 16, T>), grid, dim3(1024), 0, s, d, r, b, group, groups, codes, scales,
+                           X, ldx, C);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -1316,12 +1328,14 @@ struct ResidentPlan { int mt, tiles_m, parts; size_t bytes; };
 ResidentPlan resident_plan(const ManyPlan& many, bool prod, int d, int r, int b, int group, bool wide) {
     ResidentPlan q;
     q.mt = 0;
-    const int M = prod ? d : r, K = prod ? r : d, steps = (K + BK - 1) / BK, cols = 16 * (wide ? COLUMN_TILES<float> : COLUMN_TILES<uint16_t>);
+    const int M = prod ? d : r, K = prod ? r : d, steps = (K + BK - 1) / BK;
+    const int cols = 16 * (wide ? COLUMN_TILES<float> : COLUMN_TILES<uint16_t>);
     const int sets = (b + cols - 1) / cols;
     const double own = wide ? (prod ? 0.5 : 0.35) : 0.26, row = prod && !wide ? 0.16 : 0.145;
     double best = many.cost + 8.0 + (prod ? 4.5 : 2.5) * d * r / 4e6 + 4.0 * M * b / 8e6;
     for (int mt = wide ? 8 : 4; mt >= 2; mt /= 2) {            // (what the registers hold)
-        const size_t bytes = (size_t)steps * (prod ? 2 : 1) * 16 * mt * 64 + (prod ? 0 : sizeof(float) * ((steps * BK + group - 1) / group) * 16 * mt);
+        const size_t scale_bytes = prod ? 0 : sizeof(float) * ((steps * BK + group - 1) / group) * 16 * mt;
+        const size_t bytes = (size_t)steps * (prod ? 2 : 1) * 16 * mt * 64 + scale_bytes;
         if (bytes > RESIDENT_BYTES) continue;
         const int tiles_m = (M + 16 * mt - 1) / (16 * mt), resident = bytes > RESIDENT_BYTES / 2 ? 1 : 2;
         const double waves = (double)sets * tiles_m, step = (own + row * mt) * (waves > 1024 && resident == 2 ? 1.5 : 1.0);
@@ -1371,9 +1385,9 @@ int check4(onmf_ctx* c, const char* what, int d, int r, int group, const void* c
 
 size_t workspace_of(bool prod, int d, int r, int b, int group, bool wide) {
     int splits = 1;
-    if (prod && b <= FEW_PRODUCT) splits = product_few_plan(d, r, b).splits;
+    if (prod && b <= FEW_PRODUCT) splits = product_few_plan(d, r).splits;
     else if (prod && b <= TILE_PRODUCT) splits = product_tile_plan(d, r, b, group).splits;
-    else if (!prod && b <= FEW) splits = 1;
+    else if (!prod && b == 1) splits = 1;
     else if (!prod && b <= most_tile_columns(d, r, wide)) {
         const RangePlan q = correlate_tile_plan(d, r, b, wide);
         splits = q.one ? 1 : q.splits;
@@ -1387,12 +1401,11 @@ size_t workspace_of(bool prod, int d, int r, int b, int group, bool wide) {
 template <typename T>
 int correlate_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* X,
                 int ldx, float* C, float* ws, hipStream_t s) {
-    if (b <= FEW) {
-        const FewPlan f = few_plan(d, b);
-#define FEW_CASE(NB, CH) if (f.nb == NB && f.ch == CH) return correlate_few<NB, CH, T>(c, d, r, b, group, codes, scales, X, ldx, C, s)
-        FEW_CASE(1, 1); FEW_CASE(1, 2); FEW_CASE(1, 4); FEW_CASE(2, 1); FEW_CASE(2, 2); FEW_CASE(2, 4);
-        FEW_CASE(4, 1); FEW_CASE(4, 2); FEW_CASE(8, 1);
-#undef FEW_CASE
+    if (b == 1) {
+        const int ch = words_a_lane(d);
+        if (ch == 1) return correlate_one<1, T>(c, d, r, group, codes, scales, X, ldx, C, s);
+        if (ch == 2) return correlate_one<2, T>(c, d, r, group, codes, scales, X, ldx, C, s);
+        return correlate_one<4, T>(c, d, r, group, codes, scales, X, ldx, C, s);
     }
     if (b <= most_tile_columns(d, r, sizeof(T) == 4)) {
         const RangePlan q = correlate_tile_plan(d, r, b, sizeof(T) == 4);
@@ -1413,7 +1426,7 @@ template <typename T>
 int product_t(onmf_ctx* c, int d, int r, int b, int group, const uint32_t* codes, const uint32_t* scales, const T* H,
               int ldh, float* R, int ldr, float* ws, hipStream_t s) {
     if (b <= FEW_PRODUCT) {
-        const FewProduct q = product_few_plan(d, r, b);
+        const FewProduct q = product_few_plan(d, r);
 #define FEW_CASE(NB, CH) \
     if (b <= NB && q.ch == CH && !q.one) return product_few<NB, CH, 4, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s)
         if (q.one && b == 1) return product_few<1, 1, 16, T>(c, q, d, r, b, group, codes, scales, H, ldh, R, ldr, ws, s);
@@ -1450,8 +1463,9 @@ int onmf_dict4_pack(onmf_ctx* c, int d, int r, int group, const float* W, void* 
     if (!W) return onmf_fail(c, ONMF_ERR_ARG, "dict4_pack: W is null");
     ONMF_ENTER(c);
     const int groups = (d + group - 1) / group;
-    hipLaunchKernelGGL(dict4_pack_kernel, dim3((r + 255) / 256, groups), dim3(256), 0, (hipStream_t)stream, d, r, group,
-                       groups, W, (uint32_t*)codes, (uint32_t*)scales);
+    const dim3 grid((r + 63) / 64, groups);
+    const auto kernel = group == 128 ? dict4_pack_kernel<128> : group == 64 ? dict4_pack_kernel<64> : dict4_pack_kernel<32>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, (hipStream_t)stream, d, r, groups, W, (uint32_t*)codes, (uint32_t*)scales);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -1463,7 +1477,7 @@ int onmf_dict4_unpack(onmf_ctx* c, int d, int r, int group, const void* codes, c
     if (!W) return onmf_fail(c, ONMF_ERR_ARG, "dict4_unpack: W is null");
     ONMF_ENTER(c);
     const int groups = (d + group - 1) / group;
-    hipLaunchKernelGGL(dict4_unpack_kernel, dim3((r + 255) / 256, (d + 7) / 8), dim3(256), 0, (hipStream_t)stream, d, r, group,
+    hipLaunchKernelGGL(dict4_unpack_kernel, dim3((r + 255) / 256, (d + 31) / 32), dim3(256), 0, (hipStream_t)stream, d, r, group,
                        groups, (const uint32_t*)codes, (const uint32_t*)scales, W);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;

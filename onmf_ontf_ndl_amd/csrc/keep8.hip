@@ -53,7 +53,7 @@ struct GroupAt {
 };
 
 // 16 lanes per group, eight columns a lane, U groups a lane (their loads are on their way together).  Bound by
-// memory: 5 bytes a float32 entry, 3 a bfloat16 one.
+// memory: 5 bytes a float32 entry, 3 a bfloat16 one (1024 x 65536: float32 60 us, 5.6 TB/s, bfloat16 43, 4.7).
 template <typename T, int U>
 __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int groups, const T* __restrict__ X, int ldx,
                                                      int8_t* __restrict__ codes, float* __restrict__ scales) {
@@ -130,6 +130,8 @@ __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int group
 }
 
 // ------------------------------------------------------------------------------------------- bring back
+// 32 lanes per group, four columns a lane, U groups a lane.  Bound by memory, 5 bytes an entry (1024 x 65536: 60 us,
+// 5.6 TB/s).
 template <int U>
 __global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, int groups, const int8_t* __restrict__ codes,
                                                             const float* __restrict__ scales, float* __restrict__ X,
@@ -164,7 +166,8 @@ __global__ __launch_bounds__(256) void keep8_expand_kernel(size_t all, int n, in
     }
 }
 
-// X[:, j] = column idx[j]; a negative index counts from the end, one out of range reads NaN.
+// X[:, j] = column idx[j]; a negative index counts from the end, one out of range reads NaN.  Bound by its reads, a byte
+// of every 64 that come (8192 columns at random of 1024 x 65536: 68 us).
 __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int groups, const int8_t* __restrict__ codes,
                                                             const float* __restrict__ scales,
                                                             const long long* __restrict__ idx, int b,
@@ -190,7 +193,8 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 // in rows of 128 bytes whose 16-byte chunks are permuted by (row >> 1) & 7, so that the 16 rows of an operand read
 // meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.
 // Per group and output three vector instructions (conversion, product of the scales, fused multiply-add) stand
-// against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not.
+// against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not
+// (d=4096 r=256 n=65536, 146 GOP: 125 us; d=1024 40 us).
 template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
     static constexpr int mi = MI, nj = NJ, wm = WM_, wn = WN_, stages = STAGES;
     static constexpr int bm = 16 * MI * WM_, bn = 16 * NJ * WN_, waves = WM_ * WN_;
@@ -379,7 +383,8 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
 #pragma unroll
         for (int j = 0; j < S::nj; ++j) {
             const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
-            if (n < N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.cols + n) = acc[i][j];      // (rows of the slab are padded to whole quads)
+            // (rows of the slab are padded to whole quads)
+            if (n < N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.cols + n) = acc[i][j];
         }
     }
 }
@@ -396,7 +401,8 @@ __device__ __forceinline__ void sum_slabs(const float* src, size_t stride, int s
     }
 }
 
-// A = keep A_in + w sum, B = keep B_in + w sum; with Ad and Bd (the gradient) the sums themselves, as doubles.
+// A = keep A_in + w sum, B = keep B_in + w sum; with Ad and Bd (the gradient) the sums themselves, as doubles.  Bound by
+// reading the slabs (d=4096 r=256 n=65536 8.7 us).
 template <int ZL>
 __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int cols_h, int cols, int splits,
                                                             const float* __restrict__ slab, double w, double keep,
@@ -435,7 +441,7 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // nearly cancel.  A workgroup owns a 32 x 32 tile, its NW waves share the sum over j in sixteens and add up in LDS.  A
 // wave loads the double matrix pipe's operands (16x16x4) straight into registers, the next sixteen while these are
 // computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
-// row 4 e + l / 16.
+// row 4 e + l / 16.  Bound by the double matrix pipe where r is large (d=4096 r=1024 197 us, 44 TFLOP/s; r=256 19.5).
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 template <int NW, typename S>
 __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
@@ -509,7 +515,8 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
 // pipe: row l % 16 of W and 16 columns of H at k = 16 s + 4 (l / 16) + j in the j-th instruction, so that a lane
 // loads four neighbours of W and words of four codes; the scale of an atom goes with W, one exact double product),
 // add up in LDS and take X off; then they share the atoms of the result, with the residual's operands in registers and the
-// scale of an atom on its sum.  TILES sixteens of columns (1, 4 or 8), NW waves.
+// scale of an atom on its sum.  TILES sixteens of columns (1, 4 or 8), NW waves.  Bound by the double matrix pipe of the
+// CUs that have rows (d=2372 r=581 n=2 9.6 us, n=128 30; by the sums 60).
 template <int TILES, int NW>
 __global__ __launch_bounds__(64 * NW) void keep8_residual_kernel(int d, int r, const float* __restrict__ W,
                                                                   const int8_t* __restrict__ xc, const float* __restrict__ xs,
@@ -781,7 +788,8 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
     if (!c) return ONMF_ERR_ARG;
     ONMF_TRY(check8(c, "keep8_expand", d, n, codes, scales));
     const int cols = idx ? b : n;
-    if (!X || cols <= 0 || cols > 2147483647 - 1024 || ldx < cols) return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: bad arguments (b=%d ldx=%d)", b, ldx);
+    if (!X || cols <= 0 || cols > 2147483647 - 1024 || ldx < cols)
+        return onmf_fail(c, ONMF_ERR_ARG, "keep8_expand: bad arguments (b=%d ldx=%d)", b, ldx);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     const int groups = (n + GROUP - 1) / GROUP;
@@ -816,8 +824,8 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: workspace of %zu bytes, %zu needed, aligned to 16", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    return run_sums(c, sum_plan(d, r, n), d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in, A_out, B_out, nullptr,
-                    nullptr, s);
+    return run_sums(c, sum_plan(d, r, n), d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in,
+                    A_out, B_out, nullptr, nullptr, s);
 }
 
 int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const int8_t* x_codes, const float* x_scales,
