@@ -381,8 +381,8 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
 /*
  * Columns held in 8 bits (no counterpart in the reference): a minibatch X and its code H put away in a quarter of
  * their room until the dictionary's update or gradient needs them.  128 consecutive columns of a row share a scale
- * s = max|v| / 127 (float32); an entry stands for s q, q = rint(v / s), ties to even, decided exactly, and differs
- * from v by at most s / 2.  A group whose scale would be below 2^-126 reads as zeros, one with a NaN or an infinity
+ * s = max|v| / 127 (float32: the product with the float32 nearest to 1 / 127); an entry stands for s q, q = rint(v / s),
+ * ties to even, decided exactly, and differs from v by at most s / 2.  A group whose scale would be below 2^-126 reads as zeros, one with a NaN or an infinity
  * as NaNs.
  *   codes   int8, d rows of ceil(n / 128) * 128, aligned to 16 bytes; the padding behind column n is zeros
  *   scales  float32, d rows of ceil(n / 128)

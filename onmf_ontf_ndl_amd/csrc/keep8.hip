@@ -1,7 +1,7 @@
 // Columns held in 8 bits and what the dictionary's update needs of them, on gfx950.
 //
-// Format: 128 consecutive columns of a row share a scale s = max |v| / 127 (float32); an entry stands for s q,
-// q = rint(v / s) in -127..127.  codes is [row][padded columns] int8 (rows padded to whole groups with zeros),
+// Format: 128 consecutive columns of a row share a scale s = max |v| / 127 (float32, by the reciprocal of 127, as float
+// arrays are divided by a number on the GPU); an entry stands for s q, q = rint(v / s) in -127..127.  codes is [row][padded columns] int8 (rows padded to whole groups with zeros),
 // scales [row][group].  A minibatch X and its code H put away this way take a quarter of their room, and the
 // sums H H^T and H X^T - the gradient to the dictionary is W (H H^T) - X H^T - run on the 8-bit matrix pipe:
 // inside a group the products of whole numbers add up exactly in int32.
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void keep8_kernel(size_t all, int n, int group
 #pragma unroll
         for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(v[u][j]) & 0x7fffffffu);
         most = max16(most);
-        float s = __uint_as_float(most) / 127.f;
+        float s = __uint_as_float(most) * (1.f / 127.f);
         float q[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) q[j] = 0.f;

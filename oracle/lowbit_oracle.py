@@ -85,7 +85,7 @@ def keep8(X):
             if not np.isfinite(part).all():
                 s[i, g] = math.nan
                 continue
-            step = float(np.float32(np.abs(part).max() / 127))
+            step = float(np.float32(np.abs(part).max()) * np.float32(1 / 127))
             if step < 2.0 ** -126:
                 continue
             s[i, g] = step
