@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 // rows of any length: vectors that need no more alignment than their entries (the memory pipe takes them as they lie)
@@ -510,6 +511,170 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
     }
 }
 
+// The same on the 8-bit matrix pipe, where r is large.  Each row of W and of A (which is symmetric) is scaled by a power of
+// two to at most a half and cut into four whole digits of 7 bits, x = sum_t q_t 2^(-7 (t + 1)) within 2^-29, that is
+// 2^-27 of the row's largest entry: an eighth of what the float32 runs of A's sums are off by.  Products of digits add
+// up exactly in int32, those of one weight, t + u = 0..3, in one sum; what is left out (t + u > 3) is 2^-28 and less of
+// the largest.  The four sums, the powers of two and B meet in double.  Bound by the matrix pipe (d=4096 r=1024: the
+// ten products 45 us, 1.9 POP/s, the digits 13 us; on the double matrix pipe 182).
+constexpr int DIGITS = 4;
+constexpr int MOST_DIGIT_ROWS = 1 << 16;         // 4 products of 64 x 64 add up below 2^31
+
+// digits[t][row][kp], zeros behind column r, and the powers of two: W's d rows, then A's r; a wave a row
+template <typename S>
+__global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp, const float* __restrict__ W,
+                                                            const S* __restrict__ A, int8_t* __restrict__ digits,
+                                                            double* __restrict__ powers) {
+    const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= d + r) return;
+    // four neighbours (those behind column r - 1 are zeros)
+    auto values = [&](int k, double (&v)[4]) {
+        auto take = [&](const auto* src) {
+            if (k + 4 <= r) {
+                typedef std::remove_cv_t<std::remove_reference_t<decltype(*src)>> V;
+                typedef V V4 __attribute__((ext_vector_type(4), aligned(sizeof(V))));
+                const V4 x = *reinterpret_cast<const V4*>(src + k);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = (double)x[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = k + j < r ? (double)src[k + j] : 0.0;
+            }
+        };
+        if (row < d) take(W + (size_t)row * r);
+        else take(A + (size_t)(row - d) * r);
+    };
+    double most = 0.0;
+    bool fine = true;
+#pragma unroll 4
+    for (int k = lane * 4; k < r; k += 256) {
+        double v[4];
+        values(k, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            fine = fine && fabs(v[j]) <= 1.7976931348623157e308;
+            most = fmax(most, fabs(v[j]));
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
+    fine = __all(fine);
+    int e = 0;
+    (void)frexp(fine ? most : 0.0, &e);               // most < 2^e
+    if (lane == 0) powers[row] = fine ? ldexp(1.0, e + 1) : (double)__int_as_float(0x7fc00000);
+    const double scale = fine ? ldexp(1.0, -e - 1) : 0.0;
+    const size_t plane = (size_t)(d + r) * kp;
+#pragma unroll 2
+    for (int k = lane * 4; k < kp; k += 256) {
+        double v[4];
+        values(k, v);
+        uint32_t word[DIGITS];
+#pragma unroll
+        for (int t = 0; t < DIGITS; ++t) word[t] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            double x = fine ? v[j] * scale : 0.0;
+#pragma unroll
+            for (int t = 0; t < DIGITS; ++t) {
+                x *= 128.0;
+                const double q = rint(x);
+                x -= q;
+                word[t] |= ((uint32_t)(int)q & 0xff) << (8 * j);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < DIGITS; ++t) *reinterpret_cast<uint32_t*>(digits + t * plane + (size_t)row * kp + k) = word[t];
+    }
+}
+
+// A tile of 16 MI WM columns of dW (A's rows are the matrix instruction's rows) and 16 NJ WN rows; 64 of the contraction a
+// step, the next step's digits on their way to LDS, in rows of 64 bytes whose chunks are permuted by (row >> 2) & 3.
+template <int MI, int NJ, int WM, int WN, typename S>
+__global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d, int r, int kp, const int8_t* __restrict__ digits,
+                                                                            const double* __restrict__ powers,
+                                                                            const S* __restrict__ B, float* __restrict__ dW) {
+    constexpr int NW = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN, BLOCKS = DIGITS * (BM + BN) / 16, LOADS = BLOCKS / NW;
+    constexpr int STAGE = BLOCKS * 1024;
+    static_assert(BLOCKS % NW == 0 && BM % 16 == 0, "");
+    extern __shared__ __align__(16) int8_t lds[];      // [2][digit][BM rows of A, BN rows of W][64]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int k0 = blockIdx.x * BM, i0 = blockIdx.y * BN;
+    const int wm = wave % WM * 16 * MI, wn = wave / WM * 16 * NJ;
+    const size_t plane = (size_t)(d + r) * kp;
+    const int8_t* src[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {                  // (rows behind the last one are the last one and not stored)
+        const int block = j * NW + wave, t = block / ((BM + BN) / 16), at = block % ((BM + BN) / 16) * 16 + (lane >> 2);
+        const int row = at < BM ? d + min(k0 + at, r - 1) : min(i0 + at - BM, d - 1);
+        src[j] = digits + t * plane + (size_t)row * kp + ((lane & 3) ^ ((lane >> 4) & 3)) * 16;
+    }
+    auto fetch = [&](int k, int buf) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[j] + k),
+                                             (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (j * NW + wave) * 1024),
+                                             16, 0, 0);
+    };
+    i32x4 acc[DIGITS][MI][NJ];
+#pragma unroll
+    for (int t = 0; t < DIGITS; ++t)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[t][i][j] = i32x4{0, 0, 0, 0};
+    const int op = (lane & 15) * 64 + (((lane >> 4) ^ ((lane >> 2) & 3)) * 16);
+    fetch(0, 0);
+    for (int k = 0, buf = 0; k < kp; k += 64, buf ^= 1) {
+        // (this step's digits have come, all waves are done with the step before, whose place the next one's take)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (k + 64 < kp) fetch(k + 64, buf ^ 1);
+        const int8_t* base = lds + buf * STAGE + op;
+        i32x4 fb[DIGITS][NJ];
+#pragma unroll
+        for (int t = 0; t < DIGITS; ++t)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) fb[t][j] = *reinterpret_cast<const i32x4*>(base + (t * (BM + BN) + BM + wn + 16 * j) * 64);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            i32x4 fa[DIGITS];
+#pragma unroll
+            for (int t = 0; t < DIGITS; ++t) fa[t] = *reinterpret_cast<const i32x4*>(base + (t * (BM + BN) + wm + 16 * i) * 64);
+#pragma unroll
+            for (int t = 0; t < DIGITS; ++t)
+#pragma unroll
+                for (int u = 0; u < DIGITS - t; ++u)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        acc[t + u][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[t], fb[u][j], acc[t + u][i][j], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int i = i0 + wn + 16 * j + (lane & 15);
+        if (i >= d) continue;
+        const double pi = powers[i] * 0x1p-14;
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+            const int k = k0 + wm + 16 * m + 4 * (lane >> 4);
+            f32x4_any out;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                double v = (double)acc[DIGITS - 1][m][j][e];
+#pragma unroll
+                for (int t = DIGITS - 2; t >= 0; --t) v = v * 0x1p-7 + (double)acc[t][m][j][e];
+                const int kk = min(k + e, r - 1);
+                out[e] = (float)(v * pi * powers[d + kk] - (double)B[(size_t)kk * d + i]);
+            }
+            float* dst = dW + (size_t)i * r + k;
+            if (k + 4 <= r) *reinterpret_cast<f32x4_any*>(dst) = out;
+            else
+#pragma unroll
+                for (int e = 0; e < 3; ++e)
+                    if (k + e < r) dst[e] = out[e];
+        }
+    }
+}
+
 // The same gradient by way of the residual, dW = (W H - X) H^T, for up to 128 columns: with n < r / 2 of them it is
 // less work than W (H H^T), and one launch.  A workgroup owns 16 rows.  Its waves share the atoms of W H (double matrix
 // pipe: row l % 16 of W and 16 columns of H at k = 16 s + 4 (l / 16) + j in the j-th instruction, so that a lane
@@ -710,8 +875,35 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
     return ONMF_OK;
 }
 
+// Whole digits take a launch more.  Measured (us of the whole gradient, n=500, digits and the double pipe): d=4096 r=256 27
+// and 27, r=400 38 and 46, r=1024 75 and 178; d=1200 r=600 33 and 34; d=300 r=1024 36 and 34.
+bool by_digits(int d, int r) { return r <= MOST_DIGIT_ROWS && (double)d * r * r > 4e8; }
+int digit_columns(int r) { return (r + 63) & ~63; }
+size_t digits_bytes(int d, int r) {
+    return by_digits(d, r) ? ((size_t)DIGITS * ((size_t)d + r) * digit_columns(r) + 255 & ~(size_t)255) + sizeof(double) * ((size_t)d + r) : 0;
+}
+template <int MI, int NJ, int WM, int WN, typename S>
+int launch_digit_product(onmf_ctx* c, int d, int r, const int8_t* digits, const double* powers, const S* B, float* dW, hipStream_t s) {
+    constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
+    constexpr size_t bytes = 2 * (size_t)DIGITS * (BM + BN) * 64;
+    static LdsLimit lim;
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_digit_product_kernel<MI, NJ, WM, WN, S>, bytes));
+    hipLaunchKernelGGL((keep8_digit_product_kernel<MI, NJ, WM, WN, S>), dim3((r + BM - 1) / BM, (d + BN - 1) / BN), dim3(64 * WM * WN),
+                       bytes, s, d, r, digit_columns(r), digits, powers, B, dW);
+    HIP_TRY(c, hipGetLastError());
+    return ONMF_OK;
+}
 template <typename S>
-int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const S* A, const S* B, float* dW, hipStream_t s) {
+int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const S* A, const S* B, float* dW, char* ws, hipStream_t s) {
+    if (by_digits(d, r)) {
+        int8_t* digits = (int8_t*)ws;
+        double* powers = (double*)(ws + digits_bytes(d, r) - sizeof(double) * ((size_t)d + r));
+        hipLaunchKernelGGL(keep8_digits_kernel<S>, dim3((d + r + 3) / 4), dim3(256), 0, s, d, r, digit_columns(r), W, A, digits, powers);
+        HIP_TRY(c, hipGetLastError());
+        if ((long long)((r + 127) / 128) * ((d + 127) / 128) >= 256)
+            return launch_digit_product<4, 2, 2, 4, S>(c, d, r, digits, powers, B, dW, s);
+        return launch_digit_product<2, 2, 2, 2, S>(c, d, r, digits, powers, B, dW, s);
+    }
     const dim3 grid((r + 31) / 32, (d + 31) / 32);
     // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
     // tiles the double matrix pipe is what counts: d=4096 r=1024 197 us, with eight waves 217)
@@ -743,6 +935,12 @@ int launch_residual(onmf_ctx* c, int d, int r, const float* W, const int8_t* xc,
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
+
+// H H^T and H X^T, and the digits behind them
+size_t both_sums_bytes(const SumPlan& q, int d, int r) {
+    return ((q.splits == 1 ? sizeof(float) : sizeof(double)) * (size_t)r * ((size_t)r + d) + 255) & ~(size_t)255;
+}
+size_t gradient_bytes(const SumPlan& q, int d, int r) { return both_sums_bytes(q, d, r) + digits_bytes(d, r); }
 
 // Groups a thread handles: several where there are enough of them to fill the chip with.
 template <typename T>
@@ -809,7 +1007,7 @@ size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
     if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;
     const SumPlan q = sum_plan(d, r, n);
     if (gradient && by_residual(q, d, r, n)) return 0;
-    return sums_bytes(q, r) + (gradient ? (q.splits == 1 ? sizeof(float) : sizeof(double)) * (size_t)r * ((size_t)r + d) : 0);
+    return sums_bytes(q, r) + (gradient ? gradient_bytes(q, d, r) : 0);
 }
 
 int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes, const float* x_scales,
@@ -854,12 +1052,12 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
         float* A = (float*)ws;
         ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, nullptr, 1.0, 0.0, nullptr, nullptr, A,
                           A + (size_t)r * r, nullptr, nullptr, s));
-        return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, s);
+        return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)ws + both_sums_bytes(q, d, r), s);
     }
     double* A = (double*)((char*)ws + sums_bytes(q, r));
     ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
                       A, A + (size_t)r * r, s));
-    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, s);
+    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)A + both_sums_bytes(q, d, r), s);
 }
 
 }  // extern "C"

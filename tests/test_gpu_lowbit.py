@@ -311,7 +311,8 @@ def whole_columns(eng, rs, d, n, most=15):
 
 SUMS = [(1, 1, 1), (3, 2, 128), (441, 25, 1000), (100, 16, 127), (130, 129, 700), (1200, 100, 1500), (257, 300, 129),
         (64, 1, 5000), (1, 64, 5000), (1024, 256, 2048), (40, 600, 257),
-        (300, 40, 9), (33, 333, 16), (200, 531, 17), (17, 15, 64), (1000, 70, 128), (8300, 20, 100), (8300, 129, 65), (1, 1000, 2)]
+        (300, 40, 9), (33, 333, 16), (200, 531, 17), (17, 15, 64), (1000, 70, 128), (8300, 20, 100), (8300, 129, 65), (1, 1000, 2),
+        (4100, 330, 300), (5000, 1030, 140), (700, 1100, 2000)]        # the last three: W (H H^T) by whole digits
 
 
 @pytest.mark.parametrize("d,r,n", SUMS)
@@ -358,6 +359,34 @@ def test_aggregates_and_gradient_of_real_values(eng, torch, d, r, n):
     W64 = W1.astype(np.float64)
     size = np.abs(W64) @ (np.abs(Hh) @ np.abs(Hh).T) + np.abs(Xh) @ np.abs(Hh).T
     assert (np.abs(g - lo.gradient(W64, Xh, Hh)) <= eps * size).all()
+
+
+def test_gradient_by_digits_row_by_row(eng, torch):
+    """Rows of W of very different size, a zero one and ones that are not finite: each keeps its own precision (2^-26 of its
+    largest entry times the row sum of |A|, as for the sums' float32 runs) and touches no other."""
+    rs = np.random.RandomState(8)
+    d, r, n = 4100, 330, 400
+    X, H = np.maximum(rs.randn(d, n), 0).astype(np.float32), np.maximum(rs.randn(r, n), 0).astype(np.float32)
+    W = rs.randn(d, r).astype(np.float32)
+    W[1] *= 1e-30
+    W[2] *= 1e28
+    W[3] = 0
+    W[4, 7], W[5, 0] = np.nan, np.inf
+    W[6, :-1] *= 1e-5
+    KX, KH = eng.keep8(eng.dev(X)), eng.keep8(eng.dev(H))
+    Xh, Hh = host(KX.expand()), host(KH.expand())
+    g = host(eng.keep8_gradient(eng.dev(W), KX, KH))
+    rest = np.setdiff1d(np.arange(d), [4, 5])
+    assert np.isnan(g[4]).all() and not np.isfinite(g[5]).any()
+    W64, A = W.astype(np.float64)[rest], Hh @ Hh.T
+    want = W64 @ A - (Xh @ Hh.T)[rest]
+    size = np.abs(W64) @ A + (Xh @ Hh.T)[rest]
+    most = np.abs(W64).max(1)[:, None] * A.sum(0)[None, :] + r * np.abs(W64).max(1)[:, None] * A.max(0)[None, :]
+    # sums of four groups in float32 (and the result's rounding), digits cut at 2^-27 on both sides and 2^-28 left out
+    assert (np.abs(g[rest] - want) <= 2.0 ** -24 * (n / 128 + 4) * size + 2.0 ** -26 * most).all()
+    alone = np.zeros((d, r), dtype=np.float32)
+    alone[6] = W[6]
+    assert np.array_equal(host(eng.keep8_gradient(eng.dev(alone), KX, KH))[6], g[6])
 
 
 def test_gradient_is_the_losses_difference(eng, torch):

@@ -240,5 +240,6 @@ def test_workspaces_are_bounded():
     # a slab for each run of groups (512 workgroups of 256 x 128 results at most), and the sums: doubles, with one run floats
     for d, r, n in ((441, 25, 1000), (1024, 256, 65536), (8192, 1024, 129), (60000, 20, 100), (60, 1024, 100)):
         plain, with_gradient = lib.onmf_keep8_workspace(d, r, n, 0), lib.onmf_keep8_workspace(d, r, n, 1)
-        assert with_gradient == plain + (8 if plain else 4) * r * (r + d) and plain <= 512 * 256 * 128 * 4
+        sums, digits = (8 if plain else 4) * r * (r + d), 4 * (d + r) * (r + 63) + 8 * (d + r)
+        assert plain <= 512 * 256 * 128 * 4 and plain + sums <= with_gradient <= plain + sums + 512 + digits
     assert lib.onmf_keep8_workspace(0, 4, 4, 0) == 0
