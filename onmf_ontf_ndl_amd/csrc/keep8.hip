@@ -12,6 +12,8 @@
 #include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2_any __attribute__((ext_vector_type(2), aligned(8)));
 // rows of any length: vectors that need no more alignment than their entries (the memory pipe takes them as they lie)
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
@@ -188,14 +190,16 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 // ------------------------------------------------------------------------------------------- sums
 // Tiles of [H H^T | H X^T], one 128-column group of the contraction a step; a workgroup takes a run of groups and
 // writes its sums to a slab.  int32 inside a group (at most 128 * 127^2), float32 over a workgroup's run, double
-// over the runs.
+// over the runs.  PRECISE, for the gradient: double over a run too, rounded to float32 once where there are several (near
+// a stationary dictionary W (H H^T) and X H^T nearly cancel: with float32 runs d=5295 r=487 n=33000 was off by 5.9e-6 of
+// the gradient, with double ones 8e-7; 15% of the time).
 // Eight waves; a wave owns 16 MI x 16 NJ outputs in 16x16x64 tiles (four of X's scales and one of H's a lane
 // and tile: half the scale reads of the 32x32 shape).  The codes go from memory straight to LDS, two groups ahead,
 // in rows of 128 bytes whose 16-byte chunks are permuted by (row >> 1) & 7, so that the 16 rows of an operand read
 // meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.
 // Per group and output three vector instructions (conversion, product of the scales, fused multiply-add) stand
 // against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not
-// (d=4096 r=256 n=65536, 146 GOP: 125 us; d=1024 40 us).
+// (d=4096 r=256 n=65536, 146 GOP: 125 us, PRECISE 143; d=1024 40 us).
 template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
     static constexpr int mi = MI, nj = NJ, wm = WM_, wn = WN_, stages = STAGES;
     static constexpr int bm = 16 * MI * WM_, bn = 16 * NJ * WN_, waves = WM_ * WN_;
@@ -213,13 +217,14 @@ struct SumParams {
     int d, r, groups, per_split, splits;
     int tiles_m, tiles_h, tiles;     // tiles along r (rows); column tiles of the H H^T part; all tiles
     int cols_h, cols;         // columns of a slab row: the H H^T part's, all (both multiples of 4)
-    // one run holds everything: the results at once
+    // one run holds everything: the results at once, the gradient's as doubles
+    double *Ad, *Bd;
     double w, keep;
     const float *A_in, *B_in;
     float *A, *B;
 };
 
-template <typename S>
+template <typename S, bool PRECISE>
 __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) {
     constexpr int STAGES = S::stages, AHEAD = STAGES - 1, STAGE = S::rows * GROUP;
     extern __shared__ __align__(16) int8_t lds[];            // [STAGES][STAGE], then float [2][S::srows][SG]
@@ -288,10 +293,14 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
     };
 
     f32x4 acc[S::mi][S::nj];
+    f64x4 sums[PRECISE ? S::mi : 1][S::nj];
 #pragma unroll
     for (int i = 0; i < S::mi; ++i)
 #pragma unroll
-        for (int j = 0; j < S::nj; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < S::nj; ++j) {
+            acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (PRECISE) sums[i][j] = f64x4{0.0, 0.0, 0.0, 0.0};
+        }
     // where a lane's operands and scales lie in a stage (whole tiles of 16 rows further on the chunks lie alike)
     const int op0 = (wm + (lane & 15)) * GROUP + (((lane >> 4) ^ ((lane >> 1) & 7)) * 16), op1 = op0 ^ 64;
     const int ba = (S::bm + wn - wm) * GROUP;
@@ -321,32 +330,92 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
         const float* sb = lsc + (k / SG & 1) * SG * S::srows + k % SG + sc_x;
         // (X's rows are the matrix instruction's rows and H's its columns: a lane's four values lie side by side in
         // the slab)
-        i32x4 fa[S::mi][2];
-        float hs[S::mi];
+        if constexpr (PRECISE) {
+            // (X's operands and scales held and H's passed by: what the doubles leave room for)
+            i32x4 fb[S::nj][2];
+            float xs[S::nj][4];
 #pragma unroll
-        for (int i = 0; i < S::mi; ++i) {
-            fa[i][0] = *reinterpret_cast<const i32x4*>(la0 + 16 * i * GROUP);
-            fa[i][1] = *reinterpret_cast<const i32x4*>(la1 + 16 * i * GROUP);
-            hs[i] = sa[SG * 16 * i];
-        }
+            for (int j = 0; j < S::nj; ++j) {
+                fb[j][0] = *reinterpret_cast<const i32x4*>(la0 + ba + 16 * j * GROUP);
+                fb[j][1] = *reinterpret_cast<const i32x4*>(la1 + ba + 16 * j * GROUP);
 #pragma unroll
-        for (int j = 0; j < S::nj; ++j) {
-            const i32x4 fb0 = *reinterpret_cast<const i32x4*>(la0 + ba + 16 * j * GROUP);
-            const i32x4 fb1 = *reinterpret_cast<const i32x4*>(la1 + ba + 16 * j * GROUP);
-            float xs[4];
+                for (int e = 0; e < 4; ++e) xs[j][e] = sb[SG * (16 * j + e)];
+            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) xs[e] = sb[SG * (16 * j + e)];
-            i32x4 part[S::mi];
+            for (int i = 0; i < S::mi; ++i) {
+                const i32x4 fa0 = *reinterpret_cast<const i32x4*>(la0 + 16 * i * GROUP);
+                const i32x4 fa1 = *reinterpret_cast<const i32x4*>(la1 + 16 * i * GROUP);
+                const double hs = (double)sa[SG * 16 * i];
+                i32x4 part[S::nj];
 #pragma unroll
-            for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb0, fa[i][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
+                for (int j = 0; j < S::nj; ++j) part[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j][0], fa0, i32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb1, fa[i][1], part[i], 0, 0, 0);
+                for (int j = 0; j < S::nj; ++j) part[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[j][1], fa1, part[j], 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < S::mi; ++i)
+                for (int j = 0; j < S::nj; ++j) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(xs[e] * hs[i], (float)part[i][e], acc[i][j][e]);
+                    for (int e = 0; e < 4; ++e)
+                        sums[i][j][e] = fma((double)xs[j][e] * hs, (double)part[j][e], sums[i][j][e]);
+                    asm volatile("" : "+v"(sums[i][j]));
+                }
+            }
+        } else {
+            i32x4 fa[S::mi][2];
+            float hs[S::mi];
+#pragma unroll
+            for (int i = 0; i < S::mi; ++i) {
+                fa[i][0] = *reinterpret_cast<const i32x4*>(la0 + 16 * i * GROUP);
+                fa[i][1] = *reinterpret_cast<const i32x4*>(la1 + 16 * i * GROUP);
+                hs[i] = sa[SG * 16 * i];
+            }
+#pragma unroll
+            for (int j = 0; j < S::nj; ++j) {
+                const i32x4 fb0 = *reinterpret_cast<const i32x4*>(la0 + ba + 16 * j * GROUP);
+                const i32x4 fb1 = *reinterpret_cast<const i32x4*>(la1 + ba + 16 * j * GROUP);
+                float xs[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) xs[e] = sb[SG * (16 * j + e)];
+                i32x4 part[S::mi];
+#pragma unroll
+                for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb0, fa[i][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < S::mi; ++i) part[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb1, fa[i][1], part[i], 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < S::mi; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(xs[e] * hs[i], (float)part[i][e], acc[i][j][e]);
+            }
         }
         buf = buf == AHEAD ? 0 : buf + 1;
+    }
+    if constexpr (PRECISE) {
+        if (p.splits == 1) {
+            double* out = is_h ? p.Ad : p.Bd;
+#pragma unroll
+            for (int i = 0; i < S::mi; ++i) {
+                const int m = m0 + wm + 16 * i + (lane & 15);
+                if (m >= p.r) continue;
+#pragma unroll
+                for (int j = 0; j < S::nj; ++j) {
+                    const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
+                    double* dst = out + (size_t)m * N + n;
+                    if (n + 4 <= N) {
+                        reinterpret_cast<f64x2_any*>(dst)[0] = f64x2_any{sums[i][j][0], sums[i][j][1]};
+                        reinterpret_cast<f64x2_any*>(dst)[1] = f64x2_any{sums[i][j][2], sums[i][j][3]};
+                    } else
+#pragma unroll
+                        for (int e = 0; e < 3; ++e)
+                            if (n + e < N) dst[e] = sums[i][j][e];
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < S::mi; ++i)
+#pragma unroll
+            for (int j = 0; j < S::nj; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = (float)sums[i][j][e];
     }
     if (p.splits == 1) {
         const float* in = is_h ? p.A_in : p.B_in;
@@ -443,22 +512,21 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // wave loads the double matrix pipe's operands (16x16x4) straight into registers, the next sixteen while these are
 // computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
 // row 4 e + l / 16.  Bound by the double matrix pipe where r is large (d=4096 r=1024 197 us, 44 TFLOP/s; r=256 19.5).
-typedef double f64x4 __attribute__((ext_vector_type(4)));
-template <int NW, typename S>
+template <int NW>
 __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
-                                                                  const S* __restrict__ A, const S* __restrict__ B,
+                                                                  const double* __restrict__ A, const double* __restrict__ B,
                                                                   float* __restrict__ dW) {
     __shared__ double part[NW][32][32], tb[32][33];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, quad = lane >> 4;
     const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
     for (int e = t; e < 1024; e += 64 * NW) {
         const int k = k0 + (e >> 5), i = i0 + (e & 31);
-        tb[e & 31][e >> 5] = (k < r && i < d) ? (double)B[(size_t)k * d + i] : 0.0;
+        tb[e & 31][e >> 5] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
     }
     // (rows and columns behind the last ones are the last ones and not stored, behind the last j the weight is zero)
     const float* row[2] = {W + (size_t)min(i0 + m, d - 1) * r, W + (size_t)min(i0 + 16 + m, d - 1) * r};
     const int col[2] = {min(k0 + m, r - 1), min(k0 + 16 + m, r - 1)};
-    struct Step { f32x4_any w[2]; S a[4][2]; };
+    struct Step { f32x4_any w[2]; double a[4][2]; };
     auto fetch = [&](int j0, Step& v) {
         const int j = j0 + 4 * quad;
 #pragma unroll
@@ -481,7 +549,7 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
-                    acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v.w[h][i], (double)v.a[i][c], acc[h][c], 0, 0, 0);
+                    acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64((double)v.w[h][i], v.a[i][c], acc[h][c], 0, 0, 0);
     };
     Step even, odd;
     int j0 = wave * 16;
@@ -513,7 +581,7 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
 
 // The same on the 8-bit matrix pipe, where r is large.  Each row of W and of A (which is symmetric) is scaled by a power of
 // two to at most a half and cut into four whole digits of 7 bits, x = sum_t q_t 2^(-7 (t + 1)) within 2^-29, that is
-// 2^-27 of the row's largest entry: an eighth of what the float32 runs of A's sums are off by.  Products of digits add
+// 2^-27 of the row's largest entry: an eighth of what a float32 is off by.  Products of digits add
 // up exactly in int32, those of one weight, t + u = 0..3, in one sum; what is left out (t + u > 3) is 2^-28 and less of
 // the largest.  The four sums, the powers of two and B meet in double.  Bound by the matrix pipe (d=4096 r=1024: the
 // ten products 45 us, 1.9 POP/s, the digits 13 us; on the double matrix pipe 182).
@@ -521,9 +589,8 @@ constexpr int DIGITS = 4;
 constexpr int MOST_DIGIT_ROWS = 1 << 16;         // 4 products of 64 x 64 add up below 2^31
 
 // digits[t][row][kp], zeros behind column r, and the powers of two: W's d rows, then A's r; a wave a row
-template <typename S>
 __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp, const float* __restrict__ W,
-                                                            const S* __restrict__ A, int8_t* __restrict__ digits,
+                                                            const double* __restrict__ A, int8_t* __restrict__ digits,
                                                             double* __restrict__ powers) {
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= d + r) return;
@@ -589,10 +656,10 @@ __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp,
 
 // A tile of 16 MI WM columns of dW (A's rows are the matrix instruction's rows) and 16 NJ WN rows; 64 of the contraction a
 // step, the next step's digits on their way to LDS, in rows of 64 bytes whose chunks are permuted by (row >> 2) & 3.
-template <int MI, int NJ, int WM, int WN, typename S>
+template <int MI, int NJ, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d, int r, int kp, const int8_t* __restrict__ digits,
                                                                             const double* __restrict__ powers,
-                                                                            const S* __restrict__ B, float* __restrict__ dW) {
+                                                                            const double* __restrict__ B, float* __restrict__ dW) {
     constexpr int NW = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN, BLOCKS = DIGITS * (BM + BN) / 16, LOADS = BLOCKS / NW;
     constexpr int STAGE = BLOCKS * 1024;
     static_assert(BLOCKS % NW == 0 && BM % 16 == 0, "");
@@ -663,7 +730,7 @@ __global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d
 #pragma unroll
                 for (int t = DIGITS - 2; t >= 0; --t) v = v * 0x1p-7 + (double)acc[t][m][j][e];
                 const int kk = min(k + e, r - 1);
-                out[e] = (float)(v * pi * powers[d + kk] - (double)B[(size_t)kk * d + i]);
+                out[e] = (float)(v * pi * powers[d + kk] - B[(size_t)kk * d + i]);
             }
             float* dst = dW + (size_t)i * r + k;
             if (k + 4 <= r) *reinterpret_cast<f32x4_any*>(dst) = out;
@@ -835,15 +902,25 @@ int check8(onmf_ctx* c, const char* what, int d, int n, const void* codes, const
     return ONMF_OK;
 }
 
-template <typename S>
+template <typename S, bool PRECISE>
 int launch_sums(onmf_ctx* c, const SumParams& p, hipStream_t s) {
     constexpr size_t bytes = S::stages * (size_t)S::rows * GROUP + 2 * (size_t)S::srows * S::sg * sizeof(float);
     static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
     static LdsLimit lim;
-    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_sums_kernel<S>, bytes));
-    hipLaunchKernelGGL(keep8_sums_kernel<S>, dim3((p.tiles * p.splits + 7) / 8 * 8), dim3(64 * S::waves), bytes, s, p);
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_sums_kernel<S, PRECISE>, bytes));
+    hipLaunchKernelGGL((keep8_sums_kernel<S, PRECISE>), dim3((p.tiles * p.splits + 7) / 8 * 8), dim3(64 * S::waves), bytes, s, p);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
+}
+
+template <bool PRECISE>
+int launch_tile(onmf_ctx* c, int tile, const SumParams& p, hipStream_t s) {
+    switch (tile) {
+        case 0: return launch_sums<Slim, PRECISE>(c, p, s);
+        case 1: return launch_sums<Narrow, PRECISE>(c, p, s);
+        case 2: return launch_sums<Middle, PRECISE>(c, p, s);
+        default: return launch_sums<Wide, PRECISE>(c, p, s);
+    }
 }
 
 // The sums of a minibatch into A and B, or as doubles into Ad and Bd.
@@ -856,12 +933,8 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
     p.tiles_m = q.tiles_m; p.tiles_h = q.tiles_h; p.tiles = q.tiles_m * (q.tiles_h + q.tiles_x);
     p.cols_h = q.cols_h; p.cols = q.cols;
     p.w = w; p.keep = keep; p.A_in = A_in; p.B_in = B_in; p.A = A; p.B = B;
-    switch (q.tile) {
-        case 0: ONMF_TRY(launch_sums<Slim>(c, p, s)); break;
-        case 1: ONMF_TRY(launch_sums<Narrow>(c, p, s)); break;
-        case 2: ONMF_TRY(launch_sums<Middle>(c, p, s)); break;
-        default: ONMF_TRY(launch_sums<Wide>(c, p, s)); break;
-    }
+    p.Ad = Ad; p.Bd = Bd;
+    ONMF_TRY(Ad ? launch_tile<true>(c, q.tile, p, s) : launch_tile<false>(c, q.tile, p, s));
     if (q.splits == 1) return ONMF_OK;
     // (few entries with many slabs: more threads to an entry)
     const size_t quads = (size_t)r * q.cols / 4;
@@ -882,35 +955,34 @@ int digit_columns(int r) { return (r + 63) & ~63; }
 size_t digits_bytes(int d, int r) {
     return by_digits(d, r) ? ((size_t)DIGITS * ((size_t)d + r) * digit_columns(r) + 255 & ~(size_t)255) + sizeof(double) * ((size_t)d + r) : 0;
 }
-template <int MI, int NJ, int WM, int WN, typename S>
-int launch_digit_product(onmf_ctx* c, int d, int r, const int8_t* digits, const double* powers, const S* B, float* dW, hipStream_t s) {
+template <int MI, int NJ, int WM, int WN>
+int launch_digit_product(onmf_ctx* c, int d, int r, const int8_t* digits, const double* powers, const double* B, float* dW, hipStream_t s) {
     constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
     constexpr size_t bytes = 2 * (size_t)DIGITS * (BM + BN) * 64;
     static LdsLimit lim;
-    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_digit_product_kernel<MI, NJ, WM, WN, S>, bytes));
-    hipLaunchKernelGGL((keep8_digit_product_kernel<MI, NJ, WM, WN, S>), dim3((r + BM - 1) / BM, (d + BN - 1) / BN), dim3(64 * WM * WN),
+    ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_digit_product_kernel<MI, NJ, WM, WN>, bytes));
+    hipLaunchKernelGGL((keep8_digit_product_kernel<MI, NJ, WM, WN>), dim3((r + BM - 1) / BM, (d + BN - 1) / BN), dim3(64 * WM * WN),
                        bytes, s, d, r, digit_columns(r), digits, powers, B, dW);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
-template <typename S>
-int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const S* A, const S* B, float* dW, char* ws, hipStream_t s) {
+int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const double* A, const double* B, float* dW, char* ws, hipStream_t s) {
     if (by_digits(d, r)) {
         int8_t* digits = (int8_t*)ws;
         double* powers = (double*)(ws + digits_bytes(d, r) - sizeof(double) * ((size_t)d + r));
-        hipLaunchKernelGGL(keep8_digits_kernel<S>, dim3((d + r + 3) / 4), dim3(256), 0, s, d, r, digit_columns(r), W, A, digits, powers);
+        hipLaunchKernelGGL(keep8_digits_kernel, dim3((d + r + 3) / 4), dim3(256), 0, s, d, r, digit_columns(r), W, A, digits, powers);
         HIP_TRY(c, hipGetLastError());
         if ((long long)((r + 127) / 128) * ((d + 127) / 128) >= 256)
-            return launch_digit_product<4, 2, 2, 4, S>(c, d, r, digits, powers, B, dW, s);
-        return launch_digit_product<2, 2, 2, 2, S>(c, d, r, digits, powers, B, dW, s);
+            return launch_digit_product<4, 2, 2, 4>(c, d, r, digits, powers, B, dW, s);
+        return launch_digit_product<2, 2, 2, 2>(c, d, r, digits, powers, B, dW, s);
     }
     const dim3 grid((r + 31) / 32, (d + 31) / 32);
     // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
     // tiles the double matrix pipe is what counts: d=4096 r=1024 197 us, with eight waves 217)
     if (r > 64 && (size_t)grid.x * grid.y <= 512)
-        hipLaunchKernelGGL((keep8_gradient_kernel<8, S>), grid, dim3(512), 0, s, d, r, W, A, B, dW);
+        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, A, B, dW);
     else
-        hipLaunchKernelGGL((keep8_gradient_kernel<4, S>), grid, dim3(256), 0, s, d, r, W, A, B, dW);
+        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, A, B, dW);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -937,10 +1009,10 @@ int launch_residual(onmf_ctx* c, int d, int r, const float* W, const int8_t* xc,
 }
 
 // H H^T and H X^T, and the digits behind them
-size_t both_sums_bytes(const SumPlan& q, int d, int r) {
-    return ((q.splits == 1 ? sizeof(float) : sizeof(double)) * (size_t)r * ((size_t)r + d) + 255) & ~(size_t)255;
+size_t both_sums_bytes(int d, int r) {
+    return (sizeof(double) * (size_t)r * ((size_t)r + d) + 255) & ~(size_t)255;
 }
-size_t gradient_bytes(const SumPlan& q, int d, int r) { return both_sums_bytes(q, d, r) + digits_bytes(d, r); }
+size_t gradient_bytes(int d, int r) { return both_sums_bytes(d, r) + digits_bytes(d, r); }
 
 // Groups a thread handles: several where there are enough of them to fill the chip with.
 template <typename T>
@@ -1007,7 +1079,7 @@ size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
     if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;
     const SumPlan q = sum_plan(d, r, n);
     if (gradient && by_residual(q, d, r, n)) return 0;
-    return sums_bytes(q, r) + (gradient ? gradient_bytes(q, d, r) : 0);
+    return sums_bytes(q, r) + (gradient ? gradient_bytes(d, r) : 0);
 }
 
 int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes, const float* x_scales,
@@ -1048,16 +1120,10 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
         if (n <= 64) return launch_residual<4, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
         return launch_residual<8, 8>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
     }
-    if (q.splits == 1) {                    // (sums of one run are float32 values)
-        float* A = (float*)ws;
-        ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, nullptr, 1.0, 0.0, nullptr, nullptr, A,
-                          A + (size_t)r * r, nullptr, nullptr, s));
-        return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)ws + both_sums_bytes(q, d, r), s);
-    }
     double* A = (double*)((char*)ws + sums_bytes(q, r));
     ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
                       A, A + (size_t)r * r, s));
-    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)A + both_sums_bytes(q, d, r), s);
+    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)A + both_sums_bytes(d, r), s);
 }
 
 }  // extern "C"

@@ -237,9 +237,9 @@ def test_workspaces_are_bounded():
         assert lib.onmf_dict4_workspace(which, 4, 4, 4, 48) == 0
     for d, r, n in ((441, 25, 128), (8192, 1024, 1), (4096, 300, 100)):     # by way of the residual: none
         assert lib.onmf_keep8_workspace(d, r, n, 1) == 0
-    # a slab for each run of groups (512 workgroups of 256 x 128 results at most), and the sums: doubles, with one run floats
+    # a slab for each run of groups (512 workgroups of 256 x 128 results at most), and the sums as doubles
     for d, r, n in ((441, 25, 1000), (1024, 256, 65536), (8192, 1024, 129), (60000, 20, 100), (60, 1024, 100)):
         plain, with_gradient = lib.onmf_keep8_workspace(d, r, n, 0), lib.onmf_keep8_workspace(d, r, n, 1)
-        sums, digits = (8 if plain else 4) * r * (r + d), 4 * (d + r) * (r + 63) + 8 * (d + r)
+        sums, digits = 8 * r * (r + d), 4 * (d + r) * (r + 63) + 8 * (d + r)
         assert plain <= 512 * 256 * 128 * 4 and plain + sums <= with_gradient <= plain + sums + 512 + digits
     assert lib.onmf_keep8_workspace(0, 4, 4, 0) == 0
