@@ -511,7 +511,7 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // nearly cancel.  A workgroup owns a 32 x 32 tile, its NW waves share the sum over j in sixteens and add up in LDS.  A
 // wave loads the double matrix pipe's operands (16x16x4) straight into registers, the next sixteen while these are
 // computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
-// row 4 e + l / 16.  Bound by the double matrix pipe where r is large (d=4096 r=1024 197 us, 44 TFLOP/s; r=256 19.5).
+// row 4 e + l / 16.  Bound by the double matrix pipe where r is large (d=4096 r=256 19.5 us; r=1024 182, 47 TFLOP/s).
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
                                                                   const double* __restrict__ A, const double* __restrict__ B,
@@ -978,7 +978,7 @@ int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const double* A, 
     }
     const dim3 grid((r + 31) / 32, (d + 31) / 32);
     // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
-    // tiles the double matrix pipe is what counts: d=4096 r=1024 197 us, with eight waves 217)
+    // tiles the double matrix pipe is what counts: d=8192 r=256 36 us, with eight waves 42)
     if (r > 64 && (size_t)grid.x * grid.y <= 512)
         hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, A, B, dW);
     else
