@@ -1,10 +1,10 @@
 // Columns held in 8 bits and what the dictionary's update needs of them, on gfx950.
 //
 // Format: 128 consecutive columns of a row share a scale s = max |v| / 127 (float32, by the reciprocal of 127, as float
-// arrays are divided by a number on the GPU); an entry stands for s q, q = rint(v / s) in -127..127.  codes is [row][padded columns] int8 (rows padded to whole groups with zeros),
-// scales [row][group].  A minibatch X and its code H put away this way take a quarter of their room, and the
-// sums H H^T and H X^T - the gradient to the dictionary is W (H H^T) - X H^T - run on the 8-bit matrix pipe:
-// inside a group the products of whole numbers add up exactly in int32.
+// arrays are divided by a number on the GPU); an entry stands for s q, q = rint(v / s) in -127..127.  codes is
+// [row][padded columns] int8 (rows padded to whole groups with zeros), scales [row][group].  A minibatch X and its code H
+// put away this way take a quarter of their room, and the sums H H^T and H X^T - the gradient to the dictionary is
+// W (H H^T) - X H^T - run on the 8-bit matrix pipe: inside a group the products of whole numbers add up exactly in int32.
 #include "common.h"
 
 #include <algorithm>
@@ -192,8 +192,8 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 // writes its sums to a slab.  int32 inside a group (at most 128 * 127^2), float32 over a workgroup's run, double
 // over the runs.  PRECISE, for the gradient: double over a run too, rounded to float32 once where there are several (near
 // a stationary dictionary W (H H^T) and X H^T nearly cancel: with float32 runs d=5295 r=487 n=33000 was off by 5.9e-6 of
-// the gradient, with double ones 8e-7; 15% of the time).
-// Eight waves; a wave owns 16 MI x 16 NJ outputs in 16x16x64 tiles (four of X's scales and one of H's a lane
+// the gradient, with double ones by 8e-7, for 15% more time).
+// A wave owns 16 MI x 16 NJ outputs in 16x16x64 tiles (four of X's scales and one of H's a lane
 // and tile: half the scale reads of the 32x32 shape).  The codes go from memory straight to LDS, two groups ahead,
 // in rows of 128 bytes whose 16-byte chunks are permuted by (row >> 1) & 7, so that the 16 rows of an operand read
 // meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.

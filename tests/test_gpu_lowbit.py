@@ -485,6 +485,35 @@ def test_results_are_the_same_every_time_and_on_two_streams_at_once(eng, torch):
             assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
 
 
+def test_calls_from_several_threads(eng, torch):
+    """The operators take nothing from the engine's context but its device: threads with streams of their own may call at
+    once."""
+    import threading
+    states = [state(eng, 10 + i) for i in range(4)]
+    want = [every_operator(eng, *s) for s in states]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got = every_operator(eng, *states[i])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        wrong.append(i)
+        except Exception as e:                                  # (a thread's exception would be lost)
+            wrong.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong, wrong
+
+
 def test_captured_calls_replay(eng, torch):
     """Two graphs of the same calls, replayed in turn with new inputs, eager work and synchronizations in between."""
     s = state(eng, 5)
