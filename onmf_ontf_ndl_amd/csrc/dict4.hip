@@ -1452,6 +1452,7 @@ extern "C" {
 
 size_t onmf_dict4_workspace(int which, int d, int r, int b, int group) {
     if (d <= 0 || r <= 0 || b <= 0 || (group != 32 && group != 64 && group != 128)) return 0;
+    if (d > (1 << 18) || r > MOST_COLS || b > MOST_COLS) return 0;              // sizes that the calls refuse
     size_t need = 0;                                    // enough for either type of the columns
     for (const bool wide : {false, true}) need = std::max(need, workspace_of(which == ONMF_DICT4_PRODUCT, d, r, b, group, wide));
     return need;

@@ -23,6 +23,7 @@ namespace {
 constexpr int GROUP = 128;
 constexpr size_t MOST_GROUPS = ((size_t)1 << 29) - 32;      // eight threads a group, fewer than 2^32 in a launch
 constexpr int MOST_COLS = 1 << 28;       // eight rows' codes lie within 32 bits
+constexpr int MOST_ROWS = 2147483647 - 1024;    // tile arithmetic in int
 
 __device__ __forceinline__ float bf16_to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ float load_val(const float* p) { return *p; }
@@ -899,6 +900,7 @@ int check8(onmf_ctx* c, const char* what, int d, int n, const void* codes, const
     if (d <= 0 || n <= 0 || !codes || !scales || ((uintptr_t)codes & 15) || ((uintptr_t)scales & 3))
         return onmf_fail(c, ONMF_ERR_ARG, "%s: bad arguments (d=%d n=%d; codes must be aligned to 16 bytes)", what, d, n);
     if (n > MOST_COLS) return onmf_fail(c, ONMF_ERR_ARG, "%s: n=%d is more than 2^28 columns", what, n);
+    if (d > MOST_ROWS) return onmf_fail(c, ONMF_ERR_ARG, "%s: %d rows are more than the kernels' int counts", what, d);
     return ONMF_OK;
 }
 
@@ -1076,7 +1078,8 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
 }
 
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
-    if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;
+    if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;                  // sizes that the calls refuse
+    if (d > MOST_ROWS || r > MOST_ROWS || (gradient && (d > (1 << 18) || r > (1 << 18)))) return 0;
     const SumPlan q = sum_plan(d, r, n);
     if (gradient && by_residual(q, d, r, n)) return 0;
     return sums_bytes(q, r) + (gradient ? gradient_bytes(d, r) : 0);

@@ -243,3 +243,20 @@ def test_workspaces_are_bounded():
         sums, digits = 8 * r * (r + d), 4 * (d + r) * (r + 63) + 8 * (d + r)
         assert plain <= 512 * 256 * 128 * 4 and plain + sums <= with_gradient <= plain + sums + 512 + digits
     assert lib.onmf_keep8_workspace(0, 4, 4, 0) == 0
+
+
+def test_workspaces_of_sizes_that_the_calls_refuse():
+    """The largest ints go through no arithmetic that could overflow."""
+    lib = _lib.load()
+    large = 2 ** 31 - 1
+    for which in (0, 1):
+        assert lib.onmf_dict4_workspace(which, 2 ** 18 + 1, 64, 64, 64) == 0
+        assert lib.onmf_dict4_workspace(which, 64, large, 64, 64) == 0
+        assert lib.onmf_dict4_workspace(which, 64, 64, large, 64) == 0
+        assert lib.onmf_keep8_workspace(large, 64, 4096, which) == 0
+        assert lib.onmf_keep8_workspace(64, large, 4096, which) == 0
+        assert lib.onmf_keep8_workspace(64, 64, 2 ** 28 + 1, which) == 0
+        assert 0 < lib.onmf_dict4_workspace(which, 2 ** 18, 2 ** 18, 2 ** 18, 32) < 2 ** 62
+        # (sums of one run go straight to A and B: no workspace)
+        assert (which == 1) <= lib.onmf_keep8_workspace(2 ** 18, 2 ** 18, 2 ** 28, which) < 2 ** 62
+    assert lib.onmf_keep8_workspace(2 ** 18 + 1, 64, 4096, 1) == 0 and lib.onmf_keep8_workspace(64, 2 ** 18 + 1, 4096, 1) == 0
