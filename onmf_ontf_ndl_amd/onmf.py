@@ -178,7 +178,7 @@ class Online_NMF():
         eng = self._engine()
         like_torch = self._torch_io
         kept = isinstance(self.X, KeptColumns) and self.subsample     # minibatches are brought back one by one
-        if self._X_dev is None or (isinstance(self._X_dev, KeptColumns) and not kept):
+        if self._X_dev is None or (isinstance(self.X, KeptColumns) and isinstance(self._X_dev, KeptColumns) != kept):
             self._X_dev = self.X if kept else _columns_dev(eng, self.X)
         Xd = self._X_dev
         d, n = Xd.shape
