@@ -13,6 +13,7 @@
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 typedef double f64x2_any __attribute__((ext_vector_type(2), aligned(8)));
 // rows of any length: vectors that need no more alignment than their entries (the memory pipe takes them as they lie)
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
@@ -191,16 +192,15 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 // ------------------------------------------------------------------------------------------- sums
 // Tiles of [H H^T | H X^T], one 128-column group of the contraction a step; a workgroup takes a run of groups and
 // writes its sums to a slab.  int32 inside a group (at most 128 * 127^2), float32 over a workgroup's run, double
-// over the runs.  PRECISE, for the gradient: double over a run too, rounded to float32 once where there are several (near
-// a stationary dictionary W (H H^T) and X H^T nearly cancel: with float32 runs d=5295 r=487 n=33000 was off by 5.9e-6 of
-// the gradient, with double ones by 8e-7, for 15% more time).
+// over the runs.  PRECISE, for the gradient: double over a run too and in its slab (near a stationary dictionary W (H H^T)
+// and X H^T nearly cancel: what is rounded to float32 on the way, a run's sums included, is as large as the gradient).
 // A wave owns 16 MI x 16 NJ outputs in 16x16x64 tiles (four of X's scales and one of H's a lane
 // and tile: half the scale reads of the 32x32 shape).  The codes go from memory straight to LDS, two groups ahead,
 // in rows of 128 bytes whose 16-byte chunks are permuted by (row >> 1) & 7, so that the 16 rows of an operand read
 // meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.
 // Per group and output three vector instructions (conversion, product of the scales, fused multiply-add) stand
 // against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not
-// (d=4096 r=256 n=65536, 146 GOP: 125 us, PRECISE 143; d=1024 40 us).
+// (d=4096 r=256 n=65536, 146 GOP: 125 us, PRECISE 145 and the slabs' 62 MB; d=1024 40 us).
 template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
     static constexpr int mi = MI, nj = NJ, wm = WM_, wn = WN_, stages = STAGES;
     static constexpr int bm = 16 * MI * WM_, bn = 16 * NJ * WN_, waves = WM_ * WN_;
@@ -214,7 +214,7 @@ template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
 struct SumParams {
     const int8_t *hc, *xc;
     const float *hs, *xs;
-    float* slab;              // [split][r][cols]
+    void* slab;               // [split][r][cols], floats; PRECISE: doubles
     int d, r, groups, per_split, splits;
     int tiles_m, tiles_h, tiles;     // tiles along r (rows); column tiles of the H H^T part; all tiles
     int cols_h, cols;         // columns of a slab row: the H H^T part's, all (both multiples of 4)
@@ -293,15 +293,13 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
                                              4, 0, 0);
     };
 
-    f32x4 acc[S::mi][S::nj];
-    f64x4 sums[PRECISE ? S::mi : 1][S::nj];
+    typedef std::conditional_t<PRECISE, double, float> V;
+    typedef V V4 __attribute__((ext_vector_type(4)));
+    V4 acc[S::mi][S::nj];
 #pragma unroll
     for (int i = 0; i < S::mi; ++i)
 #pragma unroll
-        for (int j = 0; j < S::nj; ++j) {
-            acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            if constexpr (PRECISE) sums[i][j] = f64x4{0.0, 0.0, 0.0, 0.0};
-        }
+        for (int j = 0; j < S::nj; ++j) acc[i][j] = V4{0, 0, 0, 0};
     // where a lane's operands and scales lie in a stage (whole tiles of 16 rows further on the chunks lie alike)
     const int op0 = (wm + (lane & 15)) * GROUP + (((lane >> 4) ^ ((lane >> 1) & 7)) * 16), op1 = op0 ^ 64;
     const int ba = (S::bm + wn - wm) * GROUP;
@@ -356,8 +354,8 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
                 for (int j = 0; j < S::nj; ++j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        sums[i][j][e] = fma((double)xs[j][e] * hs, (double)part[j][e], sums[i][j][e]);
-                    asm volatile("" : "+v"(sums[i][j]));
+                        acc[i][j][e] = fma((double)xs[j][e] * hs, (double)part[j][e], acc[i][j][e]);
+                    asm volatile("" : "+v"(acc[i][j]));
                 }
             }
         } else {
@@ -389,35 +387,6 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
         }
         buf = buf == AHEAD ? 0 : buf + 1;
     }
-    if constexpr (PRECISE) {
-        if (p.splits == 1) {
-            double* out = is_h ? p.Ad : p.Bd;
-#pragma unroll
-            for (int i = 0; i < S::mi; ++i) {
-                const int m = m0 + wm + 16 * i + (lane & 15);
-                if (m >= p.r) continue;
-#pragma unroll
-                for (int j = 0; j < S::nj; ++j) {
-                    const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
-                    double* dst = out + (size_t)m * N + n;
-                    if (n + 4 <= N) {
-                        reinterpret_cast<f64x2_any*>(dst)[0] = f64x2_any{sums[i][j][0], sums[i][j][1]};
-                        reinterpret_cast<f64x2_any*>(dst)[1] = f64x2_any{sums[i][j][2], sums[i][j][3]};
-                    } else
-#pragma unroll
-                        for (int e = 0; e < 3; ++e)
-                            if (n + e < N) dst[e] = sums[i][j][e];
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < S::mi; ++i)
-#pragma unroll
-            for (int j = 0; j < S::nj; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] = (float)sums[i][j][e];
-    }
     if (p.splits == 1) {
         const float* in = is_h ? p.A_in : p.B_in;
         float* out = is_h ? p.A : p.B;
@@ -429,24 +398,33 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
             for (int j = 0; j < S::nj; ++j) {
                 const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
                 const size_t at = (size_t)m * N + n;
-                if (n + 3 < N) {
+                if constexpr (PRECISE) {
+                    double* dst = (is_h ? p.Ad : p.Bd) + at;
+                    if (n + 4 <= N) {
+                        reinterpret_cast<f64x2_any*>(dst)[0] = f64x2_any{acc[i][j][0], acc[i][j][1]};
+                        reinterpret_cast<f64x2_any*>(dst)[1] = f64x2_any{acc[i][j][2], acc[i][j][3]};
+                    } else
+#pragma unroll
+                        for (int e = 0; e < 3; ++e)
+                            if (n + e < N) dst[e] = acc[i][j][e];
+                } else if (n + 3 < N) {
                     f32x4_any v = {0.f, 0.f, 0.f, 0.f};
                     if (in) v = *reinterpret_cast<const f32x4_any*>(in + at);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = (float)(p.w * (double)acc[i][j][e] + p.keep * (double)v[e]);
                     *reinterpret_cast<f32x4_any*>(out + at) = v;
-                    continue;
-                }
+                } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (n + e >= N) continue;
-                    out[at + e] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at + e] : 0.0));
+                    for (int e = 0; e < 4; ++e) {
+                        if (n + e >= N) continue;
+                        out[at + e] = (float)(p.w * (double)acc[i][j][e] + (in ? p.keep * (double)in[at + e] : 0.0));
+                    }
                 }
             }
         }
         return;
     }
-    float* out = p.slab + (size_t)split * p.r * p.cols + (is_h ? 0 : p.cols_h);
+    V* out = (V*)p.slab + (size_t)split * p.r * p.cols + (is_h ? 0 : p.cols_h);
 #pragma unroll
     for (int i = 0; i < S::mi; ++i) {
         const int m = m0 + wm + 16 * i + (lane & 15);
@@ -454,8 +432,14 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
 #pragma unroll
         for (int j = 0; j < S::nj; ++j) {
             const int n = n0 + wn + 16 * j + 4 * (lane >> 4);
-            // (rows of the slab are padded to whole quads)
-            if (n < N) *reinterpret_cast<f32x4*>(out + (size_t)m * p.cols + n) = acc[i][j];
+            if (n >= N) continue;                        // (rows of the slab are padded to whole quads)
+            V* dst = out + (size_t)m * p.cols + n;
+            if constexpr (PRECISE) {
+                reinterpret_cast<f64x2*>(dst)[0] = f64x2{acc[i][j][0], acc[i][j][1]};
+                reinterpret_cast<f64x2*>(dst)[1] = f64x2{acc[i][j][2], acc[i][j][3]};
+            } else {
+                *reinterpret_cast<f32x4*>(dst) = acc[i][j];
+            }
         }
     }
 }
@@ -471,12 +455,22 @@ __device__ __forceinline__ void sum_slabs(const float* src, size_t stride, int s
         s[0] += (double)v.x; s[1] += (double)v.y; s[2] += (double)v.z; s[3] += (double)v.w;
     }
 }
-
-// A = keep A_in + w sum, B = keep B_in + w sum; with Ad and Bd (the gradient) the sums themselves, as doubles.  Bound by
-// reading the slabs (d=4096 r=256 n=65536 8.7 us).
 template <int ZL>
+__device__ __forceinline__ void sum_slabs(const double* src, size_t stride, int splits, int z0, double (&s)[4]) {
+    s[0] = s[1] = s[2] = s[3] = 0.0;
+#pragma unroll 4
+    for (int z = z0; z < splits; z += ZL) {
+        const f64x2* at = reinterpret_cast<const f64x2*>(src + (size_t)z * stride);
+        const f64x2 v = at[0], u = at[1];
+        s[0] += v.x; s[1] += v.y; s[2] += u.x; s[3] += u.y;
+    }
+}
+
+// A = keep A_in + w sum, B = keep B_in + w sum; from slabs of doubles (the gradient) the sums themselves to Ad and Bd.  Bound
+// by reading the slabs (d=4096 r=256 n=65536 8.7 us, doubles 12.5).
+template <int ZL, typename V>
 __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int cols_h, int cols, int splits,
-                                                            const float* __restrict__ slab, double w, double keep,
+                                                            const V* __restrict__ slab, double w, double keep,
                                                             const float* A_in, const float* B_in, float* A, float* B,
                                                             double* __restrict__ Ad, double* __restrict__ Bd) {
     constexpr int Q = 256 / ZL;
@@ -503,7 +497,7 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 #pragma unroll
         for (int z = 1; z < ZL; ++z) v += part[z][q][j];
         const size_t at = (size_t)k * N + n0 + j;
-        if (Ad) (is_h ? Ad : Bd)[at] = v;
+        if constexpr (sizeof(V) == 8) (is_h ? Ad : Bd)[at] = v;
         else out[at] = (float)(w * v + (in ? keep * (double)in[at] : 0.0));
     }
 }
@@ -856,7 +850,10 @@ struct SumPlan { int tile, bm, bn, tiles_m, tiles_h, tiles_x, cols_h, cols, spli
 // 8 TB/s - and, with several runs, a second launch and the slabs' way through memory at 4 TB/s.  One workgroup a CU.
 // (us: d=8192 r=64 n=1000 64 x 256 13.2, 32 x 128 6.4; d=8192 r=256 n=1000 256 x 128 20, 64 x 256 12; d=4096 r=256
 // n=65536 256 x 128 125, 64 x 256 180; d=1200 r=100 n=8191 in runs of four groups 17.3, of two 20.3.)
-SumPlan sum_plan(int d, int r, int n) {
+// Sums in double (the gradient's): a group that waits for no codes takes a third more (27 groups in 64 x 256 37 us), and an
+// entry of a slab a quarter (whole gradient, us: d=290 r=876 n=3335 in one run 59.6, in three 49.9; d=4096 r=256 n=65536
+// 256 x 128 176, 128 x 256 178; d=1024 66 and 66).
+SumPlan sum_plan(int d, int r, int n, bool precise) {
     static constexpr struct { int bm, bn, rows; double own, group; } kind[4] = {{Slim::bm, Slim::bn, Slim::rows, 2.4, 0.5},
                                                                                  {Narrow::bm, Narrow::bn, Narrow::rows, 5.0, 0.87},
                                                                                  {Middle::bm, Middle::bn, Middle::rows, 7.0, 1.25},
@@ -876,8 +873,9 @@ SumPlan sum_plan(int d, int r, int n) {
             const int per = (groups + want - 1) / want, splits = (groups + per - 1) / per;
             const double w = tiles * splits;
             double cost = std::ceil(w / 256) *
-                          (kind[i].own + per * std::max(kind[i].group, kind[i].rows * (double)GROUP * std::min(w, 256.0) / 8e6));
-            if (splits > 1) cost += 5.0 + 2e-6 * splits * r * q.cols;
+                          (kind[i].own + per * std::max(kind[i].group * (precise ? 1.35 : 1.0),
+                                                        kind[i].rows * (double)GROUP * std::min(w, 256.0) / 8e6));
+            if (splits > 1) cost += 5.0 + (precise ? 2.5e-6 : 2e-6) * splits * r * q.cols;
             if (best >= 0 && cost >= best) continue;
             best = q.cost = cost;
             q.tile = i;
@@ -892,8 +890,8 @@ SumPlan sum_plan(int d, int r, int n) {
     }
     return q;
 }
-size_t sums_bytes(const SumPlan& q, int r) {
-    return q.splits == 1 ? 0 : ((size_t)q.splits * r * q.cols * sizeof(float) + 255) & ~(size_t)255;
+size_t sums_bytes(const SumPlan& q, int r, bool precise) {
+    return q.splits == 1 ? 0 : ((size_t)q.splits * r * q.cols * (precise ? sizeof(double) : sizeof(float)) + 255) & ~(size_t)255;
 }
 
 int check8(onmf_ctx* c, const char* what, int d, int n, const void* codes, const void* scales) {
@@ -927,7 +925,7 @@ int launch_tile(onmf_ctx* c, int tile, const SumParams& p, hipStream_t s) {
 
 // The sums of a minibatch into A and B, or as doubles into Ad and Bd.
 int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* xc, const float* xs, const int8_t* hc, const float* hs,
-             float* slab, double w, double keep, const float* A_in, const float* B_in, float* A, float* B, double* Ad,
+             void* slab, double w, double keep, const float* A_in, const float* B_in, float* A, float* B, double* Ad,
              double* Bd, hipStream_t s) {
     SumParams p;
     p.hc = hc; p.xc = xc; p.hs = hs; p.xs = xs; p.slab = slab;
@@ -940,12 +938,14 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
     if (q.splits == 1) return ONMF_OK;
     // (few entries with many slabs: more threads to an entry)
     const size_t quads = (size_t)r * q.cols / 4;
-    if (quads < 16384)
-        hipLaunchKernelGGL(keep8_reduce_kernel<16>, dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, s, d, r, q.cols_h, q.cols,
-                           q.splits, slab, w, keep, A_in, B_in, A, B, Ad, Bd);
-    else
-        hipLaunchKernelGGL(keep8_reduce_kernel<4>, dim3((unsigned)((quads + 63) / 64)), dim3(256), 0, s, d, r, q.cols_h, q.cols,
-                           q.splits, slab, w, keep, A_in, B_in, A, B, Ad, Bd);
+    auto reduce = [&](auto kernel, int per, const auto* slabs) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((quads + per - 1) / per)), dim3(256), 0, s, d, r, q.cols_h, q.cols, q.splits, slabs,
+                           w, keep, A_in, B_in, A, B, Ad, Bd);
+    };
+    if (Ad && quads < 16384) reduce(keep8_reduce_kernel<16, double>, 16, (const double*)slab);
+    else if (Ad) reduce(keep8_reduce_kernel<4, double>, 64, (const double*)slab);
+    else if (quads < 16384) reduce(keep8_reduce_kernel<16, float>, 16, (const float*)slab);
+    else reduce(keep8_reduce_kernel<4, float>, 64, (const float*)slab);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -1080,9 +1080,11 @@ int onmf_keep8_expand(onmf_ctx* c, int d, int n, const int8_t* codes, const floa
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient) {
     if (d <= 0 || r <= 0 || n <= 0 || n > MOST_COLS) return 0;                  // sizes that the calls refuse
     if (d > MOST_ROWS || r > MOST_ROWS || (gradient && (d > (1 << 18) || r > (1 << 18)))) return 0;
-    const SumPlan q = sum_plan(d, r, n);
+    const SumPlan q = sum_plan(d, r, n, true);
     if (gradient && by_residual(q, d, r, n)) return 0;
-    return sums_bytes(q, r) + (gradient ? gradient_bytes(d, r) : 0);
+    // slabs for either call's runs
+    const size_t slabs = std::max(sums_bytes(q, r, true), sums_bytes(sum_plan(d, r, n, false), r, false));
+    return slabs + (gradient ? gradient_bytes(d, r) : 0);
 }
 
 int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes, const float* x_scales,
@@ -1097,7 +1099,7 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_aggregate: workspace of %zu bytes, %zu needed, aligned to 16", ws_bytes, need);
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    return run_sums(c, sum_plan(d, r, n), d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, w, 1.0 - w, A_in, B_in,
+    return run_sums(c, sum_plan(d, r, n, false), d, r, n, x_codes, x_scales, h_codes, h_scales, ws, w, 1.0 - w, A_in, B_in,
                     A_out, B_out, nullptr, nullptr, s);
 }
 
@@ -1117,14 +1119,14 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
         return onmf_fail(c, ONMF_ERR_ARG, "keep8_gradient: dW lies over W, which all of it is computed from");
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
-    const SumPlan q = sum_plan(d, r, n);
+    const SumPlan q = sum_plan(d, r, n, true);
     if (by_residual(q, d, r, n)) {
         if (n <= 16) return launch_residual<1, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
         if (n <= 64) return launch_residual<4, 16>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
         return launch_residual<8, 8>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
     }
-    double* A = (double*)((char*)ws + sums_bytes(q, r));
-    ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, (float*)ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
+    double* A = (double*)((char*)ws + sums_bytes(q, r, true));
+    ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
                       A, A + (size_t)r * r, s));
     return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)A + both_sums_bytes(d, r), s);
 }

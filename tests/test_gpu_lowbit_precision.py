@@ -1,0 +1,50 @@
+"""What the operators on dictionaries in 4 bits and columns in 8 keep of float32's and double's precision, against the NumPy
+oracle in 64 bits: every bound here is a rounding or two of the formula, with no factor for the kernels' order."""
+import numpy as np
+import pytest
+
+from oracle import lowbit_oracle as lo
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch():
+    import torch
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    return torch
+
+
+@pytest.fixture(scope="module")
+def eng(torch):
+    from onmf_ontf_ndl_amd.engine import get_engine
+    return get_engine()
+
+
+def host(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+def kept_values(eng, X):
+    K = eng.keep8(eng.dev(X))
+    return K, lo.values8(K.codes.cpu().numpy().astype(np.float64), host(K.scales), K.n)
+
+
+# ------------------------------------------------------------------------------------------------- the gradient
+@pytest.mark.parametrize("d,r,n", [(256, 64, 8000), (512, 128, 20000), (1200, 100, 8191), (300, 300, 4000), (60, 20, 3000)])
+def test_gradient_at_the_least_squares_dictionary(eng, torch, d, r, n):
+    """Where W (H H^T) and X H^T cancel down to the rounding of W itself.  Everything up to dW is in double, several runs of
+    groups included: 2^-53 a rounding of the terms' magnitudes, in a chain of at most n / 128 groups, 16 for their runs and
+    r + 8 for W A (the oracle's own: n + 2 r), and half a float32 step of the result."""
+    rs = np.random.RandomState(d + r)
+    H = np.maximum(rs.randn(r, n), 0).astype(np.float32)
+    X = np.maximum(np.maximum(rs.randn(d, r), 0) @ H + rs.rand(d, n), 0).astype(np.float32)
+    (KX, Xh), (KH, Hh) = kept_values(eng, X), kept_values(eng, H)
+    assert eng.lib.onmf_keep8_workspace(d, r, n, 1) > 8 * r * (r + d) + 512          # several runs
+    W = np.linalg.solve(Hh @ Hh.T, Hh @ Xh.T).T.astype(np.float32)
+    g = host(eng.keep8_gradient(eng.dev(W), KX, KH))
+    W64 = W.astype(np.float64)
+    want = W64 @ (Hh @ Hh.T) - Xh @ Hh.T
+    size = np.abs(W64) @ (np.abs(Hh) @ np.abs(Hh).T) + np.abs(Xh) @ np.abs(Hh).T
+    assert np.abs(want).max() <= 1e-6 * size.max()
+    assert (np.abs(g - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -53 * (n / 128 + 16 + r + 8 + n + 2 * r) * size).all()
