@@ -394,8 +394,8 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  * onmf_keep8_gradient   dW (d x r) = W (H H^T) - X H^T, the gradient of 1/2 |X - W H|^2 to W; d, r <= 2^18;
  *                       dW may not overlap W.  Up to 128 columns are taken as (W H - X) H^T where that is less work
  * Products inside a group add up exactly in int32, groups in float32 (the gradient's in double, all the way to dW), runs
- * of groups and what follows in double; the gradient's W (H H^T) with large r by 28-bit whole numbers, within 2^-26 of the largest entries'
- * product.
+ * of groups and what follows in double; the gradient's W (H H^T) with large r by whole numbers of 31 bits where that is within 2^-25 of the entry's
+ * terms, |W H H^T| + |X H^T|, and in double where it is not.
  * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, aligned to 16, in use until the call's
  * work on `stream` is done.  n <= 2^28, at most 2^29 - 32 groups in a store.  Asynchronous on `stream`, allocates
  * nothing and can be captured into a graph.

@@ -219,7 +219,7 @@ struct SumParams {
     int tiles_m, tiles_h, tiles;     // tiles along r (rows); column tiles of the H H^T part; all tiles
     int cols_h, cols;         // columns of a slab row: the H H^T part's, all (both multiples of 4)
     // one run holds everything: the results at once, the gradient's as doubles
-    double *Ad, *Bd;
+    double *Ad, *Bd, *diag;   // (diag: A's diagonal once more, or null)
     double w, keep;
     const float *A_in, *B_in;
     float *A, *B;
@@ -400,6 +400,10 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
                 const size_t at = (size_t)m * N + n;
                 if constexpr (PRECISE) {
                     double* dst = (is_h ? p.Ad : p.Bd) + at;
+                    if (p.diag && is_h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (n + e == m) p.diag[m] = acc[i][j][e];
                     if (n + 4 <= N) {
                         reinterpret_cast<f64x2_any*>(dst)[0] = f64x2_any{acc[i][j][0], acc[i][j][1]};
                         reinterpret_cast<f64x2_any*>(dst)[1] = f64x2_any{acc[i][j][2], acc[i][j][3]};
@@ -472,7 +476,8 @@ template <int ZL, typename V>
 __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int cols_h, int cols, int splits,
                                                             const V* __restrict__ slab, double w, double keep,
                                                             const float* A_in, const float* B_in, float* A, float* B,
-                                                            double* __restrict__ Ad, double* __restrict__ Bd) {
+                                                            double* __restrict__ Ad, double* __restrict__ Bd,
+                                                            double* __restrict__ diag) {
     constexpr int Q = 256 / ZL;
     __shared__ double part[ZL][Q][4];
     const int q = threadIdx.x % Q, z0 = threadIdx.x / Q;
@@ -497,8 +502,10 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 #pragma unroll
         for (int z = 1; z < ZL; ++z) v += part[z][q][j];
         const size_t at = (size_t)k * N + n0 + j;
-        if constexpr (sizeof(V) == 8) (is_h ? Ad : Bd)[at] = v;
-        else out[at] = (float)(w * v + (in ? keep * (double)in[at] : 0.0));
+        if constexpr (sizeof(V) == 8) {
+            (is_h ? Ad : Bd)[at] = v;
+            if (diag && is_h && n0 + j == k) diag[k] = v;
+        } else out[at] = (float)(w * v + (in ? keep * (double)in[at] : 0.0));
     }
 }
 
@@ -507,13 +514,16 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // wave loads the double matrix pipe's operands (16x16x4) straight into registers, the next sixteen while these are
 // computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
 // row 4 e + l / 16.  Bound by the double matrix pipe where r is large (d=4096 r=256 19.5 us; r=1024 182, 47 TFLOP/s).
+// Behind the product by digits (below): only tiles that it marked, and of those only what it left as NaN.
+struct Marks { int* tiles; int rows, cols, across; };        // a mark for `rows` x `cols` of dW, `across` of them side by side
 template <int NW>
 __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
                                                                   const double* __restrict__ A, const double* __restrict__ B,
-                                                                  float* __restrict__ dW) {
+                                                                  float* __restrict__ dW, Marks marks) {
     __shared__ double part[NW][32][32], tb[32][33];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, quad = lane >> 4;
     const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
+    if (marks.tiles && !marks.tiles[i0 / marks.rows * marks.across + k0 / marks.cols]) return;
     for (int e = t; e < 1024; e += 64 * NW) {
         const int k = k0 + (e >> 5), i = i0 + (e & 31);
         tb[e & 31][e >> 5] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
@@ -570,28 +580,49 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
         double v = part[0][i][k];
 #pragma unroll
         for (int z = 1; z < NW; ++z) v += part[z][i][k];
-        if (i0 + i < d && k0 + k < r) dW[(size_t)(i0 + i) * r + k0 + k] = (float)(v - tb[i][k]);
+        if (i0 + i >= d || k0 + k >= r) continue;
+        float* dst = dW + (size_t)(i0 + i) * r + k0 + k;
+        if (!marks.tiles || *dst != *dst) *dst = (float)(v - tb[i][k]);
     }
 }
 
-// The same on the 8-bit matrix pipe, where r is large.  Each row of W and of A (which is symmetric) is scaled by a power of
-// two to at most a half and cut into four whole digits of 7 bits, x = sum_t q_t 2^(-7 (t + 1)) within 2^-29, that is
-// 2^-27 of the row's largest entry: an eighth of what a float32 is off by.  Products of digits add
-// up exactly in int32, those of one weight, t + u = 0..3, in one sum; what is left out (t + u > 3) is 2^-28 and less of
-// the largest.  The four sums, the powers of two and B meet in double.  Bound by the matrix pipe (d=4096 r=1024: the
-// ten products 45 us, 1.9 POP/s, the digits 13 us; on the double matrix pipe 182).
-constexpr int DIGITS = 4;
-constexpr int MOST_DIGIT_ROWS = 1 << 16;         // 4 products of 64 x 64 add up below 2^31
+// The same on the 8-bit matrix pipe, where r is large.  Atoms are balanced first, by c_j = 2^floor(log2(A_jj) / 2): the terms
+// W_ij c_j and A_jk / c_j have the same products, no term of A's row k is then above twice the square root of A_kk, and what an atom
+// weighs does not depend on how its scale is shared between W and H (one that no column uses weighs nothing).  Each row x of
+// the balanced W and A (which is symmetric) is rounded to whole numbers N of 31 bits, x = p 2^-31 N with a power of two p of at
+// most about twice the largest |x|, and N = sum_t q_t 2^(8 (3 - t)) cut into four digits of 8 bits.  Products of digits
+// add up exactly in int32, those of one weight, t + u = 0..4, in one sum; they meet in double.
+// What this is off by: half a unit of each x times the other's |x|, and of 2^62 a term what is left out (t + u > 4, below
+// 2^23 (1 + 2^-8)), |error| <= 2^-32 (p_w S_a + p_a S_w) + 2^-38.9 r p_w p_a with the rows' sums S of magnitudes.  An entry is kept
+// where that is at most 2^-25 (|W A| + |B|), half a float32 step of the terms; where it is not - a row's small terms count because
+// its large ones meet zeros of A or cancel - it is left as NaN and its tile marked, for the double pipe to compute anew.  So
+// every entry depends on its own row and column alone.  Bound by the matrix pipe (d=4096 r=1024: the thirteen products 55 us,
+// 2.0 POP/s, the digits 19, the look at the marks 5; on the double matrix pipe 182.  Where nothing is held, a dictionary of both
+// signs or codes that never meet, both are run: 282 us of the whole gradient instead of 105).
+constexpr int DIGITS = 4, SUMS = 5;
+constexpr int MOST_DIGIT_ROWS = 32767;           // 4 products of 128 x 128 add up below 2^31
 
-// digits[t][row][kp], zeros behind column r, and the powers of two: W's d rows, then A's r; a wave a row
+// c_j of A_jj as a power of two; 0 for an atom without code, 1 for one that is not finite (its row of A says so)
+__device__ __forceinline__ double balance(double diag, bool inverse) {
+    if (diag == 0.0) return inverse ? 1.0 : 0.0;
+    if (!(diag <= 1.7976931348623157e308)) return 1.0;
+    const int c = (int)((__double_as_longlong(diag) >> 52) - 1023) >> 1;     // (a sum of squares of scales is no subnormal number)
+    return __longlong_as_double((long long)(1023 + (inverse ? -c : c)) << 52);
+}
+
+// digits[t][row][kp], zeros behind column r, the powers of two and the sums of magnitudes: W's d rows, then A's r; a wave a
+// row.  The product's marks are taken back.
 __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp, const float* __restrict__ W,
-                                                            const double* __restrict__ A, int8_t* __restrict__ digits,
-                                                            double* __restrict__ powers) {
+                                                            const double* __restrict__ A, const double* __restrict__ diag,
+                                                            int8_t* __restrict__ digits, double* __restrict__ powers,
+                                                            double* __restrict__ sums, int* __restrict__ marks, int n_marks) {
+    for (int e = blockIdx.x * 256 + threadIdx.x; e < n_marks; e += gridDim.x * 256) marks[e] = 0;
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= d + r) return;
-    // four neighbours (those behind column r - 1 are zeros)
+    // four neighbours, balanced (those behind column r - 1 are zeros)
+    bool fine = true;
     auto values = [&](int k, double (&v)[4]) {
-        auto take = [&](const auto* src) {
+        auto take = [&](const auto* src, bool inverse) {
             if (k + 4 <= r) {
                 typedef std::remove_cv_t<std::remove_reference_t<decltype(*src)>> V;
                 typedef V V4 __attribute__((ext_vector_type(4), aligned(sizeof(V))));
@@ -602,29 +633,39 @@ __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp,
 #pragma unroll
                 for (int j = 0; j < 4; ++j) v[j] = k + j < r ? (double)src[k + j] : 0.0;
             }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                fine = fine && fabs(v[j]) <= 1.7976931348623157e308;
+                v[j] *= balance(diag[min(k + j, r - 1)], inverse);
+            }
         };
-        if (row < d) take(W + (size_t)row * r);
-        else take(A + (size_t)(row - d) * r);
+        if (row < d) take(W + (size_t)row * r, false);
+        else take(A + (size_t)(row - d) * r, true);
     };
-    double most = 0.0;
-    bool fine = true;
+    double most = 0.0, sum = 0.0;
 #pragma unroll 4
     for (int k = lane * 4; k < r; k += 256) {
         double v[4];
         values(k, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            fine = fine && fabs(v[j]) <= 1.7976931348623157e308;
             most = fmax(most, fabs(v[j]));
+            sum += fabs(v[j]);
         }
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) most = fmax(most, __shfl_xor(most, o, 64));
+    for (int o = 32; o > 0; o >>= 1) {
+        most = fmax(most, __shfl_xor(most, o, 64));
+        sum += __shfl_xor(sum, o, 64);
+    }
     fine = __all(fine);
-    int e = 0;
-    (void)frexp(fine ? most : 0.0, &e);               // most < 2^e
-    if (lane == 0) powers[row] = fine ? ldexp(1.0, e + 1) : (double)__int_as_float(0x7fc00000);
-    const double scale = fine ? ldexp(1.0, -e - 1) : 0.0;
+    int e = 0;                                        // most <= 127/128 2^e: the first digit is at most 127
+    if (fine && frexp(most, &e) > 127.0 / 128.0) ++e;
+    if (lane == 0) {
+        powers[row] = !fine ? (double)__int_as_float(0x7fc00000) : most > 0.0 ? ldexp(1.0, e) : 0.0;
+        sums[row] = sum;
+    }
+    const double scale = fine ? ldexp(1.0, 31 - e) : 0.0;
     const size_t plane = (size_t)(d + r) * kp;
 #pragma unroll 2
     for (int k = lane * 4; k < kp; k += 256) {
@@ -635,13 +676,12 @@ __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp,
         for (int t = 0; t < DIGITS; ++t) word[t] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            double x = fine ? v[j] * scale : 0.0;
+            int x = fine ? (int)rint(v[j] * scale) : 0;
 #pragma unroll
-            for (int t = 0; t < DIGITS; ++t) {
-                x *= 128.0;
-                const double q = rint(x);
-                x -= q;
-                word[t] |= ((uint32_t)(int)q & 0xff) << (8 * j);
+            for (int t = DIGITS - 1; t >= 0; --t) {
+                const int q = t > 0 ? (int)(int8_t)(x & 0xff) : x;
+                x = (x - q) >> 8;
+                word[t] |= ((uint32_t)q & 0xff) << (8 * j);
             }
         }
 #pragma unroll
@@ -654,7 +694,9 @@ __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp,
 template <int MI, int NJ, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d, int r, int kp, const int8_t* __restrict__ digits,
                                                                             const double* __restrict__ powers,
-                                                                            const double* __restrict__ B, float* __restrict__ dW) {
+                                                                            const double* __restrict__ sums,
+                                                                            const double* __restrict__ B, float* __restrict__ dW,
+                                                                            int* __restrict__ marks) {
     constexpr int NW = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN, BLOCKS = DIGITS * (BM + BN) / 16, LOADS = BLOCKS / NW;
     constexpr int STAGE = BLOCKS * 1024;
     static_assert(BLOCKS % NW == 0 && BM % 16 == 0, "");
@@ -677,9 +719,9 @@ __global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d
                                              (__attribute__((address_space(3))) void*)(lds + buf * STAGE + (j * NW + wave) * 1024),
                                              16, 0, 0);
     };
-    i32x4 acc[DIGITS][MI][NJ];
+    i32x4 acc[SUMS][MI][NJ];
 #pragma unroll
-    for (int t = 0; t < DIGITS; ++t)
+    for (int t = 0; t < SUMS; ++t)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -704,28 +746,34 @@ __global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d
 #pragma unroll
             for (int t = 0; t < DIGITS; ++t)
 #pragma unroll
-                for (int u = 0; u < DIGITS - t; ++u)
+                for (int u = 0; u < DIGITS && t + u < SUMS; ++u)
 #pragma unroll
                     for (int j = 0; j < NJ; ++j)
                         acc[t + u][i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[t], fb[u][j], acc[t + u][i][j], 0, 0, 0);
         }
     }
+    bool unheld = false;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
         const int i = i0 + wn + 16 * j + (lane & 15);
         if (i >= d) continue;
-        const double pi = powers[i] * 0x1p-14;
+        const double pi = powers[i], si = sums[i];
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
             const int k = k0 + wm + 16 * m + 4 * (lane >> 4);
             f32x4_any out;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                double v = (double)acc[DIGITS - 1][m][j][e];
+                double v = (double)acc[SUMS - 1][m][j][e];
 #pragma unroll
-                for (int t = DIGITS - 2; t >= 0; --t) v = v * 0x1p-7 + (double)acc[t][m][j][e];
+                for (int t = SUMS - 2; t >= 0; --t) v = v * 0x1p-8 + (double)acc[t][m][j][e];
                 const int kk = min(k + e, r - 1);
-                out[e] = (float)(v * pi * powers[d + kk] - B[(size_t)kk * d + i]);
+                const double pk = powers[d + kk], b = B[(size_t)kk * d + i];
+                v = v * 0x1p-14 * pi * pk;
+                const double off = 0x1p-32 * (pi * sums[d + kk] + pk * si) + 0x1.13p-39 * r * pi * pk;
+                const bool held = off <= 0x1p-25 * (fabs(v) + fabs(b));
+                unheld = unheld || !held;
+                out[e] = held ? (float)(v - b) : __int_as_float(0x7fc00000);
             }
             float* dst = dW + (size_t)i * r + k;
             if (k + 4 <= r) *reinterpret_cast<f32x4_any*>(dst) = out;
@@ -735,6 +783,7 @@ __global__ __launch_bounds__(64 * WM * WN) void keep8_digit_product_kernel(int d
                     if (k + e < r) dst[e] = out[e];
         }
     }
+    if (unheld) marks[blockIdx.y * gridDim.x + blockIdx.x] = 1;
 }
 
 // The same gradient by way of the residual, dW = (W H - X) H^T, for up to 128 columns: with n < r / 2 of them it is
@@ -926,21 +975,21 @@ int launch_tile(onmf_ctx* c, int tile, const SumParams& p, hipStream_t s) {
 // The sums of a minibatch into A and B, or as doubles into Ad and Bd.
 int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* xc, const float* xs, const int8_t* hc, const float* hs,
              void* slab, double w, double keep, const float* A_in, const float* B_in, float* A, float* B, double* Ad,
-             double* Bd, hipStream_t s) {
+             double* Bd, double* diag, hipStream_t s) {
     SumParams p;
     p.hc = hc; p.xc = xc; p.hs = hs; p.xs = xs; p.slab = slab;
     p.d = d; p.r = r; p.groups = (n + GROUP - 1) / GROUP; p.per_split = q.per; p.splits = q.splits;
     p.tiles_m = q.tiles_m; p.tiles_h = q.tiles_h; p.tiles = q.tiles_m * (q.tiles_h + q.tiles_x);
     p.cols_h = q.cols_h; p.cols = q.cols;
     p.w = w; p.keep = keep; p.A_in = A_in; p.B_in = B_in; p.A = A; p.B = B;
-    p.Ad = Ad; p.Bd = Bd;
+    p.Ad = Ad; p.Bd = Bd; p.diag = diag;
     ONMF_TRY(Ad ? launch_tile<true>(c, q.tile, p, s) : launch_tile<false>(c, q.tile, p, s));
     if (q.splits == 1) return ONMF_OK;
     // (few entries with many slabs: more threads to an entry)
     const size_t quads = (size_t)r * q.cols / 4;
     auto reduce = [&](auto kernel, int per, const auto* slabs) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((quads + per - 1) / per)), dim3(256), 0, s, d, r, q.cols_h, q.cols, q.splits, slabs,
-                           w, keep, A_in, B_in, A, B, Ad, Bd);
+                           w, keep, A_in, B_in, A, B, Ad, Bd, diag);
     };
     if (Ad && quads < 16384) reduce(keep8_reduce_kernel<16, double>, 16, (const double*)slab);
     else if (Ad) reduce(keep8_reduce_kernel<4, double>, 64, (const double*)slab);
@@ -950,41 +999,62 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
     return ONMF_OK;
 }
 
-// Whole digits take a launch more.  Measured (us of the whole gradient, n=500, digits and the double pipe): d=4096 r=256 27
-// and 27, r=400 38 and 46, r=1024 75 and 178; d=1200 r=600 33 and 34; d=300 r=1024 36 and 34.
+// Whole digits take three launches, of which the last, for what they do not hold, mostly ends at once.  Measured (us of the
+// whole gradient, n=500, digits and the double pipe): d r^2 = 2.7e8, d=4096 r=256 34 and 31; 4.3e8 and 4.5e8, d=1200 r=600 41.0 and
+// 40.5, d=4096 r=330 47.7 and 46.5; 5.4e8, d=2048 r=512 40 and 43; 6.3e8, d=600 r=1024 46 and 55; 4.3e9, d=4096 r=1024 94 and 204.
 bool by_digits(int d, int r) { return r <= MOST_DIGIT_ROWS && (double)d * r * r > 4e8; }
 int digit_columns(int r) { return (r + 63) & ~63; }
-size_t digits_bytes(int d, int r) {
-    return by_digits(d, r) ? ((size_t)DIGITS * ((size_t)d + r) * digit_columns(r) + 255 & ~(size_t)255) + sizeof(double) * ((size_t)d + r) : 0;
-}
+// Rows and columns of a workgroup's tile
+int digit_tile(int d, int r) { return (long long)((r + 127) / 128) * ((d + 127) / 128) >= 256 ? 128 : 64; }
+struct DigitSpace {
+    int8_t* digits;                // [DIGITS][d + r][digit_columns]
+    double *powers, *sums;         // [d + r]
+    double* diag;                  // [r]
+    Marks marks;
+    size_t bytes;
+    DigitSpace(int d, int r, char* ws) {
+        const int tile = digit_tile(d, r);
+        const size_t planes = ((size_t)DIGITS * ((size_t)d + r) * digit_columns(r) + 255) & ~(size_t)255;
+        digits = (int8_t*)ws;
+        powers = (double*)(ws + planes);
+        sums = powers + d + r;
+        diag = sums + d + r;
+        marks = Marks{(int*)(diag + r), tile, tile, (r + tile - 1) / tile};
+        bytes = planes + sizeof(double) * (2 * ((size_t)d + r) + r) + sizeof(int) * (size_t)marks_count(d);
+    }
+    int marks_count(int d) const { return marks.across * ((d + marks.rows - 1) / marks.rows); }
+};
+size_t digits_bytes(int d, int r) { return by_digits(d, r) ? DigitSpace(d, r, nullptr).bytes : 0; }
 template <int MI, int NJ, int WM, int WN>
-int launch_digit_product(onmf_ctx* c, int d, int r, const int8_t* digits, const double* powers, const double* B, float* dW, hipStream_t s) {
+int launch_digit_product(onmf_ctx* c, int d, int r, const DigitSpace& q, const double* B, float* dW, hipStream_t s) {
     constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
+    static_assert(BM == BN, "a mark is a square");
     constexpr size_t bytes = 2 * (size_t)DIGITS * (BM + BN) * 64;
     static LdsLimit lim;
     ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_digit_product_kernel<MI, NJ, WM, WN>, bytes));
     hipLaunchKernelGGL((keep8_digit_product_kernel<MI, NJ, WM, WN>), dim3((r + BM - 1) / BM, (d + BN - 1) / BN), dim3(64 * WM * WN),
-                       bytes, s, d, r, digit_columns(r), digits, powers, B, dW);
+                       bytes, s, d, r, digit_columns(r), q.digits, q.powers, q.sums, B, dW, q.marks.tiles);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
 int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const double* A, const double* B, float* dW, char* ws, hipStream_t s) {
+    Marks marks = {nullptr, 1, 1, 1};
     if (by_digits(d, r)) {
-        int8_t* digits = (int8_t*)ws;
-        double* powers = (double*)(ws + digits_bytes(d, r) - sizeof(double) * ((size_t)d + r));
-        hipLaunchKernelGGL(keep8_digits_kernel, dim3((d + r + 3) / 4), dim3(256), 0, s, d, r, digit_columns(r), W, A, digits, powers);
+        const DigitSpace q(d, r, ws);
+        hipLaunchKernelGGL(keep8_digits_kernel, dim3((d + r + 3) / 4), dim3(256), 0, s, d, r, digit_columns(r), W, A, q.diag, q.digits,
+                           q.powers, q.sums, q.marks.tiles, q.marks_count(d));
         HIP_TRY(c, hipGetLastError());
-        if ((long long)((r + 127) / 128) * ((d + 127) / 128) >= 256)
-            return launch_digit_product<4, 2, 2, 4>(c, d, r, digits, powers, B, dW, s);
-        return launch_digit_product<2, 2, 2, 2>(c, d, r, digits, powers, B, dW, s);
+        if (q.marks.rows == 128) ONMF_TRY((launch_digit_product<4, 2, 2, 4>(c, d, r, q, B, dW, s)));
+        else ONMF_TRY((launch_digit_product<2, 2, 2, 2>(c, d, r, q, B, dW, s)));
+        marks = q.marks;
     }
     const dim3 grid((r + 31) / 32, (d + 31) / 32);
     // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
     // tiles the double matrix pipe is what counts: d=8192 r=256 36 us, with eight waves 42)
     if (r > 64 && (size_t)grid.x * grid.y <= 512)
-        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, A, B, dW);
+        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, A, B, dW, marks);
     else
-        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, A, B, dW);
+        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, A, B, dW, marks);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
@@ -1100,7 +1170,7 @@ int onmf_keep8_aggregate(onmf_ctx* c, int d, int r, int n, const int8_t* x_codes
     ONMF_ENTER(c);
     hipStream_t s = (hipStream_t)stream;
     return run_sums(c, sum_plan(d, r, n, false), d, r, n, x_codes, x_scales, h_codes, h_scales, ws, w, 1.0 - w, A_in, B_in,
-                    A_out, B_out, nullptr, nullptr, s);
+                    A_out, B_out, nullptr, nullptr, nullptr, s);
 }
 
 int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const int8_t* x_codes, const float* x_scales,
@@ -1126,9 +1196,10 @@ int onmf_keep8_gradient(onmf_ctx* c, int d, int r, int n, const float* W, const 
         return launch_residual<8, 8>(c, d, r, W, x_codes, x_scales, h_codes, h_scales, dW, s);
     }
     double* A = (double*)((char*)ws + sums_bytes(q, r, true));
+    char* rest = (char*)A + both_sums_bytes(d, r);
     ONMF_TRY(run_sums(c, q, d, r, n, x_codes, x_scales, h_codes, h_scales, ws, 1.0, 0.0, nullptr, nullptr, nullptr, nullptr,
-                      A, A + (size_t)r * r, s));
-    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, (char*)A + both_sums_bytes(d, r), s);
+                      A, A + (size_t)r * r, by_digits(d, r) ? DigitSpace(d, r, rest).diag : nullptr, s));
+    return launch_gradient(c, d, r, W, A, A + (size_t)r * r, dW, rest, s);
 }
 
 }  // extern "C"

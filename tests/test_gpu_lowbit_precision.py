@@ -48,3 +48,46 @@ def test_gradient_at_the_least_squares_dictionary(eng, torch, d, r, n):
     size = np.abs(W64) @ (np.abs(Hh) @ np.abs(Hh).T) + np.abs(Xh) @ np.abs(Hh).T
     assert np.abs(want).max() <= 1e-6 * size.max()
     assert (np.abs(g - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -53 * (n / 128 + 16 + r + 8 + n + 2 * r) * size).all()
+
+
+@pytest.mark.parametrize("d,r,n", [(700, 256, 500), (4100, 300, 400), (4100, 330, 400), (6000, 640, 300), (1300, 1030, 700),
+                                   (150, 2050, 300)])
+@pytest.mark.parametrize("kind", ["even", "dead", "rescaled", "apart", "signed", "dominated"])
+def test_gradient_holds_the_terms_that_are_summed(eng, torch, d, r, n, kind):
+    """W (H H^T) in double or in whole digits, whichever a size takes: an entry is off by at most half a float32 step of itself
+    and half a step of its own terms, |W| |H H^T| + |X| |H|^T - of an atom that no column uses, of scales moved from W to H, of
+    small entries beside large ones that meet zeros."""
+    rs = np.random.RandomState(d + r + n)
+    W = np.maximum(rs.randn(d, r) + 0.4, 0).astype(np.float32)
+    H = np.maximum(rs.randn(r, n), 0).astype(np.float32)
+    if kind == "dead":
+        H[3] = 0
+        H[r - 1] = 0
+        W[:, 3] *= 1e4
+        W[:, r - 1] *= 1e30
+    elif kind == "rescaled":
+        for j, f in ((5, 1e-4), (6, 1e6), (7, 1e-15), (r - 2, 1e12)):
+            W[:, j] *= f
+            H[j] /= f
+    elif kind == "apart":
+        H *= np.arange(r)[:, None] % min(n, r) == np.arange(n)[None, :] % min(n, r)
+        W *= 10.0 ** rs.randint(-6, 1, size=(d, r))
+    elif kind == "signed":
+        W = rs.randn(d, r).astype(np.float32)
+    elif kind == "dominated":
+        W[:, 1:] *= 1e-5
+        W[::3, 0] = 0
+    live = np.where(H.any(1), np.abs(W).max(0), 0) if kind != "dead" else np.where(H.any(1), 1, 0)
+    X = np.maximum((W * (live > 0)).astype(np.float64) @ H + 0.1 * rs.rand(d, n), 0).astype(np.float32)
+    (KX, Xh), (KH, Hh) = kept_values(eng, X), kept_values(eng, H)
+    g = host(eng.keep8_gradient(eng.dev(W), KX, KH))
+    W64 = W.astype(np.float64)
+    A, B = Hh @ Hh.T, Xh @ Hh.T
+    want = W64 @ A - B
+    size = np.abs(W64) @ A + np.abs(Xh) @ np.abs(Hh).T
+    bound = 2.0 ** -24 * np.abs(want) + 2.0 ** -25 * (1 + 2.0 ** -20) * size + 2.0 ** -53 * (2 * n + 4 * r + 64) * size
+    assert np.isfinite(g).all() and (np.abs(g - want) <= bound).all()
+    # ... and every entry depends on its own row of W alone, whichever way its neighbours are computed
+    other = rs.randn(d, r).astype(np.float32) * np.float32(1e3)
+    other[::7] = W[::7]
+    assert np.array_equal(host(eng.keep8_gradient(eng.dev(other), KX, KH))[::7], g[::7])
