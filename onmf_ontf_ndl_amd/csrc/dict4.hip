@@ -56,6 +56,11 @@ __device__ __forceinline__ void word_entries(uint32_t w, float (&q)[8]) {
     q[7] = (float)(o >> 24);
 }
 
+// W^T X multiplies the whole numbers q + z by the columns and adds up 32 features before the scale comes in: up to 32 * 255
+// times the largest |x|, which float32 need not hold where it holds the result.  The whole numbers (the one column's kernel: x)
+// are therefore shrunk by 2^14, exactly, and the finished sums grown again: what is added up lies within s (q + |z|) |x|.
+constexpr float SHRINK = 0x1p-14f, GROW = 0x1p14f;
+
 // ------------------------------------------------------------------------------------------- packing
 // smallest bfloat16 >= v (v >= 0, finite), as float
 __device__ __forceinline__ float bf16_up(double v) {
@@ -153,7 +158,7 @@ __global__ __launch_bounds__(256) void dict4_unpack_kernel(int d, int r, int gro
 }
 
 // ------------------------------------------------------------------------------------------- few columns
-// C = W^T x for one column: bound by reading the codes once (d=4096 r=32768, 71 MB: 18 us, 3.9 TB/s; d=441 r=25 3 us, a
+// C = W^T x for one column: bound by reading the codes once (d=4096 r=32768, 71 MB: 17 us, 4.2 TB/s; d=441 r=25 3 us, a
 // launch).  A lane owns F = 8 CH consecutive features of a segment of 64 F; x is staged in LDS as float and a
 // segment's F values are held in registers while AT atoms stream past.  An entry costs an extraction (0.4), a
 // conversion and a fused multiply-add; z is taken once a group, with the sum of its features.
@@ -180,8 +185,9 @@ __global__ __launch_bounds__(256) void dict4_correlate_one_kernel(int d, int r, 
             if (first || segs_staged < segs) {          // the whole of x fits: staged once
                 __syncthreads();
                 const int i0 = s0 * SEG, in = min(segs_staged, segs - s0) * SEG;
-                for (int i = threadIdx.x; i < in; i += 256) {
-                    const float v = i0 + i < d ? load_val(X + (size_t)(i0 + i) * ldx) : 0.f;
+#pragma unroll 4
+                for (int i = threadIdx.x; i < in; i += 256) {        // (features behind the last: its value, not used)
+                    const float x = load_val(X + (size_t)min(i0 + i, d - 1) * ldx), v = i0 + i < d ? x * SHRINK : 0.f;
                     const int g = i / SEG, l = (i % SEG) / F, f = i % F;
                     xs[((g * (F / 4) + (f >> 2)) * 64 + l) * 4 + (f & 3)] = v;
                 }
@@ -234,7 +240,7 @@ __global__ __launch_bounds__(256) void dict4_correlate_one_kernel(int d, int r, 
             float v = acc[a];
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-            if (lane == 0 && k0 + a < r) C[k0 + a] = v;
+            if (lane == 0 && k0 + a < r) C[k0 + a] = v * GROW;
         }
     }
 }
@@ -573,11 +579,11 @@ __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r,
                     xo[n][q] = __builtin_bit_cast(bf16x8, xop[(((blk * 4 + j) * NT + n) * PX + q) * 64 + lane]);
 #pragma unroll
             for (int a = 0; a < AT; ++a) {
-                const float s = word_scale(x.sc[a][j]), z = word_offset(x.sc[a][j]);
+                const float s = word_scale(x.sc[a][j]), z = word_offset(x.sc[a][j]) * SHRINK;
                 float q[8];
                 word_entries(w[a][j], q);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) q[i] += z;
+                for (int i = 0; i < 8; ++i) q[i] = fmaf(q[i], SHRINK, z);
                 const bf16x8 wo = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]),
                                                                         pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7])));
 #pragma unroll
@@ -600,11 +606,11 @@ __global__ __launch_bounds__(512) void dict4_correlate_tile_kernel(int d, int r,
             for (int n = 0; n < NT; ++n) {
                 const int col = 16 * n + 4 * kq;
                 float* dst = out + (size_t)k * b + c0 + col;
-                if (k < r && col + 4 <= cols) *reinterpret_cast<f32x4_any*>(dst) = acc[a][n];
+                if (k < r && col + 4 <= cols) *reinterpret_cast<f32x4_any*>(dst) = acc[a][n] * GROW;
                 else if (k < r)
 #pragma unroll
                     for (int e = 0; e < 3; ++e)
-                        if (col + e < cols) dst[e] = acc[a][n][e];
+                        if (col + e < cols) dst[e] = acc[a][n][e] * GROW;
             }
         }
     };
@@ -669,11 +675,11 @@ __global__ __launch_bounds__(64 * NW) void dict4_correlate_wave_kernel(int d, in
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto compute = [&](int s, Raw& v) {
-        const float sc = word_scale(v.sc), z = word_offset(v.sc);
+        const float sc = word_scale(v.sc), z = word_offset(v.sc) * SHRINK;
         float q[8];
         word_entries(v.w, q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] += z;
+        for (int i = 0; i < 8; ++i) q[i] = fmaf(q[i], SHRINK, z);
         const bf16x8 wo = __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]),
                                                                 pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7])));
 #pragma unroll
@@ -720,15 +726,15 @@ __global__ __launch_bounds__(64 * NW) void dict4_correlate_wave_kernel(int d, in
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) v += part[w][n][l][e & 3];
-        if (atom < r && col < b) C[(size_t)atom * b + col] = v;
+        if (atom < r && col < b) C[(size_t)atom * b + col] = v * GROW;
     }
 }
 
 // ------------------------------------------------------------------------------------------- many columns
 // The bfloat16 matrix pipe (16x16x32), exact to float32's rounding: a float32 value is the sum of three bfloat16
 // pieces (8 + 8 + 8 bits), a bfloat16 one is its own piece.
-//  correlate: the whole numbers q + z (|q + z| <= 255) are bfloat16 values; 32 features' products are summed on
-//             their own and multiplied by their group's scale.
+//  correlate: the whole numbers q + z (|q + z| <= 255), shrunk, are bfloat16 values; 32 features' products are summed
+//             on their own and multiplied by their group's scale.
 //  product:   s (q + z) has at most 16 significant bits: two bfloat16 pieces hold it exactly; of the six
 //             products of pieces the last (2^-24) is left out.
 // The weights are laid out as bfloat16 rows [piece][m][k] in the workspace first (unpacked in the product's kernel
@@ -753,11 +759,11 @@ __global__ __launch_bounds__(256) void dict4_lay_correlate_kernel(int d, int r, 
     for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < all; e += (size_t)gridDim.x * 256) {
         const int k = (int)(e / words), w = (int)(e % words), g = w * 8 / group;
         const uint32_t sc = scales[(size_t)k * groups + g];
-        const float z = word_offset(sc);
+        const float z = word_offset(sc) * SHRINK;
         float q[8];
         word_entries(codes[e], q);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) q[j] = w * 8 + j < d ? q[j] + z : 0.f;
+        for (int j = 0; j < 8; ++j) q[j] = w * 8 + j < d ? fmaf(q[j], SHRINK, z) : 0.f;
         A[e] = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
         if (w * 8 % group == 0) S[(size_t)g * r + k] = word_scale(sc);
     }
@@ -920,7 +926,7 @@ __device__ __forceinline__ void row_tiles(const char* a, const float* s, int lan
     }
 }
 
-template <int MT, int CT>
+template <bool PROD, int MT, int CT>
 __device__ __forceinline__ void store_tiles(float* out, int ldo, int M, int N, int m0, int n0, int lane, const f32x4 (&acc)[MT][CT]) {
     const int n = n0 + CT * (lane & 15);
     if (n >= N) return;
@@ -931,13 +937,16 @@ __device__ __forceinline__ void store_tiles(float* out, int ldo, int M, int N, i
             const int m = m0 + 16 * i + 4 * (lane >> 4) + e;
             if (m >= M) continue;
             float* dst = out + (size_t)m * ldo + n;
+            float v[CT];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) v[c] = PROD ? acc[i][c][e] : acc[i][c][e] * GROW;
             if (n + CT <= N) {
-                if constexpr (CT == 2) *reinterpret_cast<f32x2_any*>(dst) = f32x2_any{acc[i][0][e], acc[i][1][e]};
-                else *reinterpret_cast<f32x4_any*>(dst) = f32x4_any{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+                if constexpr (CT == 2) *reinterpret_cast<f32x2_any*>(dst) = f32x2_any{v[0], v[1]};
+                else *reinterpret_cast<f32x4_any*>(dst) = f32x4_any{v[0], v[1], v[2], v[3]};
             } else
 #pragma unroll
                 for (int c = 0; c < CT - 1; ++c)
-                    if (n + c < N) dst[c] = acc[i][c][e];
+                    if (n + c < N) dst[c] = v[c];
         }
 }
 
@@ -1003,8 +1012,8 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
         row_tiles<PROD, MT>(lds + buf * STAGE, lscale + buf * SROWS, lane, fb, acc);
         if (s + 1 < steps) x.split(fb);
     }
-    if (p.slab) store_tiles(p.slab + (size_t)blockIdx.y * p.M * p.N, p.N, p.M, p.N, m0, n0, lane, acc);
-    else store_tiles(p.out, p.ldo, p.M, p.N, m0, n0, lane, acc);
+    if (p.slab) store_tiles<PROD>(p.slab + (size_t)blockIdx.y * p.M * p.N, p.N, p.M, p.N, m0, n0, lane, acc);
+    else store_tiles<PROD>(p.out, p.ldo, p.M, p.N, m0, n0, lane, acc);
 }
 
 // The same for a contraction so short that a workgroup keeps all its rows' weights in LDS: it unpacks them there itself, and
@@ -1062,11 +1071,11 @@ __global__ __launch_bounds__(256, 2) void dict4_resident_kernel(ResidentParams p
             uint32_t u[4] = {0, 0, 0, 0};
             if (k < p.r) {
                 const uint32_t sc = p.scales[(size_t)k * p.groups + w * 8 / p.group];
-                const float z = word_offset(sc);
+                const float z = word_offset(sc) * SHRINK;
                 float q[8];
                 word_entries(p.codes[(size_t)k * words + w], q);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) q[j] = w * 8 + j < p.d ? q[j] + z : 0.f;
+                for (int j = 0; j < 8; ++j) q[j] = w * 8 + j < p.d ? fmaf(q[j], SHRINK, z) : 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) u[j] = pack_bf16(q[2 * j], q[2 * j + 1]);
                 if (w * 8 % p.group == 0) lscale[w * 8 / p.group * ROWS + row] = word_scale(sc);
@@ -1098,7 +1107,7 @@ __global__ __launch_bounds__(256, 2) void dict4_resident_kernel(ResidentParams p
             }
             row_tiles<PROD, MT>(lds + s * STAGE, lscale + s * BK / p.group * ROWS, lane, fb, acc);
         }
-        store_tiles(p.out, p.ldo, p.M, p.N, m0, set * 16 * CT, lane, acc);
+        store_tiles<PROD>(p.out, p.ldo, p.M, p.N, m0, set * 16 * CT, lane, acc);
     }
 }
 

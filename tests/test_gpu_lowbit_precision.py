@@ -91,3 +91,44 @@ def test_gradient_holds_the_terms_that_are_summed(eng, torch, d, r, n, kind):
     other = rs.randn(d, r).astype(np.float32) * np.float32(1e3)
     other[::7] = W[::7]
     assert np.array_equal(host(eng.keep8_gradient(eng.dev(other), KX, KH))[::7], g[::7])
+
+
+# ------------------------------------------------------------------------------------------------- the two products
+STEP = 2.0 ** -23          # a rounding, or what a matrix instruction cuts off
+# every kernel of either product: one column, few in one launch, ranges and slabs, weights resident, weights laid out
+PATHS = [(441, 25, 1, 64), (2500, 70, 1, 128), (1030, 20, 1, 32), (100, 16, 2, 64), (2100, 33, 2, 32), (1100, 8200, 2, 32),
+         (441, 72, 3, 64), (250, 40, 20, 32), (441, 72, 50, 128), (2500, 8200, 8, 64), (8192, 72, 3, 32), (4096, 40, 100, 64),
+         (2100, 3000, 31, 32), (300, 70, 1501, 64), (1200, 100, 8192, 64), (441, 100, 1101, 32), (33, 3, 1025, 32),
+         (1300, 900, 1031, 32), (3000, 300, 1026, 128)]
+
+
+def packed(eng, q, z, s, d, group):
+    from onmf_ontf_ndl_amd import PackedDictionary
+    codes, scales = lo.to_codes4(q, z, s)
+    t = eng.torch
+    return PackedDictionary(t.from_numpy(codes).to(eng.device), t.from_numpy(scales).to(eng.device), d, group)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("size", [1e-30, 1e35, 1.5e38])
+@pytest.mark.parametrize("d,r,b,group", PATHS)
+def test_products_keep_float32s_range(eng, torch, d, r, b, group, size, dtype):
+    """Columns near either end of what float32 holds, entries of a dictionary far from zero beside their scale: the result is
+    finite and as near as ever - 2^-23 a rounding, at most K / 4 + 64 of them one after another, of the magnitudes that are
+    added up - where those have a sum that float32 holds."""
+    rs = np.random.RandomState(d + r + b)
+    groups = -(-d // group)
+    q = rs.randint(0, 16, size=(r, groups * group))
+    q[:, d:] = 0
+    z = rs.randint(225, 241, size=(r, groups))
+    for K, other, call in ((d, r, "dict4_correlate"), (r, d, "dict4_product")):
+        # entries of up to 255 2^-e, K of them: their sum's magnitude stays below 1.5 times the largest |x|
+        s = np.full((r, groups), 2.0 ** -np.ceil(np.log2(255 * K / 1.5)))
+        P = packed(eng, q, z, s, d, group)
+        W = lo.values4(q, z, s, d)
+        W = W.T if call == "dict4_correlate" else W
+        X = eng.dev((rs.rand(K, b) * size).astype(np.float32))
+        X = X.bfloat16() if dtype == "bfloat16" else X
+        got, want = host(getattr(eng, call)(P, X)), W @ host(X)
+        assert np.isfinite(got).all()
+        assert (np.abs(got - want) <= STEP * (K / 4 + 64) * want).all()
