@@ -397,6 +397,7 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  * Products inside a group add up exactly in int32, groups in float32 (the gradient's in double, all the way to dW), runs
  * of groups and what follows in double; the gradient's W (H H^T) with large r by whole numbers of 31 bits where that is within 2^-25 of the entry's
  * terms, |W H H^T| + |X H^T|, and in double where it is not.
+ * H's entries are below 2^113 in onmf_keep8_aggregate (a group's whole sum times its scale is held in float32).
  * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, aligned to 16, in use until the call's
  * work on `stream` is done.  n <= 2^28, at most 2^29 - 32 groups in a store.  Asynchronous on `stream`, allocates
  * nothing and can be captured into a graph.

@@ -198,7 +198,9 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 // and tile: half the scale reads of the 32x32 shape).  The codes go from memory straight to LDS, two groups ahead,
 // in rows of 128 bytes whose 16-byte chunks are permuted by (row >> 1) & 7, so that the 16 rows of an operand read
 // meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.
-// Per group and output three vector instructions (conversion, product of the scales, fused multiply-add) stand
+// In float32 H's scale is multiplied to the whole sum and X's with the addition: the two scales' own product may lie beyond
+// what float32 holds where the sum does not, and that would make zeros NaN.
+// Per group and output three vector instructions (conversion, product with a scale, fused multiply-add) stand
 // against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not
 // (d=4096 r=256 n=65536, 146 GOP: 125 us, PRECISE 145 and the slabs' 62 MB; d=1024 40 us).
 template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(64 * S::waves) void keep8_sums_kernel(SumParams p) 
 #pragma unroll
                 for (int i = 0; i < S::mi; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(xs[e] * hs[i], (float)part[i][e], acc[i][j][e]);
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(xs[e], hs[i] * (float)part[i][e], acc[i][j][e]);
             }
         }
         buf = buf == AHEAD ? 0 : buf + 1;

@@ -93,6 +93,24 @@ def test_gradient_holds_the_terms_that_are_summed(eng, torch, d, r, n, kind):
     assert np.array_equal(host(eng.keep8_gradient(eng.dev(other), KX, KH))[::7], g[::7])
 
 
+# ------------------------------------------------------------------------------------------------- the aggregates
+@pytest.mark.parametrize("d,r,n", [(40, 20, 1000), (100, 60, 300), (130, 129, 700), (300, 300, 260), (200, 30, 5000)])
+def test_aggregates_keep_float32s_range(eng, torch, d, r, n):
+    """Scales whose own product float32 does not hold: small columns and codes (two roundings a group and its addition, half a
+    step each, as ever), and large ones that never meet, whose sums are zeros."""
+    rs = np.random.RandomState(d + n)
+    X, H = (rs.rand(d, n) * 1e-20).astype(np.float32), (rs.rand(r, n) * 1e-16).astype(np.float32)
+    (KX, Xh), (KH, Hh) = kept_values(eng, X), kept_values(eng, H)
+    _, B = eng.keep8_aggregate(KX, KH, 1.0)
+    assert (np.abs(host(B) - Hh @ Xh.T) <= 2.0 ** -24 * (n / 128 + 4) * (Hh @ Xh.T)).all()
+    early = np.arange(n) % 128 < 64
+    X, H = (rs.rand(d, n) * early * 1e36).astype(np.float32), (rs.rand(r, n) * ~early * 1e8).astype(np.float32)
+    (KX, Xh), (KH, Hh) = kept_values(eng, X), kept_values(eng, H)
+    A, B = eng.keep8_aggregate(KX, KH, 1.0)
+    assert np.array_equal(host(B), np.zeros((r, d)))
+    assert (np.abs(host(A) - Hh @ Hh.T) <= 2.0 ** -24 * (n / 128 + 4) * (Hh @ Hh.T)).all()
+
+
 # ------------------------------------------------------------------------------------------------- the two products
 STEP = 2.0 ** -23          # a rounding, or what a matrix instruction cuts off
 # every kernel of either product: one column, few in one launch, ranges and slabs, weights resident, weights laid out
