@@ -3,7 +3,8 @@
 reconstruction by overlap-averaging) - no plotting, no files written.
 
 Same constructor arguments and method names as the reference (image_reconstruction_tensor.py:15-328);
-``path`` may also be an (h, w[, 3]) array already scaled to [0, 1].
+``path`` may also be an (h, w[, 3]) array already scaled to [0, 1].  For reconstruction ``W`` may be set to a
+``PackedDictionary`` (lowbit.py).
 
 * ``extract_random_patches`` (:87-124)  (k^2, 3, n) colour / (k^2, n, 1) grey patch tensors, one
   gather kernel instead of ``np.append`` in a loop;
@@ -18,6 +19,7 @@ import numpy as np
 
 from .engine import get_engine
 from .image_reconstruction import downscale_local_mean, _to_numpy
+from .lowbit import PackedDictionary
 from .onmf import _is_torch, _out
 from .ontf import Online_NTF
 
@@ -69,6 +71,10 @@ class Image_Reconstructor():
 
     def _engine(self):
         return get_engine(self._device)
+
+    def _dict_dev(self):
+        """``self.W`` as the products take it: a PackedDictionary as it is, anything else on the GPU."""
+        return self.W if isinstance(self.W, PackedDictionary) else self._engine().dev(self.W)
 
     def read_img_as_array(self, path=None):
         """Image as an array in [0, 1] (image_reconstruction_tensor.py:68-85).  Arrays pass through."""
@@ -139,7 +145,7 @@ class Image_Reconstructor():
     def _code_windows(self, X, alpha):
         eng = self._engine()
         coder = Online_NTF(X, self.n_components, alpha=alpha, rng=self.rng, device=self._device)
-        return coder._code_dev(eng, X, eng.dev(self.W))           # r x b
+        return coder._code_dev(eng, X, self._dict_dev())          # r x b
 
     def reconstruct_image(self, path, downscale_factor=None, patch_size=10, is_matrix=False):
         """Grey image: every window coded (alpha = 2, the coder's default), averaged back; returns the
@@ -158,7 +164,7 @@ class Image_Reconstructor():
         grid = (h - k + 1, w - k + 1)
         X = eng.extract_patches(eng.dev(data), k, grid=grid, stride=1)
         code = self._code_windows(X, None)
-        out, _ = eng.fold_patches(eng.patch_product(eng.dev(self.W), code), (h, w), k, grid, stride=1)
+        out, _ = eng.fold_patches(eng.patch_product(self._dict_dev(), code), (h, w), k, grid, stride=1)
         self.img_recons = _out(out, False)
         return _out(code.t().contiguous(), False)
 
@@ -179,7 +185,7 @@ class Image_Reconstructor():
             return self.A_recons
         X = eng.extract_patches(Ad, k, grid=grid, stride=s)
         code = self._code_windows(X, 1)
-        out, count = eng.fold_patches(eng.patch_product(eng.dev(self.W), code), tuple(Ad.shape), k, grid, stride=s)
+        out, count = eng.fold_patches(eng.patch_product(self._dict_dev(), code), tuple(Ad.shape), k, grid, stride=s)
         self.A_overlap_count = _out(count, like_torch)
         self.A_recons = _out(out, like_torch)
         return self.A_recons

@@ -21,7 +21,8 @@ import numpy as np
 
 from .engine import get_engine
 from .legacy.onmf import Online_NMF
-from .onmf import _out
+from .lowbit import PackedDictionary
+from .onmf import _dict_dev, _out
 
 __all__ = ["Network_Reconstructor"]
 
@@ -227,7 +228,8 @@ class Network_Reconstructor():
         codes); ``coder="cd"``: the non-negative least-squares problem itself by coordinate descent - and
         accumulated by one kernel into dense n x n sums.  Returns a ``networkx.Graph`` when
         networkx is importable, else an (m, 2) array of node-label pairs; ``return_weights`` adds the
-        (n x n) mean and count matrices (node order = ``self.nodes``)."""
+        (n x n) mean and count matrices (node order = ``self.nodes``).  ``W`` may be set to a ``PackedDictionary``
+        (lowbit.py)."""
         eng = self._engine()
         n = len(self.nodes)
         if n > 46000:
@@ -236,10 +238,10 @@ class Network_Reconstructor():
         emb = eng.ndl_init_embeddings(self._g(), B, 1, pivots=None, seed=self.seed + self._next_steps(1))
         X, trace = eng.ndl_sample_patches(self._g(), B, emb, int(recons_iter), glauber=self.is_glauber_recons,
                                           seed=self.seed, step_offset=self._next_steps(recons_iter), want_trace=True)
-        Wd = eng.dev(self.W)
+        Wd = self.W if isinstance(self.W, PackedDictionary) else eng.dev(self.W)
         from . import _lib
         if coder == "lars" and Wd.shape[1] <= 256:
-            H = eng.sparse_code_lars(X, Wd, alpha=0.0)
+            H = eng.sparse_code_lars(X, _dict_dev(eng, Wd), alpha=0.0)
         elif coder in ("lars", "cd"):
             H0 = eng.zeros(Wd.shape[1], X.shape[1])
             # every patch is its own least-squares problem: one launch, each column with its own stopping test

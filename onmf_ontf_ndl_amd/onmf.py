@@ -153,10 +153,11 @@ class Online_NMF():
         return _out(W1, _is_torch(W))
 
     def step(self, X, aggregates, W, t):
-        """One online-NMF iteration (src/onmf.py:119-167): returns H1, [A1, B1(, C1)], W1."""
+        """One online-NMF iteration (src/onmf.py:119-167): returns H1, [A1, B1(, C1)], W1 (an array also where W is a
+        PackedDictionary)."""
         eng = self._engine()
         like_torch = _is_torch(X) or isinstance(X, KeptColumns)
-        Xd, Wd = _columns_dev(eng, X), eng.dev(W)
+        Xd, Wd = _columns_dev(eng, X), _dict_dev(eng, W)
         Ad, Bd = eng.dev(aggregates[0]), eng.dev(aggregates[1])
         Cd = eng.dev(aggregates[2]) if len(aggregates) == 3 else None
         H1, agg1, W1 = self._step_dev(eng, Xd, Ad, Bd, Cd, Wd, t, want_code=True)
@@ -194,7 +195,7 @@ class Online_NMF():
             Cd = eng.zeros(d, d) if full_code else None
             returned = None
         else:
-            Wd = eng.dev(self.initial_dict)
+            Wd = _dict_dev(eng, self.initial_dict)
             Ad, Bd = eng.dev(self.initial_agg[0]), eng.dev(self.initial_agg[1])
             Cd = eng.dev(self.initial_agg[2]) if full_code else None
         t0 = self.history
@@ -270,4 +271,4 @@ def surrogate_loss(W, A, B, C=None, device=None):
     """tr(W A W^T) - 2 tr(W B) + tr(C): the convergence monitor that the reference's drivers compute
     from the three aggregates after each round (ising_reconstruction.py:133, :164)."""
     eng = get_engine(device)
-    return eng.surrogate_loss(eng.dev(W), eng.dev(A), eng.dev(B), None if C is None else eng.dev(C))
+    return eng.surrogate_loss(_dict_dev(eng, W), eng.dev(A), eng.dev(B), None if C is None else eng.dev(C))

@@ -23,7 +23,8 @@ import numpy as np
 
 from . import _lib
 from .engine import get_engine
-from .onmf import _is_torch, _out, _weight
+from .lowbit import PackedDictionary
+from .onmf import _dict_dev, _is_torch, _out, _weight
 
 __all__ = ["Online_NTF"]
 
@@ -85,12 +86,12 @@ class Online_NTF():
         return get_engine(self._device)
 
     def _code_dev(self, eng, Xd, Wd):
-        """Device solve; returns H as (r x b)."""
+        """Device solve; returns H as (r x b).  Wd may be a PackedDictionary."""
         a = 2 if self.alpha is None else self.alpha          # src/ontf.py:79-84
         if self.coder == "lars":
             if Wd.shape[1] > 256:
                 raise ValueError("coder='lars' supports n_components <= 256; use coder='cd'")
-            return eng.sparse_code_lars(Xd, Wd, alpha=a, max_iter=self.lars_max_iter)
+            return eng.sparse_code_lars(Xd, _dict_dev(eng, Wd), alpha=a, max_iter=self.lars_max_iter)
         H0 = eng.zeros(Wd.shape[1], Xd.shape[1])
         H, sweeps = eng.sparse_code_each(Xd, Wd, H0=H0, alpha=a, sub_iter=self.cd_max_sweeps,
                                          stopping_diff=self.cd_tol, mode=_lib.CODER_EXACT_CD, want_sweeps=True)
@@ -106,7 +107,7 @@ class Online_NTF():
     def joint_sparse_code_tensor(self, X, W):
         """Code H (samples x topics) with W H^T ~ X (src/ontf.py:59-89)."""
         eng = self._engine()
-        H = self._code_dev(eng, eng.dev(X), eng.dev(W))
+        H = self._code_dev(eng, eng.dev(X), W if isinstance(W, PackedDictionary) else eng.dev(W))
         return _out(H.t().contiguous(), _is_torch(X))
 
     def update_dict(self, W, A, B):
@@ -131,7 +132,7 @@ class Online_NTF():
         """One iteration (src/ontf.py:117-154): returns H1 (b x r), A1, B1, W1."""
         eng = self._engine()
         lt = _is_torch(X)
-        H, A1, B1, W1 = self._step_dev(eng, eng.dev(X), eng.dev(A), eng.dev(B), eng.dev(W), t)
+        H, A1, B1, W1 = self._step_dev(eng, eng.dev(X), eng.dev(A), eng.dev(B), _dict_dev(eng, W), t)
         return _out(H.t().contiguous(), lt), _out(A1, lt), _out(B1, lt), _out(W1, lt)
 
     def unfold(self):
@@ -159,7 +160,7 @@ class Online_NTF():
             Ad, Bd = eng.zeros(r, r), eng.zeros(r, d)
             ran = True
         else:
-            Wd, Ad, Bd = eng.dev(self.initial_dict), eng.dev(self.initial_A), eng.dev(self.initial_B)
+            Wd, Ad, Bd = _dict_dev(eng, self.initial_dict), eng.dev(self.initial_A), eng.dev(self.initial_B)
             ran = False
         t0 = self.history
         for i in np.arange(1, self.iterations):
