@@ -1004,7 +1004,9 @@ __global__ __launch_bounds__(256, 2) void dict4_many_kernel(ManyParams p) {
     x.split(fb);
     for (int s = 0; s < steps; ++s) {
         const int buf = s & 1, k = kbeg + s * BK;
-        __syncthreads();                               // (this step's weights have come, the last step's are done with)
+        // (this step's weights have come - a barrier by itself waits for no load to LDS, and that the columns' loads, sent behind
+        // them, were waited for is the compiler's choice - and all waves are done with the last step's)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (s + 1 < steps) {
             fetch_a(k + BK, buf ^ 1);
             x.fetch(k + BK);
