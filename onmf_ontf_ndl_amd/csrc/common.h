@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/onmf_hip.h"
+#include "lds_limit.h"
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -166,20 +167,13 @@ int onmf_reserve_pinned(onmf_ctx* c, size_t bytes);
         if (_rc != ONMF_OK) return _rc;                                                         \
     } while (0)
 
-// A kernel that wants more than 64 KB of dynamic LDS must be told so once per device: the attribute
-// belongs to the current device's copy of the kernel, so the "already done" note is kept per device
-// (one static LdsLimit per kernel).  Relaxed atomics: two contexts on two threads may both set the
-// attribute, which is harmless.
-struct LdsLimit {
-    static constexpr int MAX_DEV = 64;
-    std::atomic<size_t> bytes[MAX_DEV];
-    LdsLimit() { for (auto& b : bytes) b.store(0, std::memory_order_relaxed); }
-};
 inline int onmf_raise_lds_limit(onmf_ctx* c, LdsLimit& lim, const void* kernel, size_t bytes) {
-    const bool slot = c->device >= 0 && c->device < LdsLimit::MAX_DEV;
-    if (slot && lim.bytes[c->device].load(std::memory_order_relaxed) >= bytes) return ONMF_OK;
-    HIP_TRY(c, hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (slot) lim.bytes[c->device].store(bytes, std::memory_order_relaxed);
+    hipError_t e = hipSuccess;
+    lim.raise(c->device, bytes, [&](size_t want) {
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)want);
+        return e == hipSuccess;
+    });
+    HIP_TRY(c, e);
     return ONMF_OK;
 }
 
