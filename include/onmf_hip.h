@@ -14,7 +14,9 @@
  *   - `stream` is a hipStream_t passed as void* (NULL = default stream).  Calls enqueue work on it;
  *     entry points that return host scalars (sweeps_done, dist_trace) synchronise that stream.
  *   - Return value: ONMF_OK (0) or a negative ONMF_ERR_* code; the text is onmf_last_error(ctx).
- *     Nothing throws across the ABI.  A context is not thread-safe; use one per GPU/stream.
+ *     Nothing throws across the ABI.  A context is not thread-safe; use one per GPU/stream (the calls that pack,
+ *     unpack and multiply 4-bit dictionaries and those of the 8-bit columns may be made on one context by several threads
+ *     at once).
  */
 #ifndef ONMF_HIP_H
 #define ONMF_HIP_H
@@ -344,7 +346,8 @@ int onmf_numpy_rand(onmf_ctx* ctx, const uint32_t* key, int pos, size_t n, float
 /*
  * A dictionary held in 4 bits (no counterpart in the reference, whose dictionaries are float64 arrays).  The
  * features of an atom are taken in groups of `group` = 32, 64 or 128 that share a scale s (bfloat16) and a whole
- * number z; an entry stands for s (q + z) with q in 0..15 and differs from the entry of W by at most s / 2.
+ * number z; an entry stands for s (q + z) with q in 0..15 and differs from the entry of W by at most s / 2 (which may carry
+ * one within 2^-9 of the largest float32 to infinity).
  *   codes   r rows of ceil(d / group) * group / 2 bytes, aligned to 16 bytes: entry j of an eight-feature word is
  *           nibble (j >> 1) + 4 (j & 1); the padding behind feature d is zero nibbles
  *   scales  int32[r * ceil(d / group)]: the bits of s in the upper half, z (signed) in the lower
@@ -360,7 +363,9 @@ int onmf_numpy_rand(onmf_ctx* ctx, const uint32_t* key, int pos, size_t n, float
  * of the largest one) has NaNs or infinities in its result and touches no other column.  ws: at least onmf_dict4_workspace(which, d, r, b, group) bytes of device
  * memory, aligned to 16, in use until the call's work on `stream` is done (so calls on different streams take
  * different ones).  d <= 2^18; results may not overlap what is read.  Asynchronous on `stream`, allocates nothing and
- * can be captured into a graph.
+ * can be captured into a graph - but as every entry point it first settles a step that was not waited for
+ * (ONMF_OPT_DEFER_VERDICT), which waits for the GPU and may enqueue work on that step's stream: call onmf_settle before a
+ * capture, and before a call on another stream that reads what the step wrote.
  */
 #define ONMF_TYPE_F32 0
 #define ONMF_TYPE_BF16 1
@@ -383,8 +388,8 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  * Columns held in 8 bits (no counterpart in the reference): a minibatch X and its code H put away in a quarter of
  * their room until the dictionary's update or gradient needs them.  128 consecutive columns of a row share a scale
  * s = max|v| / 127 (float32: the product with the float32 nearest to 1 / 127); an entry stands for s q, q = rint(v / s),
- * ties to even, decided exactly, and differs from v by at most s / 2.  A group whose scale would be below 2^-126 reads as zeros, one with a NaN or an infinity
- * as NaNs.
+ * ties to even, decided exactly, and differs from v by at most s / 2.  A group whose scale would be below 2^-126 reads as
+ * zeros, one with a NaN or an infinity as NaNs.
  *   codes   int8, d rows of ceil(n / 128) * 128, aligned to 16 bytes; the padding behind column n is zeros
  *   scales  float32, d rows of ceil(n / 128)
  * onmf_keep8            X (d x n, float32 or bfloat16) -> codes, scales
@@ -395,12 +400,12 @@ int onmf_sparse_code_each_dict4(onmf_ctx* ctx, int d, int r, int b, int group, c
  * onmf_keep8_gradient   dW (d x r) = W (H H^T) - X H^T, the gradient of 1/2 |X - W H|^2 to W; d, r <= 2^18;
  *                       dW may not overlap W.  Up to 128 columns are taken as (W H - X) H^T where that is less work
  * Products inside a group add up exactly in int32, groups in float32 (the gradient's in double, all the way to dW), runs
- * of groups and what follows in double; the gradient's W (H H^T) with large r by whole numbers of 31 bits where that is within 2^-25 of the entry's
- * terms, |W H H^T| + |X H^T|, and in double where it is not.
+ * of groups and what follows in double; the gradient's W (H H^T) with large r by whole numbers of 31 bits where that is
+ * within 2^-25 of the entry's terms, |W H H^T| + |X H^T|, and in double where it is not.
  * H's entries are below 2^113 in onmf_keep8_aggregate (a group's whole sum times its scale is held in float32).
  * ws: at least onmf_keep8_workspace(d, r, n, gradient) bytes of device memory, aligned to 16, in use until the call's
  * work on `stream` is done.  n <= 2^28, at most 2^29 - 32 groups in a store.  Asynchronous on `stream`, allocates
- * nothing and can be captured into a graph.
+ * nothing and can be captured into a graph, a step that was not waited for settled first as above.
  */
 size_t onmf_keep8_workspace(int d, int r, int n, int gradient);
 int onmf_keep8(onmf_ctx* ctx, int d, int n, const void* X, int x_type, int ldx, int8_t* codes, float* scales, void* stream);

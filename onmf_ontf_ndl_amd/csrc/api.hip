@@ -620,6 +620,7 @@ static int sparse_code_impl(onmf_ctx* c, int d, int r, int b, const float* X, in
                     p.dev_rounds = dev_rounds;
                     p.s = s;
                     p.redo_after = *defer_redo;
+                    c->unsettled.store(true, std::memory_order_release);
                     if (after_valid) *after_valid = true;
                     return ONMF_OK;
                 }
@@ -832,11 +833,7 @@ static int sparse_code_impl(onmf_ctx* c, int d, int r, int b, const float* X, in
 // middle of the solve, or a workgroup gave up waiting): the solve is run again the ordinary way - its
 // inputs are still there, the caller leaves a deferred call's buffers alone until the next call - and then
 // whatever consumed its code.
-int onmf_settle_pending(onmf_ctx* c) {
-    if (!c->pend.active) return ONMF_OK;
-    PendingSolve p = c->pend;
-    c->pend.active = false;
-    c->pend.redo_after = nullptr;
+static int settle(onmf_ctx* c, const PendingSolve& p) {
     HIP_TRY(c, hipEventSynchronize(c->ev_rec));
     const float* rec = c->rec_pinned;
     const double tol = (double)p.stopping_diff;
@@ -891,6 +888,16 @@ int onmf_settle_pending(onmf_ctx* c) {
     ONMF_TRY(sparse_code_impl(c, p.d, p.r, p.b, p.X, p.ldx, p.W, p.H0, p.seed, p.alpha, p.sub_iter, p.stopping_diff,
                               ONMF_CODER_DAMPED, p.H, &sweeps, nullptr, p.s, nullptr, nullptr, timed_out));
     return p.redo_after ? p.redo_after() : ONMF_OK;
+}
+int onmf_settle_pending(onmf_ctx* c) {
+    std::lock_guard<std::recursive_mutex> guard(c->settle_lock);
+    if (!c->pend.active) return ONMF_OK;              // another thread has settled it, or this one is at it
+    const PendingSolve p = c->pend;
+    c->pend.active = false;
+    c->pend.redo_after = nullptr;
+    const int rc = settle(c, p);
+    c->unsettled.store(false, std::memory_order_release);
+    return rc;
 }
 
 static int aggregate_impl(onmf_ctx* c, int d, int r, int b, const float* X, int ldx, const float* H,

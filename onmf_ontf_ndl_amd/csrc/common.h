@@ -7,6 +7,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <functional>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -112,6 +113,8 @@ struct onmf_ctx {
     // verdicts looked at by the next call instead of this one
     int defer_verdict = 0;                // ONMF_OPT_DEFER_VERDICT
     PendingSolve pend;
+    std::atomic<bool> unsettled{false};   // pend waits to be looked at, or a thread is looking at it
+    std::recursive_mutex settle_lock;     // entry points that may be called from several threads: one of them settles, the others wait
     float* rec_pinned = nullptr;          // the verdict records in host memory the device writes (screen_final_kernel)
     float* rec_pinned_dev = nullptr;      // the same memory as the device addresses it
     long long sweeps_total = 0;           // sweeps of all settled solves
@@ -144,7 +147,7 @@ int onmf_settle_pending(onmf_ctx* c);
     if (_device_guard.err != hipSuccess)                                                         \
         return onmf_fail((ctx), ONMF_ERR_HIP, "selecting device %d failed: %s", (ctx)->device,   \
                          hipGetErrorString(_device_guard.err));                                  \
-    if ((ctx)->pend.active) {                                                                    \
+    if ((ctx)->unsettled.load(std::memory_order_acquire)) {                                      \
         const int _settle_rc = onmf_settle_pending(ctx);                                         \
         if (_settle_rc != ONMF_OK) return _settle_rc;                                            \
     }

@@ -77,3 +77,69 @@ def test_steps_and_training_take_a_packed_dictionary(torch):
         W2, (A2, B2), _ = nmf.train_dict()
         out.append((H, A, B, W1, W2, A2, B2, surrogate_loss(W, A, B)))
     assert all(np.array_equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("hug", [False, True])
+def test_threads_that_find_a_step_not_waited_for(torch, hug):
+    """Four threads, streams of their own, call at once while a deferred step's verdicts have not been looked at - with a
+    tolerance that no sweep's bounds decide its solve is run again there: once, and to the same bits."""
+    import threading
+    from onmf_ontf_ndl_amd import _lib
+    from onmf_ontf_ndl_amd.engine import get_engine
+    eng = get_engine()
+    d, r, b = 200, 64, 3000
+    g = torch.Generator(device=eng.device).manual_seed(3)
+    X, W = torch.rand(d, b, device=eng.device, generator=g), torch.rand(d, r, device=eng.device, generator=g)
+    W = W / torch.linalg.norm(W, dim=0).clamp(min=1)
+    Y = torch.rand(d, 300, device=eng.device, generator=g)
+    P = eng.dict4_pack(W.contiguous(), 64)
+    A, B = eng.zeros(r, r), eng.zeros(r, d)
+    tol = 0.01
+    if hug:
+        eng.set_option(_lib.OPT_EXACT_STOP, 1)
+        _, _, dist = eng.sparse_code(X, W, seed=5, stopping_diff=0.0)
+        eng.set_option(_lib.OPT_EXACT_STOP, 0)
+        tol = float(dist[5] * 0.995)
+    def step(defer):
+        return eng.step(X, A, B, None, W, 0.5, seed=5, stopping_diff=tol, defer=defer)
+    want = step(False)
+    corr, kept = eng.dict4_correlate(P, Y), eng.keep8(Y)
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(start):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                start.wait()
+                for _ in range(3):
+                    c, k = eng.dict4_correlate(P, Y), eng.keep8(Y)
+                    stream.synchronize()
+                    if not (torch.equal(c, corr) and torch.equal(k.codes, kept.codes)):
+                        wrong.append("a result")
+                try:
+                    eng.dict4_correlate(P, Y[:5])
+                    wrong.append("no refusal")
+                except ValueError:
+                    pass
+        except Exception as e:                                  # (a thread's exception would be lost)
+            wrong.append(e)
+    eng.set_option(_lib.OPT_DEFER_VERDICT, 1)
+    try:
+        for _ in range(4):
+            before = eng.counters()
+            got = step(True)
+            start = threading.Barrier(4)
+            threads = [threading.Thread(target=work, args=(start,)) for _ in range(4)]
+            for th in threads:
+                th.start()
+            for th in threads:
+                th.join()
+            eng.settle()
+            torch.cuda.synchronize()
+            after = eng.counters()
+            assert not wrong, wrong
+            assert after["sweeps_total"] - before["sweeps_total"] == want[5]
+            assert all(torch.equal(got[i], want[i]) for i in (0, 1, 2, 4))
+    finally:
+        eng.set_option(_lib.OPT_DEFER_VERDICT, 0)
