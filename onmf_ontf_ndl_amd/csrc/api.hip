@@ -28,8 +28,14 @@ int onmf_fail(onmf_ctx* c, int code, const char* fmt, ...) {
     va_start(ap, fmt);
     vsnprintf(buf, sizeof(buf), fmt, ap);
     va_end(ap);
-    if (c) c->err = buf; else g_create_error = buf;
+    if (c) onmf_note(c, buf);
+    else g_create_error = buf;
     return code;
+}
+
+void onmf_note(onmf_ctx* c, const char* text) {
+    std::lock_guard<std::mutex> guard(c->err_lock);
+    snprintf(c->err, sizeof(c->err), "%s", text);
 }
 
 int onmf_reserve(onmf_ctx* c, DevBuf& b, size_t bytes, const char* what) {
@@ -184,7 +190,7 @@ int onmf_destroy(onmf_ctx* c) {
     return ONMF_OK;
 }
 
-const char* onmf_last_error(onmf_ctx* c) { return c ? c->err.c_str() : g_create_error.c_str(); }
+const char* onmf_last_error(onmf_ctx* c) { return c ? c->err : g_create_error.c_str(); }
 
 int onmf_set_option(onmf_ctx* c, int key, int value) {
     if (!c) return ONMF_ERR_ARG;
@@ -653,8 +659,8 @@ static int sparse_code_impl(onmf_ctx* c, int d, int r, int b, const float* X, in
                         ++c->n_sweep_timeouts;
                         c->persistent_backoff = c->persistent_backoff ? std::min(c->persistent_backoff * 2, 1 << 20) : 64;
                         c->persistent_hold = c->persistent_backoff;
-                        c->err = "sparse_code: a sweep workgroup gave up waiting for the others (grid not resident "
-                                 "as a whole?); solves run with one launch per sweep for a while";
+                        onmf_note(c, "sparse_code: a sweep workgroup gave up waiting for the others (grid not resident "
+                                     "as a whole?); solves run with one launch per sweep for a while");
                         const bool start_intact = H0 == nullptr || (H0 != buf[0] && H0 != buf[1] && H0 != buf[2]);
                         if (!second_try && start_intact)
                             return sparse_code_impl(c, d, r, b, X, ldx, W, H0, seed, alpha, sub_iter, stopping_diff,
@@ -940,8 +946,8 @@ static int dict_check(onmf_ctx* c, int d, int r, const float* W_in, const float*
         ONMF_TRY(launch_transpose(r, d, wt, W_out, s));
         src = W_out;
     }
-    c->err = "update_dict: a workgroup gave up waiting for the others (not co-resident?); the pass was redone "
-             "atom by atom";
+    onmf_note(c, "update_dict: a workgroup gave up waiting for the others (not co-resident?); the pass was redone "
+                 "atom by atom");
     return launch_dict_pass_serial(c, d, r, src, A, B, W_out, s);
 }
 

@@ -44,7 +44,9 @@ struct PendingSolve {
 
 struct onmf_ctx {
     int device = 0;
-    std::string err;
+    // the last failure's text: of a fixed size, so that one thread may read it while another fails
+    char err[1024] = "";
+    std::mutex err_lock;
     DevBuf slab;        // split-K partial products
     DevBuf cm;          // Cm = W^T X  (r x b)
     DevBuf gram;        // Gm = W^T W  (r x r)
@@ -153,6 +155,7 @@ int onmf_settle_pending(onmf_ctx* c);
     }
 
 int onmf_fail(onmf_ctx* c, int code, const char* fmt, ...);
+void onmf_note(onmf_ctx* c, const char* text);      // what onmf_last_error says from now on
 int onmf_reserve(onmf_ctx* c, DevBuf& b, size_t bytes, const char* what);
 int onmf_reserve_pinned(onmf_ctx* c, size_t bytes);
 

@@ -122,6 +122,8 @@ def test_threads_that_find_a_step_not_waited_for(torch, hug):
                     wrong.append("no refusal")
                 except ValueError:
                     pass
+                if eng.lib.onmf_keep8(eng.ctx, 1, 1, None, 0, 1, None, None, None) != -1 or not eng.lib.onmf_last_error(eng.ctx):
+                    wrong.append("no error")
         except Exception as e:                                  # (a thread's exception would be lost)
             wrong.append(e)
     eng.set_option(_lib.OPT_DEFER_VERDICT, 1)
