@@ -150,3 +150,54 @@ def test_products_keep_float32s_range(eng, torch, d, r, b, group, size, dtype):
         got, want = host(getattr(eng, call)(P, X)), W @ host(X)
         assert np.isfinite(got).all()
         assert (np.abs(got - want) <= STEP * (K / 4 + 64) * want).all()
+
+
+def one_each(rs, K, b, values):
+    """K x b columns with one entry that is not zero, at a random place; (matrix, places)"""
+    X, at = np.zeros((K, b), dtype=np.float32), rs.randint(K, size=b)
+    X[at, np.arange(b)] = values
+    return X, at
+
+
+@pytest.mark.parametrize("d,r,b,group", PATHS)
+def test_products_use_every_bit_of_a_column(eng, torch, d, r, b, group):
+    """One entry a column, with all of float32's 24 bits, against weights that are powers of two (by q, or by z alone): the
+    result is that entry shifted, whatever pieces it is taken in, so it has to be equal."""
+    rs = np.random.RandomState(d + 2 * r + b)
+    groups = -(-d // group)
+    for by_z in (False, True):
+        q = np.zeros((r, groups * group), dtype=int) if by_z else 2 ** rs.randint(0, 4, size=(r, groups * group))
+        q[:, d:] = 0
+        z = 2 ** rs.randint(3, 8, size=(r, groups)) * rs.choice([-1, 1], size=(r, groups)) if by_z else np.zeros((r, groups), dtype=int)
+        s = 2.0 ** rs.randint(-12, 5, size=(r, groups))
+        P = packed(eng, q, z, s, d, group)
+        W = lo.values4(q, z, s, d)
+        for K, M, call in ((d, W.T, "dict4_correlate"), (r, W, "dict4_product")):
+            x = (rs.randint(2 ** 23, 2 ** 24, size=b) | 1) * rs.choice([-1.0, 1.0], size=b) * 2.0 ** rs.randint(-60, 20, size=b)
+            X, at = one_each(rs, K, b, x)
+            assert np.array_equal(host(getattr(eng, call)(P, eng.dev(X))), M[:, at] * x)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d,r,b,group", PATHS)
+def test_products_use_every_bit_of_a_weight(eng, torch, d, r, b, group, dtype):
+    """Weights of 16 bits, s (q + z) = 129 * 255 2^e.  One entry a column: of 9 bits in float32, 257, which makes 24 bits and
+    needs the weight's lower half times the entry's second piece, or 1 in bfloat16 - both exact.  And any entry, within three
+    roundings or cuts of 2^-23 of the product and one of the scale, where what is left out (2^-25) has its place too."""
+    rs = np.random.RandomState(d + 3 * r + b)
+    groups = -(-d // group)
+    q = np.full((r, groups * group), 15)
+    q[:, d:] = 0
+    z = np.full((r, groups), 240)
+    s = 129 * 2.0 ** rs.randint(-20, 0, size=(r, groups))
+    P = packed(eng, q, z, s, d, group)
+    W = lo.values4(q, z, s, d)
+    for K, M, call in ((d, W.T, "dict4_correlate"), (r, W, "dict4_product")):
+        x = (257.0 if dtype == "float32" else 1.0) * rs.choice([-1.0, 1.0], size=b) * 2.0 ** rs.randint(-10, 10, size=b)
+        X, at = one_each(rs, K, b, x)
+        X = eng.dev(X).bfloat16() if dtype == "bfloat16" else eng.dev(X)
+        assert np.array_equal(host(getattr(eng, call)(P, X)), M[:, at] * x)
+        X, at = one_each(rs, K, b, rs.randn(b))
+        X = eng.dev(X).bfloat16() if dtype == "bfloat16" else eng.dev(X)
+        want = M[:, at] * host(X)[at, np.arange(b)]
+        assert (np.abs(host(getattr(eng, call)(P, X)) - want) <= 4 * STEP * np.abs(want)).all()
