@@ -1004,7 +1004,8 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
 // Whole digits take three launches, of which the last, for what they do not hold, mostly ends at once.  Measured (us of the
 // whole gradient, n=500, digits and the double pipe): d r^2 = 2.7e8, d=4096 r=256 34 and 31; 4.3e8 and 4.5e8, d=1200 r=600 41.0 and
 // 40.5, d=4096 r=330 47.7 and 46.5; 5.4e8, d=2048 r=512 40 and 43; 6.3e8, d=600 r=1024 46 and 55; 4.3e9, d=4096 r=1024 94 and 204.
-bool by_digits(int d, int r) { return r <= MOST_DIGIT_ROWS && (double)d * r * r > 4e8; }
+// With few features cutting A takes longer than the product: d=200 r=1500 57 and 56, d=100 r=2050 82 and 67, d=32 r=4096 167 and 92.
+bool by_digits(int d, int r) { return d >= 256 && r <= MOST_DIGIT_ROWS && (double)d * r * r > 4e8; }
 int digit_columns(int r) { return (r + 63) & ~63; }
 // Rows and columns of a workgroup's tile
 int digit_tile(int d, int r) { return (long long)((r + 127) / 128) * ((d + 127) / 128) >= 256 ? 128 : 64; }

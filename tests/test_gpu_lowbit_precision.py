@@ -51,7 +51,7 @@ def test_gradient_at_the_least_squares_dictionary(eng, torch, d, r, n):
 
 
 @pytest.mark.parametrize("d,r,n", [(700, 256, 500), (4100, 300, 400), (4100, 330, 400), (6000, 640, 300), (1300, 1030, 700),
-                                   (150, 2050, 300)])
+                                   (150, 2050, 300), (260, 2050, 300)])
 @pytest.mark.parametrize("kind", ["even", "dead", "rescaled", "apart", "signed", "dominated"])
 def test_gradient_holds_the_terms_that_are_summed(eng, torch, d, r, n, kind):
     """W (H H^T) in double or in whole digits, whichever a size takes: an entry is off by at most half a float32 step of itself
