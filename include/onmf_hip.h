@@ -359,7 +359,7 @@ int onmf_numpy_rand(onmf_ctx* ctx, const uint32_t* key, int pos, size_t n, float
  *   product    R = W H (d x b): np.dot(self.W, code), image_reconstruction.py:352, :385
  * Each is the other's gradient: dL/dX = W dL/dC, dL/dH = W^T dL/dR.
  * A result is within float32's roundings where the magnitudes that are added up, s (q + |z|) |x|, have a sum that float32
- * holds and |x| is 2^-100 or more of the values that count.  A column with a NaN or an infinity (or a float32 within 2^-8
+ * holds and the |x| that count in it are 2^-100 or more.  A column with a NaN or an infinity (or a float32 within 2^-8
  * of the largest one) has NaNs or infinities in its result and touches no other column.  ws: at least onmf_dict4_workspace(which, d, r, b, group) bytes of device
  * memory, aligned to 16, in use until the call's work on `stream` is done (so calls on different streams take
  * different ones).  d <= 2^18; results may not overlap what is read.  Asynchronous on `stream`, allocates nothing and

@@ -200,9 +200,11 @@ __global__ __launch_bounds__(256) void keep8_gather_kernel(int d, int n, int gro
 // meet every bank once.  Rows behind the last one read the last row's codes; what they give is not stored.
 // In float32 H's scale is multiplied to the whole sum and X's with the addition: the two scales' own product may lie beyond
 // what float32 holds where the sum does not, and that would make zeros NaN.
-// Per group and output three vector instructions (conversion, product with a scale, fused multiply-add) stand
-// against 1/256 of a matrix instruction: the vector pipe is the bound where memory is not
-// (d=4096 r=256 n=65536, 146 GOP: 125 us, PRECISE 145 and the slabs' 62 MB; d=1024 40 us).
+// Per group and output three vector instructions (conversion, product with a scale, fused multiply-add) stand against 1/256 of
+// a matrix instruction.  Where memory is not the bound, three pipes are, in turn: of a group of a 128 x 256 tile the operands
+// are 192 KB from LDS (0.64 us at 128 B a cycle), 1536 vector instructions (0.64 us) and 8.4 MOP (0.43 us), and all waves pass one
+// barrier a group, which was measured to take 1.7 us, their sum (d=4096 r=256 n=65536, 146 GOP: 125 us, PRECISE 145 and the
+// slabs' 62 MB; d=1024 40 us).
 template <int MI, int NJ, int WM_, int WN_, int STAGES> struct Tile {
     static constexpr int mi = MI, nj = NJ, wm = WM_, wn = WN_, stages = STAGES;
     static constexpr int bm = 16 * MI * WM_, bn = 16 * NJ * WN_, waves = WM_ * WN_;

@@ -2,7 +2,7 @@
 libonmf_hip.so, the formats are described in include/onmf_hip.h).
 
     P = pack_dictionary(W, group=64)         # W (d x r): an eighth of its room and a little
-    H = nmf.sparse_code(X, P)                # wherever a dictionary is only read
+    H = nmf.sparse_code(X, P)                # wherever a dictionary is read
     P.unpack()                               # the float32 matrix it stands for
 
     K = keep_columns(X)                      # X (d x n): a quarter of its room
