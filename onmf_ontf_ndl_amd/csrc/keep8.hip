@@ -518,16 +518,13 @@ __global__ __launch_bounds__(256) void keep8_reduce_kernel(int d, int r, int col
 // wave loads the double matrix pipe's operands (16x16x4) straight into registers, the next sixteen while these are
 // computed: four neighbours of W a lane, at j = 16 s + 4 (l / 16) + i in the i-th instruction, and rows of A.  Output
 // row 4 e + l / 16.  Bound by the double matrix pipe where r is large (d=4096 r=256 19.5 us; r=1024 182, 47 TFLOP/s).
-// Behind the product by digits (below): only tiles that it marked, and of those only what it left as NaN.
-struct Marks { int* tiles; int rows, cols, across; };        // a mark for `rows` x `cols` of dW, `across` of them side by side
-template <int NW>
-__global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
-                                                                  const double* __restrict__ A, const double* __restrict__ B,
-                                                                  float* __restrict__ dW, Marks marks) {
-    __shared__ double part[NW][32][32], tb[32][33];
+template <int NW> struct GradientLds { double part[NW][32][32], tb[32][33]; };
+template <int NW, bool REST>                          // REST: only entries that are NaN so far
+__device__ __forceinline__ void gradient_tile(GradientLds<NW>& lds, int i0, int k0, int d, int r, const float* __restrict__ W,
+                                              const double* __restrict__ A, const double* __restrict__ B, float* __restrict__ dW) {
+    auto& part = lds.part;
+    auto& tb = lds.tb;
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), m = lane & 15, quad = lane >> 4;
-    const int i0 = blockIdx.y * 32, k0 = blockIdx.x * 32;
-    if (marks.tiles && !marks.tiles[i0 / marks.rows * marks.across + k0 / marks.cols]) return;
     for (int e = t; e < 1024; e += 64 * NW) {
         const int k = k0 + (e >> 5), i = i0 + (e & 31);
         tb[e & 31][e >> 5] = (k < r && i < d) ? B[(size_t)k * d + i] : 0.0;
@@ -586,8 +583,30 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
         for (int z = 1; z < NW; ++z) v += part[z][i][k];
         if (i0 + i >= d || k0 + k >= r) continue;
         float* dst = dW + (size_t)(i0 + i) * r + k0 + k;
-        if (!marks.tiles || *dst != *dst) *dst = (float)(v - tb[i][k]);
+        if (!REST || *dst != *dst) *dst = (float)(v - tb[i][k]);
     }
+}
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, const float* __restrict__ W,
+                                                                  const double* __restrict__ A, const double* __restrict__ B,
+                                                                  float* __restrict__ dW) {
+    __shared__ GradientLds<NW> lds;
+    gradient_tile<NW, false>(lds, blockIdx.y * 32, blockIdx.x * 32, d, r, W, A, B, dW);
+}
+// Behind the product by digits (below): 64 x 64 entries a workgroup, if the mark of their tile is set, and of those what was left
+// as NaN.  (Where none is set, d=8192 r=1024: 5 us; a workgroup for every 32 x 32 8.6.)
+constexpr int LEFT = 64;
+__global__ __launch_bounds__(256) void keep8_left_kernel(int d, int r, const float* __restrict__ W, const double* __restrict__ A,
+                                                          const double* __restrict__ B, float* __restrict__ dW,
+                                                          const int* __restrict__ marks, int tile, int across) {
+    __shared__ GradientLds<4> lds;
+    const int i1 = blockIdx.y * LEFT, k1 = blockIdx.x * LEFT;
+    if (!marks[i1 / tile * across + k1 / tile]) return;
+    for (int i0 = i1; i0 < min(d, i1 + LEFT); i0 += 32)
+        for (int k0 = k1; k0 < min(r, k1 + LEFT); k0 += 32) {
+            gradient_tile<4, true>(lds, i0, k0, d, r, W, A, B, dW);
+            __syncthreads();
+        }
 }
 
 // The same on the 8-bit matrix pipe, where r is large.  Atoms are balanced first, by c_j = 2^floor(log2(A_jj) / 2): the terms
@@ -601,68 +620,75 @@ __global__ __launch_bounds__(64 * NW) void keep8_gradient_kernel(int d, int r, c
 // where that is at most 2^-25 (|W A| + |B|), half a float32 step of the terms; where it is not - a row's small terms count because
 // its large ones meet zeros of A or cancel - it is left as NaN and its tile marked, for the double pipe to compute anew.  So
 // every entry depends on its own row and column alone.  Bound by the matrix pipe (d=4096 r=1024: the thirteen products 55 us,
-// 2.0 POP/s, the digits 19, the look at the marks 5; on the double matrix pipe 182.  Where nothing is held, a dictionary of both
-// signs or codes that never meet, both are run: 282 us of the whole gradient instead of 105).
+// 2.0 POP/s, the digits 10, the look at the marks 4.5; on the double matrix pipe 182.  Where nothing is held, a dictionary of both
+// signs or codes that never meet, both are run: 280 us of the whole gradient instead of 84).
 constexpr int DIGITS = 4, SUMS = 5;
 constexpr int MOST_DIGIT_ROWS = 32767;           // 4 products of 128 x 128 add up below 2^31
 
 // c_j of A_jj as a power of two; 0 for an atom without code, 1 for one that is not finite (its row of A says so)
 __device__ __forceinline__ double balance(double diag, bool inverse) {
+    const int hi = __double2hiint(diag);              // (a sum of squares of scales is no subnormal number and not negative)
     if (diag == 0.0) return inverse ? 1.0 : 0.0;
-    if (!(diag <= 1.7976931348623157e308)) return 1.0;
-    const int c = (int)((__double_as_longlong(diag) >> 52) - 1023) >> 1;     // (a sum of squares of scales is no subnormal number)
-    return __longlong_as_double((long long)(1023 + (inverse ? -c : c)) << 52);
+    if (hi >= 0x7ff00000) return 1.0;
+    const int c = ((hi >> 20) - 1023) >> 1;
+    return __hiloint2double((1023 + (inverse ? -c : c)) << 20, 0);
 }
 
 // digits[t][row][kp], zeros behind column r, the powers of two and the sums of magnitudes: W's d rows, then A's r; a wave a
-// row.  The product's marks are taken back.
+// row, whose first 1024 entries are held in registers between finding the power and cutting.  The product's marks are
+// taken back.  Bound by its vector instructions and the reading of W and A (d=4096 r=1024, 46 MB: 10 us).
 __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp, const float* __restrict__ W,
                                                             const double* __restrict__ A, const double* __restrict__ diag,
                                                             int8_t* __restrict__ digits, double* __restrict__ powers,
                                                             double* __restrict__ sums, int* __restrict__ marks, int n_marks) {
+    constexpr int HELD = 4;
     for (int e = blockIdx.x * 256 + threadIdx.x; e < n_marks; e += gridDim.x * 256) marks[e] = 0;
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= d + r) return;
     // four neighbours, balanced (those behind column r - 1 are zeros)
-    bool fine = true;
     auto values = [&](int k, double (&v)[4]) {
         auto take = [&](const auto* src, bool inverse) {
+            typedef std::remove_cv_t<std::remove_reference_t<decltype(*src)>> V;
+            typedef V V4 __attribute__((ext_vector_type(4), aligned(sizeof(V))));
+            typedef double D4 __attribute__((ext_vector_type(4), aligned(8)));
             if (k + 4 <= r) {
-                typedef std::remove_cv_t<std::remove_reference_t<decltype(*src)>> V;
-                typedef V V4 __attribute__((ext_vector_type(4), aligned(sizeof(V))));
                 const V4 x = *reinterpret_cast<const V4*>(src + k);
+                const D4 c = *reinterpret_cast<const D4*>(diag + k);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = (double)x[j];
+                for (int j = 0; j < 4; ++j) v[j] = (double)x[j] * balance(c[j], inverse);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = k + j < r ? (double)src[k + j] : 0.0;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                fine = fine && fabs(v[j]) <= 1.7976931348623157e308;
-                v[j] *= balance(diag[min(k + j, r - 1)], inverse);
+                for (int j = 0; j < 4; ++j) v[j] = k + j < r ? (double)src[k + j] * balance(diag[k + j], inverse) : 0.0;
             }
         };
         if (row < d) take(W + (size_t)row * r, false);
         else take(A + (size_t)(row - d) * r, true);
     };
-    double most = 0.0, sum = 0.0;
-#pragma unroll 4
-    for (int k = lane * 4; k < r; k += 256) {
-        double v[4];
-        values(k, v);
+    double most = 0.0, sum = 0.0, held[HELD][4];
+    auto look = [&](const double (&v)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             most = fmax(most, fabs(v[j]));
             sum += fabs(v[j]);
         }
+    };
+#pragma unroll
+    for (int q = 0; q < HELD; ++q)
+        if (lane * 4 + 256 * q < r) {
+            values(lane * 4 + 256 * q, held[q]);
+            look(held[q]);
+        }
+    for (int k = lane * 4 + 256 * HELD; k < r; k += 256) {
+        double v[4];
+        values(k, v);
+        look(v);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         most = fmax(most, __shfl_xor(most, o, 64));
         sum += __shfl_xor(sum, o, 64);
     }
-    fine = __all(fine);
+    const bool fine = sum <= 1.7976931348623157e308;  // (a NaN or an infinity anywhere is in the sum)
     int e = 0;                                        // most <= 127/128 2^e: the first digit is at most 127
     if (fine && frexp(most, &e) > 127.0 / 128.0) ++e;
     if (lane == 0) {
@@ -671,25 +697,32 @@ __global__ __launch_bounds__(256) void keep8_digits_kernel(int d, int r, int kp,
     }
     const double scale = fine ? ldexp(1.0, 31 - e) : 0.0;
     const size_t plane = (size_t)(d + r) * kp;
-#pragma unroll 2
-    for (int k = lane * 4; k < kp; k += 256) {
+    auto cut = [&](int k, const double (&v)[4]) {
+        // N's digits of 8 bits with their signs: with a half of each but the first added the carries are where they
+        // belong, and the bytes' upper bits the other way round are the digits
+        uint32_t n[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n[j] = fine ? ((uint32_t)(int)rint(v[j] * scale) + 0x00808080u) ^ 0x00808080u : 0u;
+#pragma unroll
+        for (int t = 0; t < DIGITS; ++t) {
+            const uint32_t at = 3 - t, pick = at | (4 + at) << 8 | 0x0c0c0000u;      // byte `at` of both (12: zero)
+            const uint32_t lo = __builtin_amdgcn_perm(n[1], n[0], pick), hi = __builtin_amdgcn_perm(n[3], n[2], pick);
+            *reinterpret_cast<uint32_t*>(digits + t * plane + (size_t)row * kp + k) = lo | hi << 16;
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < HELD; ++q) {
+        const int k = lane * 4 + 256 * q;
+        if (k >= kp) continue;
+        if (k >= r)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) held[q][j] = 0.0;
+        cut(k, held[q]);
+    }
+    for (int k = lane * 4 + 256 * HELD; k < kp; k += 256) {
         double v[4];
         values(k, v);
-        uint32_t word[DIGITS];
-#pragma unroll
-        for (int t = 0; t < DIGITS; ++t) word[t] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            int x = fine ? (int)rint(v[j] * scale) : 0;
-#pragma unroll
-            for (int t = DIGITS - 1; t >= 0; --t) {
-                const int q = t > 0 ? (int)(int8_t)(x & 0xff) : x;
-                x = (x - q) >> 8;
-                word[t] |= ((uint32_t)q & 0xff) << (8 * j);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < DIGITS; ++t) *reinterpret_cast<uint32_t*>(digits + t * plane + (size_t)row * kp + k) = word[t];
+        cut(k, v);
     }
 }
 
@@ -1004,10 +1037,10 @@ int run_sums(onmf_ctx* c, const SumPlan& q, int d, int r, int n, const int8_t* x
 }
 
 // Whole digits take three launches, of which the last, for what they do not hold, mostly ends at once.  Measured (us of the
-// whole gradient, n=500, digits and the double pipe): d r^2 = 2.7e8, d=4096 r=256 34 and 31; 4.3e8 and 4.5e8, d=1200 r=600 41.0 and
-// 40.5, d=4096 r=330 47.7 and 46.5; 5.4e8, d=2048 r=512 40 and 43; 6.3e8, d=600 r=1024 46 and 55; 4.3e9, d=4096 r=1024 94 and 204.
-// With few features cutting A takes longer than the product: d=200 r=1500 57 and 56, d=100 r=2050 82 and 67, d=32 r=4096 167 and 92.
-bool by_digits(int d, int r) { return d >= 256 && r <= MOST_DIGIT_ROWS && (double)d * r * r > 4e8; }
+// whole gradient, n=500, digits and the double pipe): d r^2 = 2.7e8, d=4096 r=256 31.6 and 30.5; 4.3e8 and 4.5e8, d=1200 r=600 37.7
+// and 39.7, d=4096 r=330 42 and 46; 5.4e8, d=2048 r=512 36.5 and 42.5; 6.3e8, d=600 r=1024 41 and 54; 4.3e9, d=4096 r=1024 84 and 200.
+// With few features cutting A takes longer than the product: d=200 r=1500 48 and 56, d=100 r=2050 68 and 66, d=32 r=4096 147 and 92.
+bool by_digits(int d, int r) { return d >= 128 && r <= MOST_DIGIT_ROWS && (double)d * r * r > 4e8; }
 int digit_columns(int r) { return (r + 63) & ~63; }
 // Rows and columns of a workgroup's tile
 int digit_tile(int d, int r) { return (long long)((r + 127) / 128) * ((d + 127) / 128) >= 256 ? 128 : 64; }
@@ -1015,51 +1048,55 @@ struct DigitSpace {
     int8_t* digits;                // [DIGITS][d + r][digit_columns]
     double *powers, *sums;         // [d + r]
     double* diag;                  // [r]
-    Marks marks;
+    int* marks;                    // [(d + tile - 1) / tile][(r + tile - 1) / tile]
+    int tile, n_marks;
     size_t bytes;
     DigitSpace(int d, int r, char* ws) {
-        const int tile = digit_tile(d, r);
+        tile = digit_tile(d, r);
+        n_marks = ((d + tile - 1) / tile) * ((r + tile - 1) / tile);
         const size_t planes = ((size_t)DIGITS * ((size_t)d + r) * digit_columns(r) + 255) & ~(size_t)255;
         digits = (int8_t*)ws;
         powers = (double*)(ws + planes);
         sums = powers + d + r;
         diag = sums + d + r;
-        marks = Marks{(int*)(diag + r), tile, tile, (r + tile - 1) / tile};
-        bytes = planes + sizeof(double) * (2 * ((size_t)d + r) + r) + sizeof(int) * (size_t)marks_count(d);
+        marks = (int*)(diag + r);
+        bytes = planes + sizeof(double) * (2 * ((size_t)d + r) + r) + sizeof(int) * (size_t)n_marks;
     }
-    int marks_count(int d) const { return marks.across * ((d + marks.rows - 1) / marks.rows); }
 };
 size_t digits_bytes(int d, int r) { return by_digits(d, r) ? DigitSpace(d, r, nullptr).bytes : 0; }
 template <int MI, int NJ, int WM, int WN>
-int launch_digit_product(onmf_ctx* c, int d, int r, const DigitSpace& q, const double* B, float* dW, hipStream_t s) {
+int launch_digit_product(onmf_ctx* c, int d, int r, const DigitSpace& q, const float* W, const double* A, const double* B, float* dW,
+                         hipStream_t s) {
     constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
-    static_assert(BM == BN, "a mark is a square");
+    static_assert(BM == BN && BM % LEFT == 0, "a mark is a square");
     constexpr size_t bytes = 2 * (size_t)DIGITS * (BM + BN) * 64;
     static LdsLimit lim;
     ONMF_TRY(onmf_raise_lds_limit(c, lim, (const void*)keep8_digit_product_kernel<MI, NJ, WM, WN>, bytes));
-    hipLaunchKernelGGL((keep8_digit_product_kernel<MI, NJ, WM, WN>), dim3((r + BM - 1) / BM, (d + BN - 1) / BN), dim3(64 * WM * WN),
-                       bytes, s, d, r, digit_columns(r), q.digits, q.powers, q.sums, B, dW, q.marks.tiles);
+    const dim3 grid((r + BM - 1) / BM, (d + BN - 1) / BN);
+    hipLaunchKernelGGL((keep8_digit_product_kernel<MI, NJ, WM, WN>), grid, dim3(64 * WM * WN), bytes, s, d, r, digit_columns(r), q.digits,
+                       q.powers, q.sums, B, dW, q.marks);
+    HIP_TRY(c, hipGetLastError());
+    hipLaunchKernelGGL(keep8_left_kernel, dim3((r + LEFT - 1) / LEFT, (d + LEFT - 1) / LEFT), dim3(256), 0, s, d, r, W, A, B, dW, q.marks, BM,
+                       (int)grid.x);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
 int launch_gradient(onmf_ctx* c, int d, int r, const float* W, const double* A, const double* B, float* dW, char* ws, hipStream_t s) {
-    Marks marks = {nullptr, 1, 1, 1};
     if (by_digits(d, r)) {
         const DigitSpace q(d, r, ws);
         hipLaunchKernelGGL(keep8_digits_kernel, dim3((d + r + 3) / 4), dim3(256), 0, s, d, r, digit_columns(r), W, A, q.diag, q.digits,
-                           q.powers, q.sums, q.marks.tiles, q.marks_count(d));
+                           q.powers, q.sums, q.marks, q.n_marks);
         HIP_TRY(c, hipGetLastError());
-        if (q.marks.rows == 128) ONMF_TRY((launch_digit_product<4, 2, 2, 4>(c, d, r, q, B, dW, s)));
-        else ONMF_TRY((launch_digit_product<2, 2, 2, 2>(c, d, r, q, B, dW, s)));
-        marks = q.marks;
+        if (q.tile == 128) return launch_digit_product<4, 2, 2, 4>(c, d, r, q, W, A, B, dW, s);
+        return launch_digit_product<2, 2, 2, 2>(c, d, r, q, W, A, B, dW, s);
     }
     const dim3 grid((r + 31) / 32, (d + 31) / 32);
     // (more waves a tile where there are few tiles and enough of j: d=215 r=1017 15.3 us, with four waves 28; with many
     // tiles the double matrix pipe is what counts: d=8192 r=256 36 us, with eight waves 42)
     if (r > 64 && (size_t)grid.x * grid.y <= 512)
-        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, A, B, dW, marks);
+        hipLaunchKernelGGL(keep8_gradient_kernel<8>, grid, dim3(512), 0, s, d, r, W, A, B, dW);
     else
-        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, A, B, dW, marks);
+        hipLaunchKernelGGL(keep8_gradient_kernel<4>, grid, dim3(256), 0, s, d, r, W, A, B, dW);
     HIP_TRY(c, hipGetLastError());
     return ONMF_OK;
 }
